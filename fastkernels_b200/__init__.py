@@ -17,6 +17,7 @@ from .moe import (
     qwen36_single_expert_mlp_decode,
     synthetic_qwen36_moe_decode,
 )
+from .kv_cache import PagedKVCache, paged_attention, paged_kv_append, paged_kv_gather
 
 __all__ = [
     "MoESpec", "MoEWeights", "moe_weights_tuple", "qwen36_35b_a3b_spec", "synthetic_qwen36_spec",
@@ -25,4 +26,5 @@ __all__ = [
     "qwen36_batched_routed_experts_decode", "qwen36_batched_routed_shared_experts_decode",
     "qwen36_moe_decode", "qwen36_moe_router_decode", "qwen36_routed_experts_decode",
     "qwen36_routed_shared_experts_decode", "qwen36_single_expert_mlp_decode", "synthetic_qwen36_moe_decode",
+    "PagedKVCache", "paged_attention", "paged_kv_append", "paged_kv_gather",
 ]

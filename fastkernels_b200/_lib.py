@@ -12,7 +12,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libfkmoe.so"
 
-FK_F32, FK_BF16, FK_F16 = 0, 1, 2
+FK_F32, FK_BF16, FK_F16, FK_E4M3 = 0, 1, 2, 3
 FLAG_FORCE_GENERIC = 1
 FLAG_FORCE_GEMV = 2
 FLAG_FORCE_TENSOR = 4
@@ -54,6 +54,30 @@ class EpComm(C.Structure):          # struct fk_ep_comm
                 ("base", C.c_void_p * EP_MAX_RANKS), ("bytes", C.c_size_t)]
 
 
+MAX_HEAD_DIM = 256
+
+
+class KvCache(C.Structure):         # struct fk_kv_cache
+    _fields_ = [("pages", C.c_int32), ("kv_heads", C.c_int32), ("page_size", C.c_int32), ("head_dim", C.c_int32),
+                ("dtype", C.c_int32), ("seqs", C.c_int32), ("max_pages", C.c_int32), ("reserved", C.c_int32),
+                ("table_stride", C.c_int64), ("key_stride", C.c_int64 * 3), ("value_stride", C.c_int64 * 3),
+                ("key_scale_stride", C.c_int64 * 3), ("value_scale_stride", C.c_int64 * 3),
+                ("key", C.c_void_p), ("value", C.c_void_p), ("key_scale", C.c_void_p), ("value_scale", C.c_void_p),
+                ("page_table", C.c_void_p), ("lengths", C.c_void_p)]
+
+
+class KvRows(C.Structure):          # struct fk_kv_rows
+    _fields_ = [("key", C.c_void_p), ("value", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_int32), ("zero_rest", C.c_int32),
+                ("reserved", C.c_int32), ("key_stride", C.c_int64 * 2), ("value_stride", C.c_int64 * 2), ("starts", C.c_void_p)]
+
+
+class AttentionCall(C.Structure):   # struct fk_attention_call
+    _fields_ = [("cache", KvCache), ("query", C.c_void_p), ("out", C.c_void_p), ("dtype", C.c_int32), ("rows", C.c_int32),
+                ("q_heads", C.c_int32), ("max_query", C.c_int32), ("query_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2),
+                ("starts", C.c_void_p), ("scale", C.c_float), ("window", C.c_int32), ("sinks", C.c_int32), ("zero_rest", C.c_int32),
+                ("flags", C.c_uint32), ("reserved", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 # name -> (restype, argtypes); every symbol include/fkmoe.h declares
 SIGNATURES = {
     "fk_version": (C.c_int, []),
@@ -88,6 +112,10 @@ SIGNATURES = {
     "fk_ep_status": (C.c_int, [C.POINTER(EpComm), C.POINTER(C.c_int)]),
     "fk_ep_buffer_reset": (C.c_int, [C.c_void_p]),
     "fk_moe_layer_ep_timed": (C.c_int, [C.POINTER(Call), C.POINTER(EpComm), C.c_void_p, C.POINTER(C.c_float), C.POINTER(C.c_int)]),
+    "fk_kv_append": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvRows), C.c_void_p]),
+    "fk_kv_gather": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvRows), C.c_void_p]),
+    "fk_paged_attention_workspace_bytes": (C.c_size_t, [C.POINTER(AttentionCall)]),
+    "fk_paged_attention": (C.c_int, [C.POINTER(AttentionCall), C.c_void_p]),
     "fk_set_wait_limit_cycles": (C.c_int, [C.c_longlong]),
     "fk_moe_status": (C.c_int, [C.c_void_p, C.c_size_t, C.POINTER(C.c_int)]),
 }

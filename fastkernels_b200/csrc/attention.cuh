@@ -1,0 +1,97 @@
+// Paged attention: what its kernels share.
+#pragma once
+
+#include "kv_cache.cuh"
+
+namespace fk {
+
+struct AttnParams {
+    fk_kv_cache c;
+    const void* query;
+    void* out;
+    const int* starts;
+    int64_t qs[2], os[2];      // row, head
+    int rows, q_heads, group;  // group = query heads per key/value head
+    int window, sinks, zero_rest;
+    float scale_log2;          // scale * log2(e): scores are held as powers of two
+    int splits;                // pieces of the key axis (shape-agnostic kernel)
+    float* part;               // partial results
+    int blocks;                // grid of the kernels that deal key tiles evenly
+};
+
+// What a token at position p sees: [0, min(sinks, lo)) and [lo, p], lo = first position of its window.
+__device__ __forceinline__ int window_start(const AttnParams& p, int pos) { return p.window > 0 && pos >= p.window ? pos - p.window + 1 : 0; }
+
+__device__ __forceinline__ float load_elem(const float* p) { return *p; }
+__device__ __forceinline__ float load_elem(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ float load_elem(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load_elem(const __nv_fp8_e4m3* p) { return (float)*p; }
+__device__ __forceinline__ void store_elem(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_elem(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_elem(__half* p, float v) { *p = __float2half_rn(v); }
+
+// The sums of one row over some keys, held by a warp: lane l has the elements l, l + 32, ... of acc.
+struct RowSums {
+    float m, l;
+    float acc[FK_MAX_HEAD_DIM / 32];
+};
+
+// One warp, one query row (fp32 in shared memory, already scaled by scale * log2 e): keys first, first + step, ... groups of 32
+// of the `count` visible ones.  One lane computes one key's score (no reduction per key); then the value rows are added one at
+// a time, a lane per column.  Keys that are masked never enter any sum, whatever their rows hold.
+template <typename TC, bool WIDE>
+__device__ __forceinline__ void warp_row(const AttnParams& p, const float* q, int seq, int head, int pos, int first, int step, RowSums& r) {
+    const int lane = threadIdx.x & 31, D = p.c.head_dim;
+    const int end = min(pos + 1, p.c.max_pages * p.c.page_size);       // positions that the table does not hold are not visible
+    const int lo = window_start(p, pos), n_sinks = max(0, min(p.sinks, min(lo, end)));
+    const int count = n_sinks + max(0, end - lo);
+    r.m = -INFINITY;
+    r.l = 0.f;
+#pragma unroll
+    for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] = 0.f;
+    const TC* keys = reinterpret_cast<const TC*>(p.c.key) + head * p.c.key_stride[1];
+    const TC* values = reinterpret_cast<const TC*>(p.c.value) + head * p.c.value_stride[1];
+    for (int64_t k0 = (int64_t)first * 32; k0 < count; k0 += (int64_t)step * 32) {
+        const int k = (int)k0 + lane;
+        int in_page = 0, page = -1;
+        if (k < count) page = page_of(p.c, seq, k < n_sinks ? k : lo + k - n_sinks, in_page);
+        float s = -INFINITY, vscale = 1.f;
+        int64_t voff = 0;
+        if (page >= 0) {
+            const TC* row = keys + page * p.c.key_stride[0] + in_page * p.c.key_stride[2];
+            voff = page * p.c.value_stride[0] + in_page * p.c.value_stride[2];
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int d = 0; d < D; d += 8) {
+                float v[8];
+                load8<WIDE>(row + d, D - d, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[i & 3] = fmaf(q[d + i], v[i], sum[i & 3]);
+            }
+            s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if (sizeof(TC) == 1) {
+                s *= p.c.key_scale[row_offset(p.c.key_scale_stride, page, head, in_page)];
+                vscale = p.c.value_scale[row_offset(p.c.value_scale_stride, page, head, in_page)];
+            }
+        }
+        const unsigned seen = __ballot_sync(kFull, page >= 0);
+        if (seen == 0) continue;
+        const float m = fmaxf(r.m, warp_max(s));
+        const float base = m == -INFINITY ? 0.f : m;        // nothing but scores of -infinity so far
+        const float alpha = exp2f(r.m - base);
+        const float w = page >= 0 ? exp2f(s - base) : 0.f;
+        r.m = m;
+        r.l = r.l * alpha + warp_sum(w);
+#pragma unroll
+        for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] *= alpha;
+        for (int i = 0; i < 32; ++i) {
+            const int64_t off = __shfl_sync(kFull, voff, i);
+            const float wi = __shfl_sync(kFull, w * vscale, i);
+            if (!((seen >> i) & 1u) || wi == 0.f) continue;
+#pragma unroll
+            for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
+                if (c * 32 + lane < D) r.acc[c] = fmaf(wi, load_elem(values + off + c * 32 + lane), r.acc[c]);
+        }
+    }
+}
+
+}  // namespace fk

@@ -1,0 +1,332 @@
+"""Paged key/value cache and the attention that reads it, over libfkmoe.so.
+
+The reference's attention layer appends to one growing key and value tensor and scans it head by head
+(src/fastkernels/kernels/triton/qwen36_attention.py:321-380, src/fastkernels/reference/qwen36_real.py:317-323); pages,
+8-bit storage, windows and ragged batches have no counterpart there.
+
+  paged_kv_append   writes new tokens into the cache, as they are or as e4m3 codes with one scale per token and head
+  paged_kv_gather   reads the last tokens of each sequence back
+  paged_attention   attention of new tokens (one per sequence in decode, chunks in a prompt) over the cache
+  PagedKVCache      one layer's cache with its pages handed out, calling the three
+
+Cache tensors are `[pages, kv_heads, page_size, head_dim]`, any strides with a contiguous last dimension (a cache laid
+out `[pages, page_size, kv_heads, head_dim]` is passed as `.transpose(1, 2)`).  The three functions take the same ragged
+description: `page_table` int32 `[seqs, max_pages]`, `lengths` int32 `[seqs]` counting the new tokens, `query_starts`
+int32 `[seqs + 1]`: rows `query_starts[s] .. query_starts[s+1]-1` of a call are the last tokens of sequence `s`
+(`None`: one token per sequence).  All of it is read on the device; nothing synchronises, so calls can be captured in a
+CUDA graph and replayed with other lengths.  Page numbers outside the cache (-1 for a page that was given back, say)
+are safe: such tokens are skipped, read as zeros, or not visible.  A position must not be mapped to a page that another
+position of the same call writes.  No gradients.
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Any, Optional
+
+import torch
+
+from . import _lib
+from ._lib import AttentionCall, KvCache, KvRows
+from .moe import _DTYPES
+
+_CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.FK_E4M3}
+
+
+def _on(device: torch.device):
+    """Context in which `device` is the current one; the stream to launch on is that device's current stream."""
+    return torch.cuda.device(device)
+
+
+def _check_index(t: Any, what: str, shape: tuple, device: torch.device) -> None:
+    if t.dtype != torch.int32 or t.shape != shape:
+        raise ValueError(f"{what} must be int32 with shape {list(shape)}, got {t.dtype} {list(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} must be on {device}")
+    if shape and shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{what} must be contiguous in its last dimension")
+
+
+def _fill_cache(c: KvCache, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale) -> None:
+    """Checks the description of a cache and a ragged batch, and fills the ABI's struct."""
+    if not key_cache.is_cuda:
+        raise ValueError("key_cache must be a CUDA tensor")
+    if key_cache.ndim != 4 or value_cache.shape != key_cache.shape:
+        raise ValueError("key_cache and value_cache must have the same shape [pages, kv_heads, page_size, head_dim]")
+    device, dtype = key_cache.device, key_cache.dtype
+    if value_cache.device != device or value_cache.dtype != dtype:
+        raise ValueError("key_cache and value_cache must have the same dtype and device")
+    code = _CACHE_DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"the cache must be float32, bfloat16, float16 or float8_e4m3fn, got {dtype}")
+    pages, heads, page_size, dim = key_cache.shape
+    if pages < 1 or heads < 1 or page_size < 1:
+        raise ValueError("the cache must have at least one page, head and row per page")
+    if dim < 1 or dim > _lib.MAX_HEAD_DIM:
+        raise ValueError(f"head_dim must be between 1 and {_lib.MAX_HEAD_DIM}")
+    ks, vs = key_cache.stride(), value_cache.stride()
+    if dim > 1 and (ks[3] != 1 or vs[3] != 1):
+        raise ValueError("key_cache and value_cache must be contiguous in their last dimension")
+    if page_table.ndim != 2:
+        raise ValueError("page_table must have shape [seqs, max_pages]")
+    seqs, max_pages = page_table.shape
+    _check_index(page_table, "page_table", (seqs, max_pages), device)
+    _check_index(lengths, "lengths", (seqs,), device)
+    if max_pages * page_size >= 1 << 31:
+        raise ValueError("page_table must hold less than 2^31 positions per sequence")
+    if query_starts is not None:
+        _check_index(query_starts, "query_starts", (seqs + 1,), device)
+    if dtype == torch.float8_e4m3fn:
+        for name, t in (("key_scale", key_scale), ("value_scale", value_scale)):
+            if t is None:
+                raise ValueError(f"{name} is required with a float8_e4m3fn cache")
+            if t.dtype != torch.float32 or t.shape != key_cache.shape[:3] or t.device != device:
+                raise ValueError(f"{name} must be float32 [pages, kv_heads, page_size] on the cache's device")
+        c.key_scale_stride[:] = key_scale.stride()
+        c.value_scale_stride[:] = value_scale.stride()
+        c.key_scale, c.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
+    elif key_scale is not None or value_scale is not None:
+        raise ValueError("key_scale and value_scale belong to a float8_e4m3fn cache")
+    c.pages, c.kv_heads, c.page_size, c.head_dim, c.dtype = pages, heads, page_size, dim, code
+    c.seqs, c.max_pages, c.table_stride = seqs, max_pages, page_table.stride(0)
+    c.key_stride[:] = ks[:3]
+    c.value_stride[:] = vs[:3]
+    c.key, c.value = key_cache.data_ptr(), value_cache.data_ptr()
+    c.page_table, c.lengths = page_table.data_ptr(), lengths.data_ptr()
+
+
+def _check_rows(t: Any, what: str, rows: Optional[int], heads: int, key_cache) -> None:
+    if t.ndim != 3 or (rows is not None and t.shape[0] != rows) or t.shape[1] != heads or t.shape[2] != key_cache.shape[3]:
+        raise ValueError(f"{what} must have shape [{'rows' if rows is None else rows}, {heads}, {key_cache.shape[3]}], got {list(t.shape)}")
+    if t.device != key_cache.device:
+        raise ValueError(f"{what} must be on the cache's device")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    if key_cache.dtype != torch.float8_e4m3fn and t.dtype != key_cache.dtype:
+        raise ValueError(f"{what} must have the cache's dtype {key_cache.dtype}, got {t.dtype}")
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{what} must be contiguous in its last dimension")
+
+
+def _span(t: Any) -> tuple[int, int]:
+    """First and one-past-last byte that a tensor can touch."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _overlap(a: Any, b: Any) -> bool:
+    """Whether two tensors may touch the same bytes: their spans meet, unless they are interleaved rows of one layout (equal
+    strides, all of them multiples of the smallest, which holds a row of each)."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a0 >= b1 or b0 >= a1:
+        return False
+    if a.shape == b.shape and a.stride() == b.stride() and a.dtype == b.dtype and (b0 - a0) % a.element_size() == 0:
+        steps = [s for n, s in zip(a.shape[:-1], a.stride()[:-1]) if n > 1]
+        least, width = min(steps, default=0), a.shape[-1]
+        if least > 0 and all(s % least == 0 for s in steps):
+            shift = (b0 - a0) // a.element_size() % least
+            return not width <= shift <= least - width
+    return True
+
+
+def _fill_rows(r: KvRows, key, value, query_starts, zero_rest: bool) -> None:
+    r.key, r.value, r.dtype, r.rows, r.zero_rest = key.data_ptr(), value.data_ptr(), _DTYPES[key.dtype], key.shape[0], zero_rest
+    r.key_stride[:] = key.stride()[:2]
+    r.value_stride[:] = value.stride()[:2]
+    r.starts = None if query_starts is None else query_starts.data_ptr()
+
+
+def paged_kv_append(key: Any, value: Any, key_cache: Any, value_cache: Any, page_table: Any, lengths: Any, query_starts: Any = None, *,
+                    key_scale: Any = None, value_scale: Any = None) -> None:
+    """Write `key` and `value` `[rows, kv_heads, head_dim]` into the cache: row `query_starts[s] + i` goes to position
+    `lengths[s] - n_s + i` of sequence `s`, `n_s` its number of rows.
+
+    A float8_e4m3fn cache keeps `value = code * scale` with one fp32 scale per token and head in `key_scale` / `value_scale`
+    `[pages, kv_heads, page_size]`: scale = max(|x|, 2^-100) / 448, the code is the nearest one (ties to even) to
+    x * 448 / max.  A row with an infinity or a NaN reads back as NaN.  Rows behind the last sequence are ignored.
+    """
+    c, r = KvCache(), KvRows()
+    _fill_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    _check_rows(key, "key", None, c.kv_heads, key_cache)
+    _check_rows(value, "value", key.shape[0], c.kv_heads, key_cache)
+    if key.dtype != value.dtype:
+        raise ValueError("key and value must have the same dtype")
+    _fill_rows(r, key, value, query_starts, False)
+    with _on(key_cache.device):
+        _lib.check(_lib.load().fk_kv_append(C.byref(c), C.byref(r), torch.cuda.current_stream().cuda_stream), "fk_kv_append")
+
+
+def paged_kv_gather(key_cache: Any, value_cache: Any, page_table: Any, lengths: Any, query_starts: Any, rows: int, *,
+                    key_scale: Any = None, value_scale: Any = None, dtype: Optional[torch.dtype] = None, out: Any = None):
+    """Read the last tokens of each sequence back: `(key, value)` `[rows, kv_heads, head_dim]`, row `query_starts[s] + i`
+    from position `lengths[s] - n_s + i`; the inverse of `paged_kv_append` with the same arguments.
+
+    `dtype` is the result's type for a float8_e4m3fn cache (bfloat16 by default).  `out=(key, value)` receives the rows
+    and keeps what it holds behind the last sequence; new tensors hold zeros there.
+    """
+    c, r = KvCache(), KvRows()
+    _fill_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    if rows < 0:
+        raise ValueError("rows must not be negative")
+    if dtype is None:
+        dtype = out[0].dtype if out is not None else torch.bfloat16 if key_cache.dtype == torch.float8_e4m3fn else key_cache.dtype
+    with _on(key_cache.device):
+        if out is None:
+            key = torch.empty((rows, c.kv_heads, c.head_dim), device=key_cache.device, dtype=dtype)
+            value = torch.empty_like(key)
+        else:
+            key, value = out
+        _check_rows(key, "key" if out is None else "out[0]", rows, c.kv_heads, key_cache)
+        _check_rows(value, "value" if out is None else "out[1]", rows, c.kv_heads, key_cache)
+        if key.dtype != dtype or value.dtype != dtype:
+            raise ValueError(f"out must have dtype {dtype}")
+        if out is not None and (_overlap(key, value) or any(_overlap(a, b) for a in out for b in (key_cache, value_cache))):
+            raise ValueError("out must not overlap the cache, nor its two tensors each other")
+        _fill_rows(r, key, value, query_starts, out is None)
+        _lib.check(_lib.load().fk_kv_gather(C.byref(c), C.byref(r), torch.cuda.current_stream().cuda_stream), "fk_kv_gather")
+    return key, value
+
+
+def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: Any, lengths: Any, query_starts: Any = None, *,
+                    scale: Optional[float] = None, window: int = 0, sinks: int = 0, key_scale: Any = None, value_scale: Any = None,
+                    max_query: int = 0, out: Any = None, flags: int = 0):
+    """softmax(scale * query . key) value for `query` `[rows, q_heads, head_dim]` over the cached keys and values.
+
+    Row `query_starts[s] + i` is the token at position `p = lengths[s] - n_s + i` of sequence `s` (its own key and value are
+    in the cache already); it sees positions `j <= p`, with `window > 0` only those with `j > p - window` or `j < sinks`.
+    Query head `a` reads key/value head `a // (q_heads // kv_heads)`.  `scale` defaults to `head_dim ** -0.5`.
+
+    Result `[rows, q_heads, head_dim]` in the query's dtype (`out` if given; it must not overlap the query or the cache).
+    A row that sees nothing (or only scores of -infinity) gives zeros.  Rows behind the last sequence keep what `out`
+    held; in a new tensor they are zero.  What masked positions hold, NaN included, has no influence on a row.
+    `max_query`, the largest number of rows of one sequence if the caller knows it, only chooses between kernels.
+    Sums and softmax statistics are fp32.
+    """
+    call = AttentionCall()
+    c = call.cache
+    _fill_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    if query.ndim != 3 or query.shape[1] < 1 or query.shape[1] % c.kv_heads:
+        raise ValueError("query must have shape [rows, q_heads, head_dim] with q_heads a multiple of the cache's kv_heads")
+    rows, q_heads, dim = query.shape
+    _check_rows(query, "query", rows, q_heads, key_cache)
+    if query_starts is None and rows > c.seqs:
+        raise ValueError("query has more rows than there are sequences: query_starts is required")
+    if window < 0 or sinks < 0 or max_query < 0:
+        raise ValueError("window, sinks and max_query must not be negative")
+    if sinks and not window:
+        raise ValueError("sinks need a window: without one every earlier position is visible")
+    if window >= 1 << 31 or sinks >= 1 << 31:
+        raise ValueError("window and sinks must be below 2^31")
+    if scale is None:
+        scale = dim ** -0.5
+    elif not math.isfinite(scale):
+        raise ValueError("scale must be finite")
+    with _on(query.device):
+        call.zero_rest = out is None
+        if out is None:
+            out = torch.empty((rows, q_heads, dim), device=query.device, dtype=query.dtype)
+        else:
+            _check_rows(out, "out", rows, q_heads, key_cache)
+            if out.dtype != query.dtype:
+                raise ValueError("out must have the query's dtype")
+            if any(_overlap(out, t) for t in (query, key_cache, value_cache)):
+                raise ValueError("out must not overlap the query or the cache")
+        call.query, call.out, call.dtype, call.rows, call.q_heads = query.data_ptr(), out.data_ptr(), _DTYPES[query.dtype], rows, q_heads
+        call.max_query = 1 if query_starts is None else min(max_query, rows)
+        call.query_stride[:] = query.stride()[:2]
+        call.out_stride[:] = out.stride()[:2]
+        call.starts = None if query_starts is None else query_starts.data_ptr()
+        call.scale, call.window, call.sinks, call.flags = scale, window, sinks, flags
+        lib = _lib.load()
+        need = lib.fk_paged_attention_workspace_bytes(C.byref(call))
+        # a new workspace per call: the allocator orders its reuse with the stream, and gives captured calls their own
+        ws = torch.empty(need, device=query.device, dtype=torch.uint8) if need else None
+        if need:
+            call.workspace, call.workspace_bytes = ws.data_ptr(), need
+        _lib.check(lib.fk_paged_attention(C.byref(call), torch.cuda.current_stream().cuda_stream), "fk_paged_attention")
+    return out
+
+
+class PagedKVCache:
+    """One layer's paged cache for a fixed number of sequences, with the pages handed out as the sequences grow.
+
+    `append` writes each sequence's new tokens and grows it, `attend` runs their attention, `read` returns whole
+    sequences, `release` gives a sequence's pages back.  The lengths live on the host as well, so that growing a sequence
+    needs no synchronisation; the page table and the lengths on the device are updated by copies on the current stream.
+    """
+
+    def __init__(self, pages: int, kv_heads: int, head_dim: int, *, seqs: int = 1, page_size: int = 16,
+                 dtype: torch.dtype = torch.bfloat16, device: Any = "cuda"):
+        if dtype not in _CACHE_DTYPES:
+            raise ValueError(f"the cache must be float32, bfloat16, float16 or float8_e4m3fn, got {dtype}")
+        if min(pages, kv_heads, seqs, page_size) < 1 or not 1 <= head_dim <= _lib.MAX_HEAD_DIM:
+            raise ValueError(f"pages, kv_heads, seqs and page_size must be positive, head_dim between 1 and {_lib.MAX_HEAD_DIM}")
+        shape = (pages, kv_heads, page_size, head_dim)
+        self.key, self.value = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if dtype == torch.float8_e4m3fn
+                                else torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
+        self.key_scale = self.value_scale = None
+        if dtype == torch.float8_e4m3fn:
+            self.key_scale, self.value_scale = (torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2))
+        self.page_size, self.seqs = page_size, seqs
+        self.host_lengths = [0] * seqs
+        self._owned: list[list[int]] = [[] for _ in range(seqs)]
+        self._free = list(range(pages - 1, -1, -1))
+        self.page_table = torch.full((seqs, pages), -1, dtype=torch.int32, device=self.key.device)
+        self.lengths = torch.zeros(seqs, dtype=torch.int32, device=self.key.device)
+        self._starts: Any = None
+        self._new = [0] * seqs
+
+    def _scales(self) -> dict:
+        return {"key_scale": self.key_scale, "value_scale": self.value_scale}
+
+    def _grow(self, new) -> None:
+        need = [-(-(n + m) // self.page_size) - len(own) for n, m, own in zip(self.host_lengths, new, self._owned)]
+        if sum(max(0, n) for n in need) > len(self._free):
+            raise ValueError("the cache has no pages left for these tokens")
+        for s, n in enumerate(need):
+            if n > 0:
+                got = [self._free.pop() for _ in range(n)]
+                at = len(self._owned[s])
+                self._owned[s] += got
+                self.page_table[s, at:at + n] = torch.tensor(got, dtype=torch.int32, device=self.key.device)
+        self.host_lengths = [n + m for n, m in zip(self.host_lengths, new)]
+        self.lengths.copy_(torch.tensor(self.host_lengths, dtype=torch.int32))
+
+    def append(self, key: Any, value: Any, new=None) -> None:
+        """`key`, `value` `[rows, kv_heads, head_dim]`: `new[s]` rows for each sequence in turn (default: one each)."""
+        new = [1] * self.seqs if new is None else [int(n) for n in new]
+        if len(new) != self.seqs or min(new) < 0 or sum(new) != key.shape[0]:
+            raise ValueError("new must name each sequence's number of rows, with key's rows as their sum")
+        self._grow(new)
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        self._new, self._starts = new, torch.tensor(starts, dtype=torch.int32, device=self.key.device)
+        paged_kv_append(key, value, self.key, self.value, self.page_table, self.lengths, self._starts, **self._scales())
+
+    def attend(self, query: Any, *, scale: Optional[float] = None, window: int = 0, sinks: int = 0):
+        """Attention of the rows that the last `append` wrote, `query` `[rows, q_heads, head_dim]`."""
+        if self._starts is None or query.shape[0] != sum(self._new):
+            raise ValueError("attend takes the rows of the last append")
+        return paged_attention(query, self.key, self.value, self.page_table, self.lengths, self._starts, scale=scale, window=window,
+                               sinks=sinks, max_query=max(self._new), **self._scales())
+
+    def read(self, dtype: Optional[torch.dtype] = None):
+        """Every sequence whole: `(key, value)` `[sum of lengths, kv_heads, head_dim]`, one sequence after the other."""
+        starts = [0]
+        for n in self.host_lengths:
+            starts.append(starts[-1] + n)
+        return paged_kv_gather(self.key, self.value, self.page_table, self.lengths, torch.tensor(starts, dtype=torch.int32, device=self.key.device),
+                               starts[-1], dtype=dtype, **self._scales())
+
+    def release(self, seq: int) -> None:
+        """Empty one sequence and give its pages back."""
+        self._free += reversed(self._owned[seq])
+        self._owned[seq] = []
+        self.host_lengths[seq] = 0
+        self.page_table[seq].fill_(-1)
+        self.lengths[seq].zero_()
+        self._starts = None

@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-enum fk_dtype { FK_F32 = 0, FK_BF16 = 1, FK_F16 = 2 };
+enum fk_dtype { FK_F32 = 0, FK_BF16 = 1, FK_F16 = 2, FK_E4M3 = 3 /* key/value caches only */ };
 
 enum fk_status {
     FK_OK = 0,
@@ -236,6 +236,79 @@ int fk_moe_permute(const int64_t* topk_ids, int tokens, int top_k, int num_exper
  * (src/fastkernels/kernels/triton/qwen36_layer.py:94-105) and the norm feeding the MoE block (:167-190). */
 int fk_moe_layer_residual(const fk_moe_call* c, const float* resid_in, const float* update_in, float* resid_out,
                           float norm_eps, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Paged key/value cache and the attention that reads it.  The reference keeps one growing key and value
+ * tensor per layer and scans it head by head (KV append and causal attention,
+ * src/fastkernels/kernels/triton/qwen36_attention.py:321-380; src/fastkernels/reference/qwen36_real.py:317-323);
+ * paging, 8-bit storage, windows and ragged batches have no counterpart there.
+ *
+ * Pages hold page_size rows of every head.  Row r of page p, head h starts at element
+ * p * stride[0] + h * stride[1] + r * stride[2]; its head_dim elements are contiguous.
+ * Sequence s consists of the tokens at positions 0 .. lengths[s]-1; position j lies in row j % page_size of
+ * page page_table[s * table_stride + j / page_size].  `starts` (seqs + 1 entries) deals the rows of a call to the
+ * sequences: rows starts[s] .. starts[s+1]-1 are the LAST starts[s+1]-starts[s] tokens of sequence s, so lengths[s]
+ * counts them.  NULL starts: one row per sequence.
+ * Nothing on the device is trusted: a page number outside [0, pages), a position outside the table, or starts out of order
+ * lead to rows that are skipped (append), zero (gather) or not visible (attention), never to an access out of bounds.
+ * FK_E4M3: a row is kept as codes with one fp32 scale, value = code * scale; scale = max(|x|, 2^-100) / 448 over the row,
+ * code = the e4m3 number nearest to x * 448 / max(|x|, 2^-100), ties to even.  A row that holds an infinity or a NaN reads
+ * back as NaN.
+ * --------------------------------------------------------------------------------------------- */
+#define FK_MAX_HEAD_DIM 256
+
+typedef struct fk_kv_cache {
+    int32_t pages, kv_heads, page_size, head_dim;
+    int32_t dtype;                     /* fk_dtype of key and value */
+    int32_t seqs, max_pages;           /* page_table is [seqs, max_pages] */
+    int32_t reserved;
+    int64_t table_stride;
+    int64_t key_stride[3], value_stride[3];              /* page, head, row; in elements */
+    int64_t key_scale_stride[3], value_scale_stride[3];  /* page, head, row; FK_E4M3 only */
+    void* key;
+    void* value;
+    float* key_scale;                  /* f32 [pages, kv_heads, page_size]; FK_E4M3 only */
+    float* value_scale;
+    const int32_t* page_table;
+    const int32_t* lengths;            /* i32 [seqs] */
+} fk_kv_cache;
+
+typedef struct fk_kv_rows {
+    void* key;                         /* [rows, kv_heads, head_dim]: read by append, written by gather */
+    void* value;
+    int32_t dtype;                     /* FK_F32, FK_BF16 or FK_F16; equal to the cache's unless that is FK_E4M3 */
+    int32_t rows;
+    int32_t zero_rest;                 /* gather: also write zeros to the rows behind the last sequence */
+    int32_t reserved;
+    int64_t key_stride[2], value_stride[2];              /* row, head; in elements */
+    const int32_t* starts;
+} fk_kv_rows;
+
+typedef struct fk_attention_call {
+    fk_kv_cache cache;
+    const void* query;                 /* [rows, q_heads, head_dim]; query head a reads key/value head a / (q_heads / kv_heads) */
+    void* out;                         /* like query; must not overlap it */
+    int32_t dtype;                     /* of query and out; equal to the cache's unless that is FK_E4M3 */
+    int32_t rows, q_heads;
+    int32_t max_query;                 /* most rows of one sequence, or 0 if not known: it chooses between kernels, no result depends on it */
+    int64_t query_stride[2], out_stride[2];              /* row, head; in elements */
+    const int32_t* starts;
+    float scale;                       /* of the scores */
+    int32_t window;                    /* > 0: a token sees the last `window` positions up to its own, and the first `sinks`; 0: all up to its own */
+    int32_t sinks;
+    int32_t zero_rest;                 /* also write zeros to the rows behind the last sequence (otherwise they are left alone) */
+    uint32_t flags;                    /* FK_FLAG_FORCE_GENERIC: the shape-agnostic kernel */
+    int32_t reserved;
+    void* workspace;                   /* fk_paged_attention_workspace_bytes(); needs no clearing, not shared by calls that overlap */
+    size_t workspace_bytes;
+} fk_attention_call;
+
+/* Write new tokens into the cache / read the last tokens of each sequence back. */
+int fk_kv_append(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
+int fk_kv_gather(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
+/* out = softmax(scale * query . key) value over the positions that each row sees; a row that sees none gives zeros. */
+size_t fk_paged_attention_workspace_bytes(const fk_attention_call* call);
+int fk_paged_attention(const fk_attention_call* call, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Expert-parallel layer over peer memory (one node, one process per GPU, NVLink).
