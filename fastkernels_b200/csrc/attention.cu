@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(32 * kAnyWarps) attention_any_kernel(const __g
     const int64_t rh = item / p.splits;
     const int split = (int)(item - rh * p.splits);
     const int row = (int)(rh / p.q_heads), qh = (int)(rh - (int64_t)row * p.q_heads);
-    const RowPlace at = place_of_row(p.starts, p.c.lengths, p.c.seqs, row);
+    const RowPlace at = place_of_row(p.starts, p.c.lengths, p.c.seqs, p.rows, row);
     T* out = reinterpret_cast<T*>(p.out) + row * p.os[0] + qh * p.os[1];
     RowSums r;
     if (at.seq < 0) {
@@ -132,8 +132,23 @@ static AttnParams attn_params(const fk_attention_call& a) {
     return p;
 }
 
-static size_t workspace_need(const fk_attention_call& a) {
-    if (a.rows == 0) return 0;
+enum class Path { any, few };
+
+// Few rows per key/value head (up to 16: decode and short continuations) are a stream of the cache; everything else, and what
+// that kernel has no form for (fp32, other head sizes, rows off 16-byte boundaries), takes the shape-agnostic kernel.
+static Path path_of(const fk_attention_call& a, const AttnParams& p) {
+    if (a.flags & FK_FLAG_FORCE_GENERIC) return Path::any;
+    const int most = a.starts == nullptr ? 1 : a.max_query;
+    if (attention_few_supported(p, a.dtype, most)) return Path::few;
+    return Path::any;
+}
+
+static size_t workspace_need(const fk_attention_call& a, const AttnParams& p, Path path) {
+    size_t need = 0;
+    if (path == Path::few) {
+        attention_few(p, a.dtype, a.starts == nullptr ? 1 : a.max_query, &need, nullptr);
+        return need;
+    }
     const int splits = any_splits(a);
     return splits > 1 ? (size_t)a.rows * a.q_heads * splits * (a.cache.head_dim + 2) * sizeof(float) : 0;
 }
@@ -145,21 +160,24 @@ using namespace fk;
 extern "C" {
 
 size_t fk_paged_attention_workspace_bytes(const fk_attention_call* a) {
-    if (a == nullptr || a->rows <= 0 || a->q_heads < 1 || a->cache.kv_heads < 1 || a->cache.head_dim < 1) return 0;
-    return workspace_need(*a);
+    if (check_attention(a) != FK_OK || a->rows == 0) return 0;
+    const AttnParams p = attn_params(*a);
+    return workspace_need(*a, p, path_of(*a, p));
 }
 
 int fk_paged_attention(const fk_attention_call* a, void* stream) {
     const int st = check_attention(a);
     if (st != FK_OK) return st;
     if (a->rows == 0 || (a->cache.seqs == 0 && !a->zero_rest)) return FK_OK;
-    const size_t need = workspace_need(*a);
-    if (need > 0 && (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15))) return FK_ERR_WORKSPACE;
     AttnParams p = attn_params(*a);
+    const Path path = path_of(*a, p);
+    const size_t need = workspace_need(*a, p, path);
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15))) return FK_ERR_WORKSPACE;
+    cudaStream_t s = (cudaStream_t)stream;
+    if (path == Path::few) return attention_few(p, a->dtype, a->starts == nullptr ? 1 : a->max_query, nullptr, s);
     p.splits = any_splits(*a);
     const int cb = dtype_bytes(a->cache.dtype);
     const bool wide = a->cache.head_dim % 8 == 0 && groups_aligned(a->cache.key, a->cache.key_stride, 3, cb, cb == 1 ? 8 : 16);
-    cudaStream_t s = (cudaStream_t)stream;
     if (a->cache.dtype == FK_E4M3) {
         if (a->dtype == FK_BF16) return launch_any<__nv_bfloat16, __nv_fp8_e4m3>(p, wide, s);
         if (a->dtype == FK_F16) return launch_any<__half, __nv_fp8_e4m3>(p, wide, s);

@@ -16,7 +16,7 @@ struct AttnParams {
     float scale_log2;          // scale * log2(e): scores are held as powers of two
     int splits;                // pieces of the key axis (shape-agnostic kernel)
     float* part;               // partial results
-    int blocks;                // grid of the kernels that deal key tiles evenly
+    int tile_tokens;           // tokens of an item of the kernels that work on tiles of tokens
 };
 
 // What a token at position p sees: [0, min(sinks, lo)) and [lo, p], lo = first position of its window.
@@ -93,5 +93,9 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const float* q, in
         }
     }
 }
+
+// Kernel for few query rows per key/value head (attention_few.cu).  need != null: only the workspace's size.
+bool attention_few_supported(const AttnParams& p, int dtype, int max_query);
+int attention_few(const AttnParams& p, int dtype, int max_query, size_t* need, cudaStream_t stream);
 
 }  // namespace fk

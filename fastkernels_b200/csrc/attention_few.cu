@@ -1,0 +1,619 @@
+// Attention of few new tokens per sequence (decode) over a paged cache: a stream of the cache's bytes.
+//
+// The query rows that share a key/value head (heads of the group x tokens) are the 8 * NT columns of the products, the keys
+// their rows: S^T[16 keys, columns] = K Q^T and O^T[dim, columns] += V^T P^T, both mma.sync m16n8k16 with fp32 sums.  At 8
+// columns an instruction carries 512 bytes of the cache, so the tensor pipe is idle nine tenths of the time and what bounds the
+// kernel is HBM; swapping the operands instead (queries as 16 rows) would double the instructions for nothing.  tcgen05 has no
+// use here: its operands would have to be at least 64 rows.
+//
+// Every warp works alone: it takes 16 keys at a time through its own ring of shared-memory slots (cp.async, a slot of keys, then
+// one of values), keeps its own running maximum and sum, and never waits for another warp.  The groups of 16 keys of all
+// (sequence, head) items, in order, are dealt to the warps of the grid in equal contiguous runs, so uneven sequences need no
+// schedule.  A run covers some items whole (written out at once) and at most two in part; those are joined by
+// attention_few_join_kernel in key order, so the result does not depend on timing.
+//
+// 8-bit caches: the codes go to fp16 exactly; a query row is scaled by a power of two into fp16's range (exact for what is
+// within 2^-14 of its largest element, to 2^-25 of it below), scores are multiplied by their key's scale, and the weights by
+// their value's scale over the largest one met so far.  Weights are rounded to the type of the products' operands, fp16 ones
+// after a factor of 2^14 so that small ones keep their bits; sums stay in fp32.
+
+#include <type_traits>
+
+#include "attention_items.cuh"
+#include "kernels.cuh"
+#include "tma.cuh"
+
+namespace fk {
+
+template <typename TC> struct FewOps {           // operand type of the products
+    using T = TC;
+    static constexpr bool kCodes = false;
+};
+template <> struct FewOps<__nv_fp8_e4m3> {
+    using T = __half;
+    static constexpr bool kCodes = true;
+};
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2], __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t codes_to_half2(uint32_t two) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
+    return (uint32_t)h.x | ((uint32_t)h.y << 16);
+}
+__device__ __forceinline__ uint4 lds16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds8(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds_float(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+// `bytes` (0 or all) are copied, the rest of the destination becomes zero
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+constexpr int kFewKeys = 16;                    // keys of a group
+constexpr int kFewLeast = 2;                    // shortest run of a warp, in groups
+
+// What a warp's partial result belongs to.
+struct PartHead {
+    int first_row, tokens, head, seq, pos0;
+    int begins, ends;                           // the run has the item's first / last key group
+    int last;                                   // warp of the grid whose run has the item's last key group
+};
+
+template <int D, int NT, typename TC>
+struct FewShape {
+    static constexpr bool kCodes = FewOps<TC>::kCodes;
+    static constexpr int kPitch = D * (int)sizeof(TC);                 // bytes of a row in a slot
+    static constexpr int kSlot = 16 * kPitch + (kCodes ? 128 : 0);     // rows, then their 16 scales
+    static constexpr int kWarps = kCodes && NT == 1 && D <= 128 ? 16 : 8;      // as many as the registers hold
+    static constexpr int kFit = 192 * 1024 / kWarps / kSlot;           // slots per warp in 192 KB
+    static constexpr int kSlots = kFit > 8 ? 8 : kFit;
+    static constexpr int kCols = 8 * NT;
+    static constexpr int kPart = (D + 2) * kCols;                      // floats of a partial result: m, l per column, [column][D]
+    static constexpr int kQueryRow = FK_MAX_HEAD_DIM + 8;              // floats, for a row that is computed again
+    static constexpr int kSmem = kWarps * (kSlots * (kSlot + 16) + kQueryRow * 4) + 256;
+    static_assert(kSlots >= 3, "a slot being read and two on their way");
+};
+
+// 16-byte chunk of a slot's row in which a chunk of the source row is kept.  16-bit rows: ldmatrix reads eight rows of one
+// chunk.  Codes: a quarter of a warp reads chunks t = 0..3 of two neighbouring rows (keys), or two neighbouring chunks (units of 8
+// bytes at 64 dimensions) of rows four apart (values).
+template <int D, typename TC, bool VALUES>
+__device__ __forceinline__ int slot_chunk(int row, int chunk) {
+    if (!FewOps<TC>::kCodes) return chunk ^ (row & 7);
+    if (!VALUES) return D >= 128 ? chunk ^ ((row & 1) << 2) : chunk;
+    return D >= 128 ? chunk ^ (((row >> 2) & 3) << 1) : chunk ^ ((row >> 2) & 3);
+}
+
+// Runs of the warps: [w * all / warps, (w + 1) * all / warps), or kFewLeast groups each if that is more.
+struct Runs {
+    int64_t all, warps;
+    __device__ __forceinline__ bool even() const { return all >= warps * kFewLeast; }
+    __device__ __forceinline__ int64_t begin(int64_t w) const { return even() ? w * all / warps : min(w * kFewLeast, all); }
+    __device__ __forceinline__ int warp_of(int64_t group) const { return (int)(even() ? ((group + 1) * warps - 1) / all : group / kFewLeast); }
+};
+
+template <int D, int NT, typename T, typename TC>
+__global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention_few_kernel(const __grid_constant__ AttnParams p) {
+    using S = FewShape<D, NT, TC>;
+    using OT = typename FewOps<TC>::T;
+    constexpr bool kCodes = S::kCodes;
+    constexpr int kMT = D / 16, kSlots = S::kSlots;
+    constexpr float kShift = std::is_same<OT, __half>::value ? 14.f : 0.f;
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    unsigned char* mine = smem + 256 + warp * (kSlots * (S::kSlot + 16) + S::kQueryRow * 4);
+    const uint32_t ring = smem_u32(mine);
+    int2* meta = reinterpret_cast<int2*>(mine + kSlots * S::kSlot);
+    float* query_row = reinterpret_cast<float*>(mine + kSlots * (S::kSlot + 16));
+    pdl_trigger();
+    pdl_wait();
+
+    Runs runs{total_tiles<kFewKeys>(p, reinterpret_cast<int64_t*>(smem)), (int64_t)gridDim.x * S::kWarps};
+    zero_blind_rows<T>(p);
+    const int64_t me = (int64_t)blockIdx.x * S::kWarps + warp;
+    PartHead* heads = reinterpret_cast<PartHead*>(p.part) + me * 2;
+    float* parts = p.part + runs.warps * 2 * (sizeof(PartHead) / 4) + me * 2 * S::kPart;
+    const int64_t run0 = runs.begin(me), run1 = runs.begin(me + 1);
+    if (lane < 2) heads[lane].begins = heads[lane].ends = -1;
+    if (run0 >= run1) return;
+
+    ItemCursor<kFewKeys> cur, ahead;
+    locate(p, run0, cur);
+    ahead = cur;
+
+    // ---- issue side: keys and values of one group after the other into the ring
+    int64_t left = run1 - run0;
+    int page = -1, in_page = 0;                  // of this lane's row (lanes 0..15) of the next group
+    int64_t koff = -1, voff = -1;                // bytes
+    int issue_slot = 0;
+    auto look = [&] {                            // the page table is read one group ahead of its use
+        page = -1;
+        const int j = ahead.key0() + (lane & 15);
+        if (left > 0 && ahead.some_row_sees(p, j)) page = page_of(p.c, ahead.seq, j, in_page);
+    };
+    auto issue = [&](bool values) {
+        if (left > 0) {
+            const uint32_t base = ring + issue_slot * S::kSlot;
+            if (!values) {
+                koff = page < 0 ? -1 : row_offset(p.c.key_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
+                voff = page < 0 ? -1 : row_offset(p.c.value_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
+                const unsigned rows = __ballot_sync(kFull, page >= 0) & 0xffffu;
+                if (lane == 0) meta[issue_slot * 2] = make_int2(ahead.key0(), (int)rows);
+            }
+            const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
+            constexpr int kChunks = S::kPitch / 16, kAtOnce = 32 / kChunks;
+#pragma unroll
+            for (int i = 0; i < 16 / kAtOnce; ++i) {
+                const int row = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                const int64_t off = __shfl_sync(kFull, values ? voff : koff, row);
+                const int to = values ? slot_chunk<D, TC, true>(row, chunk) : slot_chunk<D, TC, false>(row, chunk);
+                copy16(base + row * S::kPitch + to * 16, off < 0 ? from : from + off + chunk * 16, off < 0 ? 0 : 16);
+            }
+            if (kCodes && lane < 16) {
+                const float* s = values ? p.c.value_scale : p.c.key_scale;
+                copy4(base + 16 * S::kPitch + lane * 4,
+                      page < 0 ? s : s + (values ? row_offset(p.c.value_scale_stride, page, ahead.head, in_page) : row_offset(p.c.key_scale_stride, page, ahead.head, in_page)),
+                      page < 0 ? 0 : 4);
+            }
+            if (values) {
+                --left;
+                if (++ahead.k >= ahead.span.count && left > 0) ahead.next_item(p);
+                look();
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (++issue_slot == kSlots) issue_slot = 0;
+    };
+    look();
+#pragma unroll
+    for (int i = 0; i < kSlots - 1; ++i) issue(i & 1);
+    int slot = 0;
+    // the oldest slot has landed for the whole warp, and the one before it is free
+    auto next_slot = [&](bool issue_values) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+        __syncwarp();
+        issue(issue_values);
+        const int now = slot;
+        if (++slot == kSlots) slot = 0;
+        return now;
+    };
+
+    const int row_lo = kCodes ? 4 * (g >> 1) + (g & 1) : g, row_hi = kCodes ? row_lo + 2 : g + 8;      // this thread's key rows of S^T
+    int64_t at = run0;
+    while (at < run1) {
+        const int steps = (int)min((int64_t)(cur.span.count - cur.k), run1 - at);
+        const bool begins = cur.k == 0, ends = cur.k + steps == cur.span.count;
+        const int first_row = cur.first_row(p), tokens = cur.tokens(p), cols = tokens * p.group;
+        // ---- query fragments
+        uint32_t qf[NT][kMT][2];
+        float qscale[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int n = nt * 8 + g;
+            const int tok = n / p.group;
+            const T* q = reinterpret_cast<const T*>(p.query) + (int64_t)(first_row + (n < cols ? tok : 0)) * p.qs[0] +
+                         (int64_t)(cur.head * p.group + (n < cols ? n - tok * p.group : 0)) * p.qs[1];
+#pragma unroll
+            for (int kk = 0; kk < kMT; ++kk)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int d = kCodes ? ((kk >> 2) * 4 + t) * 16 + (kk & 3) * 4 + 2 * h : kk * 16 + 2 * t + 8 * h;
+                    qf[nt][kk][h] = n < cols ? *reinterpret_cast<const uint32_t*>(q + d) : 0u;
+                }
+            if (kCodes) {
+                float most = 0.f;
+#pragma unroll
+                for (int kk = 0; kk < kMT; ++kk)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const T* two = reinterpret_cast<const T*>(&qf[nt][kk][h]);
+                        most = fmaxf(most, fmaxf(fabsf(to_float(two[0])), fabsf(to_float(two[1]))));
+                    }
+                most = fmaxf(most, __shfl_xor_sync(kFull, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
+                const int e = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
+                const float down = ldexpf(1.f, -e);
+#pragma unroll
+                for (int kk = 0; kk < kMT; ++kk)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const T* two = reinterpret_cast<const T*>(&qf[nt][kk][h]);
+                        qf[nt][kk][h] = pack2(to_float(two[0]) * down, to_float(two[1]) * down, __half{});
+                    }
+                const float up = ldexpf(p.scale_log2, e);
+                qscale[nt][0] = __shfl_sync(kFull, up, 8 * t);
+                qscale[nt][1] = __shfl_sync(kFull, up, 8 * t + 4);
+            } else {
+                qscale[nt][0] = qscale[nt][1] = p.scale_log2;
+            }
+        }
+        float acc[NT][kMT][4], m[NT][2], l[NT][2], top = 0.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int i = 0; i < kMT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
+        const int sure_lo = window_start(p, cur.pos1);        // keys that every token of the item sees: sure_lo .. pos0
+
+        for (int step = 0; step < steps; ++step) {
+            // ---- scores
+            const int ks = next_slot((kSlots - 1) & 1);
+            const uint32_t kbase = ring + ks * S::kSlot;
+            const int2 what = meta[ks * 2];
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+            if (kCodes) {
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) {
+                    const uint4 lo = lds16(kbase + row_lo * S::kPitch + slot_chunk<D, TC, false>(row_lo, 4 * i + t) * 16);
+                    const uint4 hi = lds16(kbase + row_hi * S::kPitch + slot_chunk<D, TC, false>(row_hi, 4 * i + t) * 16);
+                    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t a[4] = {codes_to_half2(wl[j]), codes_to_half2(wh[j]), codes_to_half2(wl[j] >> 16), codes_to_half2(wh[j] >> 16)};
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a, qf[nt][4 * i + j], OT{});
+                    }
+                }
+                const float k0 = lds_float(kbase + 16 * S::kPitch + row_lo * 4), k1 = lds_float(kbase + 16 * S::kPitch + row_hi * 4);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    s[nt][0] *= qscale[nt][0] * k0; s[nt][1] *= qscale[nt][1] * k0;
+                    s[nt][2] *= qscale[nt][0] * k1; s[nt][3] *= qscale[nt][1] * k1;
+                }
+            } else {
+                float s2[NT][4];                  // two chains of products
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
+                const int row = lane & 15;
+#pragma unroll
+                for (int kk = 0; kk < kMT; ++kk) {
+                    uint32_t a[4];
+                    ldmatrix4(a, kbase + row * S::kPitch + slot_chunk<D, TC, false>(row, 2 * kk + (lane >> 4)) * 16);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816(kk & 1 ? s2[nt] : s[nt], a, qf[nt][kk], OT{});
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * p.scale_log2;
+            }
+            // ---- masks: rows that are not there, and keys that only some of the tokens see
+            const bool all = tokens == 1 || (what.x + 15 <= cur.pos0 && (p.window == 0 || what.x >= sure_lo || what.x + 15 < p.sinks));
+            if (what.y != 0xffff || !all) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = i < 2 ? row_lo : row_hi, n = nt * 8 + 2 * t + (i & 1);
+                        if (!((what.y >> row) & 1) || (!all && !sees(p, cur.pos0 + n / p.group, what.x + row))) s[nt][i] = -INFINITY;
+                    }
+            }
+            // ---- running maximum, weights
+            bool grew = false;
+            float mn[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float x = fmaxf(s[nt][c], s[nt][c + 2]);
+                    x = fmaxf(x, __shfl_xor_sync(kFull, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(kFull, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(kFull, x, 16));
+                    mn[nt][c] = fmaxf(m[nt][c], x);
+                    grew |= mn[nt][c] > m[nt][c];
+                }
+            if (__any_sync(kFull, grew)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float a = mn[nt][c] > m[nt][c] ? exp2_fast(m[nt][c] - mn[nt][c]) : 1.f;
+                        m[nt][c] = mn[nt][c];
+                        l[nt][c] *= a;
+#pragma unroll
+                        for (int i = 0; i < kMT; ++i) { acc[nt][i][c] *= a; acc[nt][i][c + 2] *= a; }
+                    }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float base = m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1] - kShift;
+                    s[nt][i] = exp2_fast(s[nt][i] - base);
+                    l[nt][i & 1] += s[nt][i];
+                }
+            // ---- values
+            const int vs = next_slot(((kSlots - 1) & 1) ^ 1);
+            const uint32_t vbase = ring + vs * S::kSlot;
+            if (kCodes) {
+                float v0 = lds_float(vbase + 16 * S::kPitch + row_lo * 4), v1 = lds_float(vbase + 16 * S::kPitch + row_hi * 4);
+                float most = fmaxf(fabsf(v0), fabsf(v1));
+                most = fmaxf(most, __shfl_xor_sync(kFull, most, 4));
+                most = fmaxf(most, __shfl_xor_sync(kFull, most, 8));
+                most = fmaxf(most, __shfl_xor_sync(kFull, most, 16));
+                if (most > top) {                 // the same in all lanes
+                    const float a = top / most;
+                    top = most;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < kMT; ++i)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) acc[nt][i][c] *= a;
+                }
+                if (top > 0.f) { v0 /= top; v1 /= top; }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) { s[nt][0] *= v0; s[nt][1] *= v0; s[nt][2] *= v1; s[nt][3] *= v1; }
+            }
+            uint32_t pf[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                pf[nt][0] = transpose8x8(pack2(s[nt][0], s[nt][1], OT{}));
+                pf[nt][1] = transpose8x8(pack2(s[nt][2], s[nt][3], OT{}));
+            }
+            if (kCodes) {
+                constexpr int kUnits = D >= 128 ? D / 128 : 1, kWords = D >= 128 ? 4 : 2;
+#pragma unroll
+                for (int u = 0; u < kUnits; ++u) {
+                    uint32_t w[4][4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 4 * t + i;
+                        if (D >= 128) {
+                            const uint4 x = lds16(vbase + row * S::kPitch + slot_chunk<D, TC, true>(row, g + 8 * u) * 16);
+                            w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
+                        } else {
+                            const uint2 x = lds8(vbase + row * S::kPitch + slot_chunk<D, TC, true>(row, g >> 1) * 16 + (g & 1) * 8);
+                            w[i][0] = x.x; w[i][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < kWords; ++j)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t c[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) c[i] = codes_to_half2(w[i][j] >> (16 * h));
+                            const uint32_t a[4] = {__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[0], c[1], 0x7632), __byte_perm(c[2], c[3], 0x5410),
+                                                   __byte_perm(c[2], c[3], 0x7632)};
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][u * 8 + j * 2 + h], a, pf[nt], OT{});
+                        }
+                }
+            } else {
+                const int row = (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+                for (int i = 0; i < kMT; ++i) {
+                    uint32_t a[4];
+                    ldmatrix4_trans(a, vbase + row * S::kPitch + slot_chunk<D, TC, true>(row, 2 * i + ((lane >> 3) & 1)) * 16);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][i], a, pf[nt], OT{});
+                }
+            }
+        }
+
+        // ---- the item's result, or this run's part of it.  acc[.][i][c + 2 h] is column 2t + c at dimension dim_of(i, h)
+        auto dim_of = [&](int i, int h) { return kCodes ? (D >= 128 ? ((i >> 3) * 8 + g) * 16 + (i & 7) * 2 + h : g * 8 + i * 2 + h) : i * 16 + g + 8 * h; };
+        const float unit = kCodes ? top : 1.f;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 4);
+                l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 8);
+                l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 16);
+            }
+        if (begins && ends) {
+            bool odd = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int n = nt * 8 + 2 * t + c;
+                    if (n >= cols) continue;
+                    const int tok = n / p.group;
+                    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first_row + tok) * p.os[0] + (int64_t)(cur.head * p.group + n - tok * p.group) * p.os[1];
+                    const float inv = l[nt][c] == 0.f ? 0.f : unit / l[nt][c];
+#pragma unroll
+                    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const float v = l[nt][c] == 0.f ? 0.f : acc[nt][i][c + 2 * h] * inv;
+                            odd |= !(fabsf(v) < INFINITY);
+                            store_elem(out + dim_of(i, h), v);
+                        }
+                }
+            if (tokens > 1 && __any_sync(kFull, odd))
+                for (int n = 0; n < cols; ++n)
+                    row_again<T, TC>(p, query_row, cur.seq, first_row + n / p.group, cur.pos0 + n / p.group, cur.head * p.group + n % p.group);
+        } else {
+            const int which = at == run0 ? 0 : 1;
+            float* part = parts + which * S::kPart;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const int n = nt * 8 + 2 * t + c;
+                    if (n >= cols) continue;
+                    if (g == 0) { part[n] = m[nt][c]; part[S::kCols + n] = l[nt][c]; }
+#pragma unroll
+                    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) part[2 * S::kCols + n * D + dim_of(i, h)] = acc[nt][i][c + 2 * h] * unit;
+                }
+            if (lane == 0)
+                heads[which] = PartHead{first_row, tokens, cur.head, cur.seq, cur.pos0, begins, ends, runs.warp_of(at - cur.k + cur.span.count - 1)};
+        }
+        at += steps;
+        if (at < run1) cur.next_item(p);
+    }
+}
+
+// Joins the parts of one item, a block per (warp of the grid above whose run has the item's beginning, column).
+constexpr int kJoinWarps = 4;
+
+template <int D, int NT, typename T, typename TC>
+__global__ void __launch_bounds__(32 * kJoinWarps) attention_few_join_kernel(const __grid_constant__ AttnParams p) {
+    using S = FewShape<D, NT, TC>;
+    __shared__ float sums[kJoinWarps][D + 2];
+    __shared__ float again[S::kQueryRow];
+    pdl_trigger();
+    pdl_wait();
+    const int64_t warps = gridDim.x;
+    const PartHead* heads = reinterpret_cast<const PartHead*>(p.part);
+    const float* parts = p.part + warps * 2 * (sizeof(PartHead) / 4);
+    const int w0 = blockIdx.x, n = blockIdx.y;
+    int which = -1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (heads[2 * w0 + i].begins == 1 && heads[2 * w0 + i].ends == 0) which = i;
+    if (which < 0) return;
+    const PartHead h = heads[2 * w0 + which];
+    if (n >= h.tokens * p.group) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, count = h.last - w0 + 1;
+    auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * w0 + which : 2 * (w0 + i)) * S::kPart; };
+    float m = -INFINITY;
+    for (int i = threadIdx.x; i < count; i += blockDim.x) m = fmaxf(m, part(i)[n]);
+    m = warp_max(m);
+    if (lane == 0) sums[warp][0] = m;
+    __syncthreads();
+    for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, sums[i][0]);
+    __syncthreads();
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, acc[D / 32] = {};
+    for (int i = warp; i < count; i += kJoinWarps) {
+        const float* one = part(i);
+        const float weight = exp2_fast(one[n] - base);
+        l = fmaf(weight, one[S::kCols + n], l);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(weight, one[2 * S::kCols + n * D + c * 32 + lane], acc[c]);
+    }
+    if (lane == 0) sums[warp][D] = l;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) sums[warp][c * 32 + lane] = acc[c];
+    __syncthreads();
+    if (warp != 0) return;
+    l = 0.f;
+    for (int i = 0; i < kJoinWarps; ++i) l += sums[i][D];
+    const int row = h.first_row + n / p.group, qh = h.head * p.group + n % p.group;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)row * p.os[0] + (int64_t)qh * p.os[1];
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        float v = 0.f;
+        for (int i = 0; i < kJoinWarps; ++i) v += sums[i][c * 32 + lane];
+        v = l == 0.f ? 0.f : v / l;
+        odd |= !(fabsf(v) < INFINITY);
+        store_elem(out + c * 32 + lane, v);
+    }
+    if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, again, h.seq, row, h.pos0 + n / p.group, qh);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+template <int D, int NT, typename T, typename TC>
+static int few(AttnParams p, int max_warps, size_t* need, cudaStream_t stream) {
+    using S = FewShape<D, NT, TC>;
+    p.tile_tokens = S::kCols / p.group;
+    const int blocks = (int)min((int64_t)sm_count(), ((int64_t)max_warps + S::kWarps - 1) / S::kWarps);
+    const int64_t warps = (int64_t)blocks * S::kWarps;
+    if (need) {
+        *need = warps * 2 * (sizeof(PartHead) + S::kPart * sizeof(float));
+        return FK_OK;
+    }
+    auto kern = attention_few_kernel<D, NT, T, TC>;
+    FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), "attention (few) attr");
+    FK_CUDA_OK(launch_pdl(kern, dim3(blocks), dim3(32 * S::kWarps), (size_t)S::kSmem, stream, p), "attention (few) launch");
+    FK_LAUNCH_OK("attention (few) launch");
+    const int cols = (int)min((int64_t)S::kCols, (int64_t)p.tile_tokens * p.group);
+    FK_CUDA_OK(launch_pdl(attention_few_join_kernel<D, NT, T, TC>, dim3((unsigned)warps, cols), dim3(32 * kJoinWarps), 0, stream, p), "attention (few) join launch");
+    FK_LAUNCH_OK("attention (few) join launch");
+    return FK_OK;
+}
+
+template <int D, typename T, typename TC>
+static int few_columns(const AttnParams& p, int cols, int max_warps, size_t* need, cudaStream_t stream) {
+    if (cols <= 8) return few<D, 1, T, TC>(p, max_warps, need, stream);
+    return few<D, 2, T, TC>(p, max_warps, need, stream);
+}
+
+template <typename T, typename TC>
+static int few_dim(const AttnParams& p, int cols, int max_warps, size_t* need, cudaStream_t stream) {
+    switch (p.c.head_dim) {
+        case 64: return few_columns<64, T, TC>(p, cols, max_warps, need, stream);
+        case 128: return few_columns<128, T, TC>(p, cols, max_warps, need, stream);
+        default: return few_columns<256, T, TC>(p, cols, max_warps, need, stream);
+    }
+}
+
+bool attention_few_supported(const AttnParams& p, int dtype, int max_query) {
+    if (dtype != FK_BF16 && dtype != FK_F16) return false;
+    if (p.c.head_dim != 64 && p.c.head_dim != 128 && p.c.head_dim != 256) return false;
+    if (max_query < 1 || (int64_t)max_query * p.group > 16) return false;
+    const int cb = dtype_bytes(p.c.dtype);
+    return groups_aligned(p.c.key, p.c.key_stride, 3, cb, 16) && groups_aligned(p.c.value, p.c.value_stride, 3, cb, 16) && groups_aligned(p.query, p.qs, 2, 2, 4);
+}
+
+// need != null: only the workspace's size
+int attention_few(const AttnParams& p, int dtype, int max_query, size_t* need, cudaStream_t stream) {
+    // most runs that the call can have: no more warps are launched
+    const int64_t longest = ((int64_t)p.c.max_pages * p.c.page_size + kFewKeys - 1) / kFewKeys;
+    const int64_t groups = longest * p.c.kv_heads * (p.c.seqs < p.rows ? p.c.seqs : p.rows);
+    const int max_warps = (int)min((int64_t)1 << 20, max((int64_t)1, (groups + kFewLeast - 1) / kFewLeast));
+    const int cols = max_query * p.group;
+    if (dtype == FK_BF16)
+        return p.c.dtype == FK_E4M3 ? few_dim<__nv_bfloat16, __nv_fp8_e4m3>(p, cols, max_warps, need, stream)
+                                    : few_dim<__nv_bfloat16, __nv_bfloat16>(p, cols, max_warps, need, stream);
+    return p.c.dtype == FK_E4M3 ? few_dim<__half, __nv_fp8_e4m3>(p, cols, max_warps, need, stream) : few_dim<__half, __half>(p, cols, max_warps, need, stream);
+}
+
+}  // namespace fk

@@ -1,0 +1,211 @@
+// Items of paged attention (sequence, key/value head, tile of new tokens) and the tiles of keys that each of them reads, in one
+// order that every block and warp derives for itself from the lengths on the device.
+#pragma once
+
+#include "attention.cuh"
+
+namespace fk {
+
+// Sequence s of a call: rows [first, first + n), the token of row r at position base + r.
+struct SeqRows { int first, n, base; };
+
+__device__ __forceinline__ SeqRows rows_of_seq(const AttnParams& p, int s) {
+    SeqRows r;
+    if (p.starts == nullptr) {
+        r.first = s;
+        r.n = s < p.rows ? 1 : 0;
+        r.base = max(p.c.lengths[s], 0) - 1 - s;
+        return r;
+    }
+    const int a = p.starts[s], b = p.starts[s + 1];
+    r.first = min(max(a, 0), p.rows);
+    const int end = min(max(b, 0), p.rows);
+    r.n = max(0, end - r.first);
+    r.base = max(p.c.lengths[s], 0) - end;          // no position exceeds lengths - 1, whatever the starts hold
+    return r;
+}
+
+// Key tiles of KT positions that some token at pos0 .. pos1 sees: tiles 0 .. sink_tiles-1, then lo_tile .. ; count in all.
+struct TileSpan { int sink_tiles, lo_tile, count, end; };
+
+template <int KT>
+__device__ __forceinline__ TileSpan span_of(const AttnParams& p, int pos0, int pos1) {
+    TileSpan s{0, 0, 0, 0};
+    s.end = min(pos1 + 1, p.c.max_pages * p.c.page_size);
+    if (s.end <= 0) return s;
+    const int lo = min(window_start(p, pos0), s.end);
+    const int hi_tile = (s.end + KT - 1) / KT;
+    const int sink_tiles = (min(p.sinks, lo) + KT - 1) / KT, lo_tile = lo / KT;
+    if (sink_tiles >= lo_tile) {
+        s.count = hi_tile;
+    } else {
+        s.sink_tiles = sink_tiles;
+        s.lo_tile = lo_tile;
+        s.count = sink_tiles + (lo < s.end ? hi_tile - lo_tile : 0);
+    }
+    return s;
+}
+
+__device__ __forceinline__ bool sees(const AttnParams& p, int pos, int j) {
+    return j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
+}
+
+// A position in the order (sequence, head, tile of tokens, key tile).  All lanes of a warp hold the same.
+template <int KT>
+struct ItemCursor {
+    int seq, head, tile;       // item: tokens [tile * p.tile_tokens, ..) of the sequence
+    SeqRows rows;
+    int pos0, pos1;            // first and last token's position
+    TileSpan span;
+    int k;                     // key tile of the item
+
+    __device__ __forceinline__ int tokens(const AttnParams& p) const { return min(p.tile_tokens, rows.n - tile * p.tile_tokens); }
+    __device__ __forceinline__ int first_row(const AttnParams& p) const { return rows.first + tile * p.tile_tokens; }
+    __device__ __forceinline__ int key0() const { return (k < span.sink_tiles ? k : span.lo_tile + k - span.sink_tiles) * KT; }
+    __device__ __forceinline__ bool some_row_sees(const AttnParams& p, int j) const {
+        return j < span.end && (p.window == 0 || j >= window_start(p, pos0) || j < p.sinks);
+    }
+    __device__ __forceinline__ void set_item(const AttnParams& p) {
+        pos0 = rows.base + first_row(p);
+        pos1 = pos0 + tokens(p) - 1;
+        span = span_of<KT>(p, pos0, pos1);
+    }
+    // to the first key tile of the next item that has any
+    __device__ __forceinline__ void next_item(const AttnParams& p) {
+        k = 0;
+        while (true) {
+            if (++tile * p.tile_tokens >= rows.n) {
+                tile = 0;
+                if (rows.n == 0 || ++head >= p.c.kv_heads) {
+                    head = 0;
+                    do {
+                        if (++seq >= p.c.seqs) return;
+                        rows = rows_of_seq(p, seq);
+                    } while (rows.n == 0);
+                }
+            }
+            set_item(p);
+            if (span.count > 0) return;
+        }
+    }
+};
+
+// Key tiles of one head's items of a sequence.
+template <int KT>
+__device__ __forceinline__ int64_t seq_tiles(const AttnParams& p, const SeqRows& r) {
+    int64_t sum = 0;
+    for (int t = 0; t < r.n; t += p.tile_tokens) {
+        const int pos0 = r.base + r.first + t;
+        sum += span_of<KT>(p, pos0, pos0 + min(p.tile_tokens, r.n - t) - 1).count;
+    }
+    return sum;
+}
+
+__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    return v;
+}
+
+// All items' key tiles; every thread of the block calls it, `scratch` holds a word per warp.
+template <int KT>
+__device__ __forceinline__ int64_t total_tiles(const AttnParams& p, int64_t* scratch) {
+    int64_t sum = 0;
+    for (int s = threadIdx.x; s < p.c.seqs; s += blockDim.x) {
+        const SeqRows r = rows_of_seq(p, s);
+        if (r.n > 0) sum += seq_tiles<KT>(p, r);
+    }
+    sum = warp_sum64(sum);
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    int64_t all = 0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) all += scratch[i];
+    return all * p.c.kv_heads;
+}
+
+// Cursor at key tile `target` of the order (target < total_tiles); a whole warp calls it.
+template <int KT>
+__device__ __forceinline__ void locate(const AttnParams& p, int64_t target, ItemCursor<KT>& c) {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int s0 = 0; s0 < p.c.seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int64_t mine = 0;
+        if (s < p.c.seqs) {
+            const SeqRows r = rows_of_seq(p, s);
+            if (r.n > 0) mine = seq_tiles<KT>(p, r) * p.c.kv_heads;
+        }
+        int64_t upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t up = __shfl_up_sync(kFull, upto, o);
+            if (lane >= o) upto += up;
+        }
+        const unsigned past = __ballot_sync(kFull, before + upto > target);
+        if (past == 0) {
+            before += __shfl_sync(kFull, upto, 31);
+            continue;
+        }
+        const int at = __ffs(past) - 1;
+        int64_t rest = target - before - __shfl_sync(kFull, upto - mine, at);
+        const int64_t per_head = __shfl_sync(kFull, mine, at) / p.c.kv_heads;
+        c.seq = s0 + at;
+        c.rows = rows_of_seq(p, c.seq);
+        c.head = (int)(rest / per_head);
+        rest -= c.head * per_head;
+        for (c.tile = 0;; ++c.tile) {
+            c.set_item(p);
+            if (rest < c.span.count) break;
+            rest -= c.span.count;
+        }
+        c.k = (int)rest;
+        return;
+    }
+}
+
+// Zeros for the rows that see nothing, and for those behind the last sequence if asked for.  Sequences are dealt to the blocks.
+template <typename T>
+__device__ __forceinline__ void zero_blind_rows(const AttnParams& p) {
+    const int width = p.q_heads * p.c.head_dim;
+    T* out = reinterpret_cast<T*>(p.out);
+    auto clear = [&](int row) {
+        for (int i = threadIdx.x; i < width; i += blockDim.x) {
+            const int a = i / p.c.head_dim;
+            store_elem(out + row * p.os[0] + a * p.os[1] + (i - a * p.c.head_dim), 0.f);
+        }
+    };
+    for (int s = blockIdx.x; s < p.c.seqs; s += gridDim.x) {
+        const SeqRows r = rows_of_seq(p, s);
+        if (r.n == 0) continue;
+        const int pos = r.base + r.first;
+        // only a sequence shorter than its rows, or one that reaches beyond its table, has such rows
+        if (pos >= 0 && (int64_t)pos + r.n <= p.c.max_pages * p.c.page_size) continue;
+        for (int i = 0; i < r.n; ++i)
+            if (span_of<1>(p, pos + i, pos + i).count == 0) clear(r.first + i);
+    }
+    if (p.zero_rest) {
+        const int used = p.starts ? min(max(p.starts[p.c.seqs], 0), p.rows) : min(p.c.seqs, p.rows);
+        const int unused = p.starts ? min(max(p.starts[0], 0), p.rows) : 0;         // 0 unless the starts are no starts
+        for (int row = blockIdx.x; row < p.rows; row += gridDim.x)
+            if (row < unused || row >= used) clear(row);
+    }
+}
+
+// A row whose result is not finite, alone and exactly: in a tile of several tokens a key that one of them must not see may have
+// entered the row's product as 0 * infinity.  A whole warp; `q` is FK_MAX_HEAD_DIM + 8 floats of shared memory of its own.
+template <typename T, typename TC>
+__device__ __noinline__ void row_again(const AttnParams& p, float* q, int seq, int row, int pos, int qh) {
+    const int lane = threadIdx.x & 31, D = p.c.head_dim;
+    const T* query = reinterpret_cast<const T*>(p.query) + row * p.qs[0] + qh * p.qs[1];
+    __syncwarp();
+    for (int d = lane; d < D + 8; d += 32) q[d] = d < D ? load_elem(query + d) * p.scale_log2 : 0.f;
+    __syncwarp();
+    RowSums r;
+    warp_row<TC, false>(p, q, seq, qh / p.group, pos, 0, 1, r);
+    T* out = reinterpret_cast<T*>(p.out) + row * p.os[0] + qh * p.os[1];
+#pragma unroll
+    for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
+        if (c * 32 + lane < D) store_elem(out + c * 32 + lane, r.l == 0.f ? 0.f : r.acc[c] / r.l);
+}
+
+}  // namespace fk

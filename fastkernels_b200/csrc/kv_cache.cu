@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const __grid_constant__ 
     const int64_t* from = is_value ? p.r.value_stride : p.r.key_stride;
     float v[8] = {};
     if (n > 0) load8<WIDE>(reinterpret_cast<const T*>(is_value ? p.r.value : p.r.key) + row * from[0] + head * from[1] + d0, n, v);
-    const RowPlace at = place_of_row(p.r.starts, p.c.lengths, p.c.seqs, row);
+    const RowPlace at = place_of_row(p.r.starts, p.c.lengths, p.c.seqs, p.r.rows, row);
     int in_page = 0;
     const int page = at.seq < 0 ? -1 : page_of(p.c, at.seq, at.pos, in_page);
     if (sizeof(TC) == 1) {
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) kv_gather_kernel(const __grid_constant__ 
     const bool is_value = rest >= p.c.kv_heads;
     const int head = is_value ? rest - p.c.kv_heads : rest;
     const int d0 = lane * 8, n = min(8, p.c.head_dim - d0);
-    const RowPlace at = place_of_row(p.r.starts, p.c.lengths, p.c.seqs, row);
+    const RowPlace at = place_of_row(p.r.starts, p.c.lengths, p.c.seqs, p.r.rows, row);
     if (n <= 0 || (at.seq < 0 && !p.r.zero_rest)) return;
     int in_page = 0;
     const int page = at.seq < 0 ? -1 : page_of(p.c, at.seq, at.pos, in_page);

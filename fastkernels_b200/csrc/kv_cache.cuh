@@ -15,12 +15,12 @@ struct RowPlace {
 
 __device__ __forceinline__ int seq_first(const int* starts, int s) { return starts ? starts[s] : s; }
 
-__device__ __forceinline__ RowPlace place_of_row(const int* __restrict__ starts, const int* __restrict__ lengths, int seqs, int row) {
+__device__ __forceinline__ RowPlace place_of_row(const int* __restrict__ starts, const int* __restrict__ lengths, int seqs, int rows, int row) {
     RowPlace r{-1, 0};
     if (starts == nullptr) {
         if (row >= seqs) return r;
         r.seq = row;
-        r.pos = lengths[row] - 1;
+        r.pos = max(lengths[row], 0) - 1;
         return r;
     }
     // the first s with starts[s + 1] > row
@@ -31,7 +31,7 @@ __device__ __forceinline__ RowPlace place_of_row(const int* __restrict__ starts,
     }
     if (lo >= seqs || starts[lo] > row) return r;
     r.seq = lo;
-    r.pos = lengths[lo] - starts[lo + 1] + row;
+    r.pos = max(lengths[lo], 0) - min(starts[lo + 1], rows) + row;        // at most lengths - 1, whatever the starts hold
     return r;
 }
 
