@@ -5,6 +5,9 @@
 // sums and statistics in fp32.  Pieces (m, l, acc) of one row over disjoint keys join as
 // m = max m_i, l = sum 2^(m_i - m) l_i, acc = sum 2^(m_i - m) acc_i.
 
+#include <cfloat>
+#include <cmath>
+
 #include "attention.cuh"
 
 namespace fk {
@@ -37,7 +40,7 @@ __global__ void __launch_bounds__(32 * kAnyWarps) attention_any_kernel(const __g
         const T* query = reinterpret_cast<const T*>(p.query) + row * p.qs[0] + qh * p.qs[1];
         for (int d = lane; d < D + 8; d += 32) q[d] = d < D ? load_elem(query + d) * p.scale_log2 : 0.f;
         __syncwarp();
-        warp_row<TC, WIDE>(p, q, at.seq, qh / p.group, at.pos, split, p.splits, r);
+        warp_row<TC, WIDE>(p, [q](int d) { return q[d]; }, at.seq, qh / p.group, at.pos, split, p.splits, r);
     }
     if (p.splits == 1) {
         const float inv = r.l > 0.f || r.l != r.l ? 1.f / r.l : 0.f;
@@ -128,18 +131,21 @@ static AttnParams attn_params(const fk_attention_call& a) {
     p.rows = a.rows; p.q_heads = a.q_heads; p.group = a.q_heads / a.cache.kv_heads;
     p.window = a.window; p.sinks = a.window > 0 ? a.sinks : 0; p.zero_rest = a.zero_rest;
     p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+    if (fabsf(p.scale_log2) < FLT_MIN) p.scale_log2 = FLT_MIN;
     p.part = reinterpret_cast<float*>(a.workspace);
     return p;
 }
 
-enum class Path { any, few };
+enum class Path { any, few, tile };
 
-// Few rows per key/value head (up to 16: decode and short continuations) are a stream of the cache; everything else, and what
-// that kernel has no form for (fp32, other head sizes, rows off 16-byte boundaries), takes the shape-agnostic kernel.
+// Few rows per key/value head (up to 16: decode and short continuations) are a stream of the cache; more, and head sizes that
+// the stream has no form for, go to the tensor cores; fp32, head sizes off a multiple of 8 and rows off 16-byte boundaries take
+// the shape-agnostic kernel.
 static Path path_of(const fk_attention_call& a, const AttnParams& p) {
     if (a.flags & FK_FLAG_FORCE_GENERIC) return Path::any;
     const int most = a.starts == nullptr ? 1 : a.max_query;
     if (attention_few_supported(p, a.dtype, most)) return Path::few;
+    if (attention_tile_supported(p, a.dtype)) return Path::tile;
     return Path::any;
 }
 
@@ -147,6 +153,10 @@ static size_t workspace_need(const fk_attention_call& a, const AttnParams& p, Pa
     size_t need = 0;
     if (path == Path::few) {
         attention_few(p, a.dtype, a.starts == nullptr ? 1 : a.max_query, &need, nullptr);
+        return need;
+    }
+    if (path == Path::tile) {
+        attention_tile(p, a.dtype, &need, nullptr);
         return need;
     }
     const int splits = any_splits(a);
@@ -175,6 +185,7 @@ int fk_paged_attention(const fk_attention_call* a, void* stream) {
     if (need > 0 && (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15))) return FK_ERR_WORKSPACE;
     cudaStream_t s = (cudaStream_t)stream;
     if (path == Path::few) return attention_few(p, a->dtype, a->starts == nullptr ? 1 : a->max_query, nullptr, s);
+    if (path == Path::tile) return attention_tile(p, a->dtype, nullptr, s);
     p.splits = any_splits(*a);
     const int cb = dtype_bytes(a->cache.dtype);
     const bool wide = a->cache.head_dim % 8 == 0 && groups_aligned(a->cache.key, a->cache.key_stride, 3, cb, cb == 1 ? 8 : 16);

@@ -13,7 +13,7 @@ struct AttnParams {
     int64_t qs[2], os[2];      // row, head
     int rows, q_heads, group;  // group = query heads per key/value head
     int window, sinks, zero_rest;
-    float scale_log2;          // scale * log2(e): scores are held as powers of two
+    float scale_log2;          // scale * log2(e): scores are held as powers of two; never zero, so that masked scores stay -infinity
     int splits;                // pieces of the key axis (shape-agnostic kernel)
     float* part;               // partial results
     int tile_tokens;           // tokens of an item of the kernels that work on tiles of tokens
@@ -36,11 +36,11 @@ struct RowSums {
     float acc[FK_MAX_HEAD_DIM / 32];
 };
 
-// One warp, one query row (fp32 in shared memory, already scaled by scale * log2 e): keys first, first + step, ... groups of 32
-// of the `count` visible ones.  One lane computes one key's score (no reduction per key); then the value rows are added one at
+// One warp, one query row (q(d) is element d times scale * log2 e, q(d >= head_dim) anything finite): groups first, first + step, ..
+// of 32 of the visible keys.  One lane computes one key's score (no reduction per key); then the value rows are added one at
 // a time, a lane per column.  Keys that are masked never enter any sum, whatever their rows hold.
-template <typename TC, bool WIDE>
-__device__ __forceinline__ void warp_row(const AttnParams& p, const float* q, int seq, int head, int pos, int first, int step, RowSums& r) {
+template <typename TC, bool WIDE, typename Q>
+__device__ __forceinline__ void warp_row(const AttnParams& p, const Q& q, int seq, int head, int pos, int first, int step, RowSums& r) {
     const int lane = threadIdx.x & 31, D = p.c.head_dim;
     const int end = min(pos + 1, p.c.max_pages * p.c.page_size);       // positions that the table does not hold are not visible
     const int lo = window_start(p, pos), n_sinks = max(0, min(p.sinks, min(lo, end)));
@@ -65,7 +65,7 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const float* q, in
                 float v[8];
                 load8<WIDE>(row + d, D - d, v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i & 3] = fmaf(q[d + i], v[i], sum[i & 3]);
+                for (int i = 0; i < 8; ++i) sum[i & 3] = fmaf(q(d + i), v[i], sum[i & 3]);
             }
             s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
             if (sizeof(TC) == 1) {
@@ -97,5 +97,8 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const float* q, in
 // Kernel for few query rows per key/value head (attention_few.cu).  need != null: only the workspace's size.
 bool attention_few_supported(const AttnParams& p, int dtype, int max_query);
 int attention_few(const AttnParams& p, int dtype, int max_query, size_t* need, cudaStream_t stream);
+// Kernel for tiles of 256 query rows (attention_tile.cu).
+bool attention_tile_supported(const AttnParams& p, int dtype);
+int attention_tile(const AttnParams& p, int dtype, size_t* need, cudaStream_t stream);
 
 }  // namespace fk

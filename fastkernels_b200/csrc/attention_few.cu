@@ -96,13 +96,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
 constexpr int kFewKeys = 16;                    // keys of a group
 constexpr int kFewLeast = 2;                    // shortest run of a warp, in groups
 
-// What a warp's partial result belongs to.
-struct PartHead {
-    int first_row, tokens, head, seq, pos0;
-    int begins, ends;                           // the run has the item's first / last key group
-    int last;                                   // warp of the grid whose run has the item's last key group
-};
-
 template <int D, int NT, typename TC>
 struct FewShape {
     static constexpr bool kCodes = FewOps<TC>::kCodes;
@@ -113,8 +106,7 @@ struct FewShape {
     static constexpr int kSlots = kFit > 8 ? 8 : kFit;
     static constexpr int kCols = 8 * NT;
     static constexpr int kPart = (D + 2) * kCols;                      // floats of a partial result: m, l per column, [column][D]
-    static constexpr int kQueryRow = FK_MAX_HEAD_DIM + 8;              // floats, for a row that is computed again
-    static constexpr int kSmem = kWarps * (kSlots * (kSlot + 16) + kQueryRow * 4) + 256;
+    static constexpr int kSmem = kWarps * kSlots * (kSlot + 16) + 256;
     static_assert(kSlots >= 3, "a slot being read and two on their way");
 };
 
@@ -128,14 +120,6 @@ __device__ __forceinline__ int slot_chunk(int row, int chunk) {
     return D >= 128 ? chunk ^ (((row >> 2) & 3) << 1) : chunk ^ ((row >> 2) & 3);
 }
 
-// Runs of the warps: [w * all / warps, (w + 1) * all / warps), or kFewLeast groups each if that is more.
-struct Runs {
-    int64_t all, warps;
-    __device__ __forceinline__ bool even() const { return all >= warps * kFewLeast; }
-    __device__ __forceinline__ int64_t begin(int64_t w) const { return even() ? w * all / warps : min(w * kFewLeast, all); }
-    __device__ __forceinline__ int warp_of(int64_t group) const { return (int)(even() ? ((group + 1) * warps - 1) / all : group / kFewLeast); }
-};
-
 template <int D, int NT, typename T, typename TC>
 __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention_few_kernel(const __grid_constant__ AttnParams p) {
     using S = FewShape<D, NT, TC>;
@@ -145,18 +129,17 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     constexpr float kShift = std::is_same<OT, __half>::value ? 14.f : 0.f;
     extern __shared__ __align__(128) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    unsigned char* mine = smem + 256 + warp * (kSlots * (S::kSlot + 16) + S::kQueryRow * 4);
+    unsigned char* mine = smem + 256 + warp * kSlots * (S::kSlot + 16);
     const uint32_t ring = smem_u32(mine);
     int2* meta = reinterpret_cast<int2*>(mine + kSlots * S::kSlot);
-    float* query_row = reinterpret_cast<float*>(mine + kSlots * (S::kSlot + 16));
     pdl_trigger();
     pdl_wait();
 
-    Runs runs{total_tiles<kFewKeys>(p, reinterpret_cast<int64_t*>(smem)), (int64_t)gridDim.x * S::kWarps};
+    Runs runs{total_tiles<kFewKeys>(p, reinterpret_cast<int64_t*>(smem)), (int64_t)gridDim.x * S::kWarps, kFewLeast};
     zero_blind_rows<T>(p);
     const int64_t me = (int64_t)blockIdx.x * S::kWarps + warp;
     PartHead* heads = reinterpret_cast<PartHead*>(p.part) + me * 2;
-    float* parts = p.part + runs.warps * 2 * (sizeof(PartHead) / 4) + me * 2 * S::kPart;
+    float* parts = p.part + runs.workers * 2 * (sizeof(PartHead) / 4) + me * 2 * S::kPart;
     const int64_t run0 = runs.begin(me), run1 = runs.begin(me + 1);
     if (lane < 2) heads[lane].begins = heads[lane].ends = -1;
     if (run0 >= run1) return;
@@ -473,7 +456,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 }
             if (tokens > 1 && __any_sync(kFull, odd))
                 for (int n = 0; n < cols; ++n)
-                    row_again<T, TC>(p, query_row, cur.seq, first_row + n / p.group, cur.pos0 + n / p.group, cur.head * p.group + n % p.group);
+                    row_again<T, TC>(p, cur.seq, first_row + n / p.group, cur.pos0 + n / p.group, cur.head * p.group + n % p.group);
         } else {
             const int which = at == run0 ? 0 : 1;
             float* part = parts + which * S::kPart;
@@ -490,7 +473,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                         for (int h = 0; h < 2; ++h) part[2 * S::kCols + n * D + dim_of(i, h)] = acc[nt][i][c + 2 * h] * unit;
                 }
             if (lane == 0)
-                heads[which] = PartHead{first_row, tokens, cur.head, cur.seq, cur.pos0, begins, ends, runs.warp_of(at - cur.k + cur.span.count - 1)};
+                heads[which] = PartHead{first_row, tokens, cur.head, cur.seq, cur.pos0, begins, ends, runs.worker_of(at - cur.k + cur.span.count - 1)};
         }
         at += steps;
         if (at < run1) cur.next_item(p);
@@ -504,7 +487,6 @@ template <int D, int NT, typename T, typename TC>
 __global__ void __launch_bounds__(32 * kJoinWarps) attention_few_join_kernel(const __grid_constant__ AttnParams p) {
     using S = FewShape<D, NT, TC>;
     __shared__ float sums[kJoinWarps][D + 2];
-    __shared__ float again[S::kQueryRow];
     pdl_trigger();
     pdl_wait();
     const int64_t warps = gridDim.x;
@@ -554,7 +536,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_few_join_kernel(con
         odd |= !(fabsf(v) < INFINITY);
         store_elem(out + c * 32 + lane, v);
     }
-    if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, again, h.seq, row, h.pos0 + n / p.group, qh);
+    if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, row, h.pos0 + n / p.group, qh);
 }
 
 // ---------------------------------------------------------------------------------------------

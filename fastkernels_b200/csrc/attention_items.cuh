@@ -192,20 +192,33 @@ __device__ __forceinline__ void zero_blind_rows(const AttnParams& p) {
 }
 
 // A row whose result is not finite, alone and exactly: in a tile of several tokens a key that one of them must not see may have
-// entered the row's product as 0 * infinity.  A whole warp; `q` is FK_MAX_HEAD_DIM + 8 floats of shared memory of its own.
+// entered the row's product as 0 * infinity.  A whole warp.
 template <typename T, typename TC>
-__device__ __noinline__ void row_again(const AttnParams& p, float* q, int seq, int row, int pos, int qh) {
+__device__ __noinline__ void row_again(const AttnParams& p, int seq, int row, int pos, int qh) {
     const int lane = threadIdx.x & 31, D = p.c.head_dim;
     const T* query = reinterpret_cast<const T*>(p.query) + row * p.qs[0] + qh * p.qs[1];
-    __syncwarp();
-    for (int d = lane; d < D + 8; d += 32) q[d] = d < D ? load_elem(query + d) * p.scale_log2 : 0.f;
-    __syncwarp();
     RowSums r;
-    warp_row<TC, false>(p, q, seq, qh / p.group, pos, 0, 1, r);
+    warp_row<TC, false>(p, [&](int d) { return d < D ? load_elem(query + d) * p.scale_log2 : 0.f; }, seq, qh / p.group, pos, 0, 1, r);
     T* out = reinterpret_cast<T*>(p.out) + row * p.os[0] + qh * p.os[1];
 #pragma unroll
     for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
         if (c * 32 + lane < D) store_elem(out + c * 32 + lane, r.l == 0.f ? 0.f : r.acc[c] / r.l);
 }
+
+// Runs of key tiles: worker w of `workers` has [w * all / workers, (w + 1) * all / workers), or `least` tiles if that is more.
+struct Runs {
+    int64_t all, workers;
+    int least;
+    __device__ __forceinline__ bool even() const { return all >= workers * least; }
+    __device__ __forceinline__ int64_t begin(int64_t w) const { return even() ? w * all / workers : min(w * least, all); }
+    __device__ __forceinline__ int worker_of(int64_t tile) const { return (int)(even() ? ((tile + 1) * workers - 1) / all : tile / least); }
+};
+
+// What a worker's partial result belongs to.
+struct PartHead {
+    int first_row, tokens, head, seq, pos0;
+    int begins, ends;                           // the run has the item's first / last key tile
+    int last;                                   // worker whose run has the item's last key tile
+};
 
 }  // namespace fk

@@ -1,0 +1,733 @@
+// Attention of chunks of new tokens over a paged cache on the tensor cores (tcgen05, two SMs per tile).
+//
+// A tile is 256 query rows (tokens x heads of the group) of one (sequence, key/value head) on a pair of SMs, 128 rows on each;
+// it walks over its keys 128 at a time:
+//   S[256, 128] = Q K^T          operands in shared memory, each SM holding 64 of the 128 keys
+//   P = 2^(S - m)                one thread per row: no exchange between threads, statistics in registers
+//   O[256, dim] += P V           P from tensor memory, where it replaces S; each SM holds half of the values' columns
+// The pair shares every key and value row, so an SM fetches half of them: at 256 dimensions one SM alone would need 64 bytes
+// of L2 per clock for 128 rows, and the whole chip gets 41 (11.8 TB/s measured); a pair needs 32.  It is also what lets the ring
+// hold 128-key tiles at 256 dimensions: 64 KB of queries + five slots of 32 KB.  Tensor memory: O (dim columns) and two S buffers
+// (128 columns each), so the products of the next tile run while this tile's softmax is taken.
+//
+// Warps of a block: 0..3 softmax (a row per thread, its sums, and the scaling of O), 4..7 producers (rows gathered through the page
+// table with cp.async, written in the 128-byte-swizzled layout; codes are converted to fp16 on the way), 8 issues the products
+// (in the pair's first block).  m is only raised when a row's maximum grows by more than 2^kLazy, which spares nearly all
+// passes over O.  Weights are rounded to the type of the operands (fp16 after a factor 2^7, which with 2^kLazy stays below
+// 2^15); sums are fp32.
+//
+// Key tiles of all tiles are dealt to the pairs in equal contiguous runs as in the few-row kernel; a run's first and last tile
+// may be partial, and attention_tile_join_kernel joins those in key order.
+
+#include <cfloat>
+#include <type_traits>
+
+#include "attention_items.cuh"
+#include "kernels.cuh"
+#include "tcgen05.cuh"
+
+namespace fk {
+
+constexpr int kTileRows = 256, kTileKeys = 128;
+constexpr int kTileThreads = 288;
+constexpr int kMetaRing = 8;
+
+template <int D, typename TC>
+struct TileShape {
+    static constexpr bool kCodes = sizeof(TC) == 1;
+    static constexpr int kQuery = 128 * D * 2;                       // bytes of a block's query rows
+    static constexpr int kSlot = 64 * D * 2;                         // 64 keys, or 128 values' half rows
+    static constexpr int kSlots = D == 256 ? (kCodes ? 4 : 5) : (kCodes ? 10 : 11);
+    static constexpr int kMeta = kMetaRing * (kCodes ? 2 * kTileKeys * 4 + 32 : 16);
+    static constexpr int kSmem = kQuery + kSlots * kSlot + kMeta + 4 * 128 * (kCodes ? 4 : 0) + 512;
+    static constexpr int kPart = (D + 2) * kTileRows;                // floats of a partial result: m, l per row, [row][D]
+    static_assert(kSmem <= 227 * 1024, "shared memory of a block");
+    static_assert(2 * kMetaRing >= kSlots + 3, "a key tile's description outlives its softmax");
+};
+
+struct TileBarriers {
+    uint64_t full[12], empty[12];
+    uint64_t q_full, q_empty, s_full[2], p_full[2], o_done, o_empty;
+    uint64_t keys_full[kMetaRing];
+    uint32_t tmem;
+    int abort_flag;
+    int64_t sums[kTileThreads / 32];
+};
+static_assert(sizeof(TileBarriers) <= 512, "fits behind the ring");
+
+// ---- cluster-wide barriers and two-SM tensor-core instructions -----------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// arrive at the barrier of the same offset in the pair's first block
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
+// bounded like mbar_wait, without its back-off: every waiter here has its own barrier and the next step depends on it
+__device__ __forceinline__ void wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (try_wait_cluster(bar, parity)) return;
+    const long long limit = *abort_flag ? kWaitCyclesAfterAbort : kWaitCycles;
+    const long long t0 = clock64();
+    while (!try_wait_cluster(bar, parity)) {
+        if (clock64() - t0 > limit) {
+            *abort_flag = 1;
+            return;
+        }
+    }
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t* dst) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+}
+__device__ __forceinline__ void pair_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void pair_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// arrive at the barrier of this offset in both blocks when all products issued so far are done
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
+}
+// K-major operand with rows of 64 elements (128 bytes, swizzled), 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
+    return ((uint64_t)(addr >> 4) & 0x3fffull) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// MN-major operand: rows of 64 columns (128 bytes, swizzled) per k, 8-k groups 1024 bytes apart, 64-column groups `group` bytes apart
+__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t group) {
+    return ((uint64_t)(addr >> 4) & 0x3fffull) | ((uint64_t)(group >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+template <typename OT>
+__device__ __forceinline__ constexpr uint32_t pair_idesc(uint32_t n, bool b_mn_major) {
+    constexpr uint32_t type = std::is_same<OT, __nv_bfloat16>::value ? 1u : 0u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((256u >> 4) << 24);
+}
+// 32 consecutive 32-bit columns of this thread's lane
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+    uint32_t* r = reinterpret_cast<uint32_t*>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+          "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+          "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+          "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+          "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tile_copy16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void sts16(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ float tile_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t tile_pack(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t tile_pack(float lo, float hi, __half) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 codes8_to_half(uint2 c) {
+    uint4 r;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xffffu), __NV_E4M3);
+        w[i] = (uint32_t)h.x | ((uint32_t)h.y << 16);
+    }
+    return r;
+}
+
+// Key of column / value row n of a tile, relative to its first: producer warp w looks up keys 32 w .. 32 w + 31 and puts 16 of
+// them into each block's half of the columns.
+__device__ __forceinline__ constexpr int key_of_column(int n) { return ((n & 63) >> 4) * 32 + (n >> 6) * 16 + (n & 15); }
+
+// D: dimensions of the tiles, a multiple of 128 not below head_dim (the rest is zero).  T: type of queries and results, TC: of the cache.
+template <int D, typename T, typename TC>
+__global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ AttnParams p) {
+    using S = TileShape<D, TC>;
+    constexpr bool kCodes = S::kCodes;
+    using OT = typename std::conditional<kCodes, __half, TC>::type;
+    constexpr bool kHalf = std::is_same<OT, __half>::value;
+    constexpr float kShift = kHalf ? 7.f : 0.f, kLazy = 8.f - (kCodes ? 1.f : 0.f);
+    constexpr int kSlots = S::kSlots;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    const uint32_t q_smem = smem_u32(smem), ring = q_smem + S::kQuery;
+    unsigned char* tail = smem + S::kQuery + kSlots * S::kSlot;
+    TileBarriers& bar = *reinterpret_cast<TileBarriers*>(tail);
+    uint32_t* key_mask = reinterpret_cast<uint32_t*>(tail + 512);                       // [kMetaRing][4]
+    float* key_scale = reinterpret_cast<float*>(tail + 512 + kMetaRing * 16);           // codes: [kMetaRing][128], by column
+    float* value_scale = key_scale + kMetaRing * kTileKeys;                             // codes: [kMetaRing][128], by value row
+    float* value_top = value_scale + kMetaRing * kTileKeys;                             // codes: [kMetaRing][4]
+    float* query_scale = value_top + kMetaRing * 4;                                     // codes: [4][128], by row of the block
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)cluster_rank();
+    const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kSlots; ++i) { mbar_init(&bar.full[i], 8); mbar_init(&bar.empty[i], 1); }
+        mbar_init(&bar.q_full, 8);
+        mbar_init(&bar.q_empty, 1);
+        for (int i = 0; i < 2; ++i) { mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 8); }
+        mbar_init(&bar.o_done, 1);
+        mbar_init(&bar.o_empty, 8);
+        for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], 4);
+        bar.abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == 8) pair_tmem_alloc(&bar.tmem);
+    pdl_trigger();
+    tc_fence_before_sync();
+    cluster_sync();                                  // barriers are there in both blocks
+    tc_fence_after_sync();
+    const uint32_t tmem = bar.tmem, tmem_s = tmem + (D == 256 ? 256 : 128);
+    volatile int* abort_flag = &bar.abort_flag;
+    pdl_wait();
+
+    const Runs runs{total_tiles<kTileKeys>(p, bar.sums), pairs, 1};
+    zero_blind_rows<T>(p);
+    const int64_t run0 = runs.begin(pair), run1 = runs.begin(pair + 1);
+    const int tiles = (int)(run1 - run0);
+    PartHead* heads = reinterpret_cast<PartHead*>(p.part) + 2 * (int64_t)pair;
+    float* parts = p.part + runs.workers * 2 * (sizeof(PartHead) / 4) + 2 * (int64_t)pair * S::kPart;
+    if (threadIdx.x == 0 && rank == 0) heads[0].begins = heads[0].ends = heads[1].begins = heads[1].ends = -1;
+
+    if (tiles > 0) {
+        ItemCursor<kTileKeys> c;
+        locate(p, run0, c);
+        const int dim = p.c.head_dim;
+        if (warp >= 4 && warp < 8) {
+            // ------------------------------------------------------------------------------------------------- producers
+            const int w = warp - 4;
+            int page = -1, in_page = 0;              // of key w * 32 + lane of the cursor's tile
+            auto look = [&] {
+                page = -1;
+                const int j = c.key0() + w * 32 + lane;
+                if (c.some_row_sees(p, j)) page = page_of(p.c, c.seq, j, in_page);
+            };
+            int x = 0;                               // loads so far
+            int arrived = 0;                         // of them announced
+            constexpr int kLag = 2;                  // loads in flight behind the newest
+            auto announce = [&](int upto) {          // loads below `upto` have landed for this thread
+                fence_async_proxy();
+                __syncwarp();
+                for (; arrived < upto; ++arrived)
+                    if (lane == 0) arrive_first(&bar.full[arrived % kSlots]);
+            };
+            auto load_query = [&](int segment) {     // 32 of the block's 128 rows per warp
+                if (!kCodes) asm volatile("cp.async.wait_group 0;" ::: "memory");
+                announce(x);                         // the products that read the old rows wait for these loads
+                wait_cluster(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
+                const int cols = c.tokens(p) * p.group, first_row = c.first_row(p);
+                constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks < 1 ? 1 : 32 / kChunks;
+                const bool flip = p.scale_log2 < 0.f;              // the scale's sign goes into the query
+                for (int i = 0; i < 32 / kAtOnce; ++i) {
+                    const int r = w * 32 + i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                    const int n = rank * 128 + r, tok = n / p.group;
+                    float v[8] = {};
+                    if (n < cols && chunk * 8 < dim) {
+                        const T* q = reinterpret_cast<const T*>(p.query) + (int64_t)(first_row + tok) * p.qs[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.qs[1] + chunk * 8;
+                        load8<true>(q, 8, v);
+                    }
+                    if (kCodes) {
+                        float most = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+#pragma unroll
+                        for (int o = kChunks / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
+                        const int e2 = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
+                        const float down = ldexpf(1.f, -e2);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] *= down;
+                        if (chunk == 0) query_scale[(segment & 3) * 128 + r] = fmaxf(ldexpf(fabsf(p.scale_log2), e2), FLT_MIN);
+                    }
+                    uint4 out;
+                    uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[e] = tile_pack(v[2 * e], v[2 * e + 1], OT{});
+                        if (flip) o[e] ^= 0x80008000u;
+                    }
+                    sts16(q_smem + (chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), out);
+                }
+                fence_async_proxy();
+                __syncwarp();
+                if (lane == 0) arrive_first(&bar.q_full);
+            };
+            // rows of a slot: keys take 16 of this warp's 32 (those of this block's half), values all 32 with half of their columns
+            constexpr int kKeyChunks = D / 8, kKeyAtOnce = 32 / kKeyChunks < 1 ? 1 : 32 / kKeyChunks;
+            constexpr int kValueChunks = D / 16, kValueAtOnce = 32 / kValueChunks;
+            auto key_addr = [&](uint32_t base, int i, int chunk) {
+                const int r = w * 16 + i;
+                return base + (chunk >> 3) * (64 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+            };
+            auto value_addr = [&](uint32_t base, int i, int chunk) {
+                const int r = (i >> 4) * 64 + w * 16 + (i & 15);
+                return base + (chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
+            };
+            auto load = [&](bool values, int64_t offset) {       // offset: bytes of this lane's row, < 0: no such row
+                const int slot = x % kSlots;
+                wait_cluster(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
+                const uint32_t base = ring + slot * S::kSlot;
+                const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
+                if (!values) {
+#pragma unroll
+                    for (int i0 = 0; i0 < 16; i0 += kKeyAtOnce) {
+                        const int i = i0 + lane / kKeyChunks, chunk = lane % kKeyChunks;
+                        const int64_t off = __shfl_sync(kFull, offset, rank * 16 + i);
+                        const bool there = off >= 0 && chunk * 8 < dim;
+                        if (kCodes) {
+                            const uint2 v = there ? *reinterpret_cast<const uint2*>(from + off + chunk * 8) : make_uint2(0, 0);
+                            sts16(key_addr(base, i, chunk), codes8_to_half(v));
+                        } else {
+                            tile_copy16(key_addr(base, i, chunk), there ? from + off + chunk * 16 : from, there ? 16 : 0);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i0 = 0; i0 < 32; i0 += kValueAtOnce) {
+                        const int i = i0 + lane / kValueChunks, chunk = lane % kValueChunks, at = rank * kValueChunks + chunk;
+                        const int64_t off = __shfl_sync(kFull, offset, i);
+                        const bool there = off >= 0 && at * 8 < dim;
+                        if (kCodes) {
+                            const uint2 v = there ? *reinterpret_cast<const uint2*>(from + off + at * 8) : make_uint2(0, 0);
+                            sts16(value_addr(base, i, chunk), codes8_to_half(v));
+                        } else {
+                            tile_copy16(value_addr(base, i, chunk), there ? from + off + at * 16 : from, there ? 16 : 0);
+                        }
+                    }
+                }
+                ++x;
+                if (kCodes) {
+                    announce(x);
+                } else {
+                    asm volatile("cp.async.commit_group;" ::: "memory");
+                    if (x > kLag) {
+                        asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                        announce(x - kLag);
+                    }
+                }
+            };
+            look();
+            int64_t value_offset = -1;
+            int segment = 0;
+            bool first = true;
+            for (int t = 0; t < tiles; ++t) {
+                if (first) {
+                    if (t > 0) load(true, value_offset);
+                    load_query(segment);
+                }
+                // this tile's rows: their offsets, which of them are there, their scales
+                const int64_t key_offset = page < 0 ? -1 : row_offset(p.c.key_stride, page, c.head, in_page) * (int64_t)sizeof(TC);
+                const int64_t next_value = page < 0 ? -1 : row_offset(p.c.value_stride, page, c.head, in_page) * (int64_t)sizeof(TC);
+                const unsigned rows = __ballot_sync(kFull, page >= 0);
+                const int meta = t % kMetaRing;
+                // a description is written anew only when its last reader has passed: the key slot of this tile, waited for below,
+                // was freed later than that (static_assert above); so wait for the slot first
+                wait_cluster(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
+                if (lane == 0) key_mask[meta * 4 + w] = rows;
+                if (kCodes) {
+                    const float ks = page < 0 ? 0.f : p.c.key_scale[row_offset(p.c.key_scale_stride, page, c.head, in_page)];
+                    const float vs = page < 0 ? 0.f : p.c.value_scale[row_offset(p.c.value_scale_stride, page, c.head, in_page)];
+                    const int n = (lane >> 4) * 64 + w * 16 + (lane & 15);
+                    key_scale[meta * kTileKeys + n] = ks;
+                    value_scale[meta * kTileKeys + n] = vs;
+                    const float top = warp_max(fabsf(vs));
+                    if (lane == 0) value_top[meta * 4 + w] = top;
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bar.keys_full[meta]);
+                // on to the next tile before the copies: its page numbers arrive meanwhile
+                const bool ends = c.k + 1 >= c.span.count;
+                if (t + 1 < tiles) {
+                    if (ends) c.next_item(p); else ++c.k;
+                    look();
+                } else {
+                    page = -1;
+                }
+                load(false, key_offset);
+                if (t > 0 && !first) load(true, value_offset);
+                value_offset = next_value;
+                first = ends;
+                if (ends) ++segment;
+            }
+            load(true, value_offset);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            announce(x);
+        } else if (warp == 8) {
+            // ------------------------------------------------------------------------------------------------- products
+            if (rank == 0 && lane == 0) {
+                constexpr uint32_t s_idesc = pair_idesc<OT>(kTileKeys, false), o_idesc = pair_idesc<OT>(D, true);
+                const int key_steps = (dim + 15) / 16;
+                int x = 0, segment = 0, o_segment = 0;
+                auto scores = [&](int t, bool ends) {
+                    const int slot = x % kSlots;
+                    wait_cluster(&bar.full[slot], (x / kSlots) & 1, abort_flag);
+                    tc_fence_after_sync();
+                    const uint32_t k = ring + slot * S::kSlot;
+                    for (int i = 0; i < key_steps; ++i)
+                        pair_mma_ss(tmem_s + (t & 1) * kTileKeys, desc_k_major(q_smem + (i >> 2) * (128 * 128) + (i & 3) * 32),
+                                    desc_k_major(k + (i >> 2) * (64 * 128) + (i & 3) * 32), s_idesc, i > 0);
+                    pair_commit(&bar.empty[slot]);
+                    pair_commit(&bar.s_full[t & 1]);
+                    if (ends) pair_commit(&bar.q_empty);
+                    ++x;
+                };
+                auto values = [&](int t, bool begins) {
+                    wait_cluster(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
+                    if (begins) {
+                        if (o_segment > 0) wait_cluster(&bar.o_empty, (o_segment - 1) & 1, abort_flag);
+                        ++o_segment;
+                    }
+                    const int slot = x % kSlots;
+                    wait_cluster(&bar.full[slot], (x / kSlots) & 1, abort_flag);
+                    tc_fence_after_sync();
+                    const uint32_t v = ring + slot * S::kSlot;
+#pragma unroll
+                    for (int i = 0; i < kTileKeys / 16; ++i)
+                        pair_mma_ts(tmem, tmem_s + (t & 1) * kTileKeys + i * 8, desc_mn_major(v + i * 2048, 128 * 128), o_idesc, !begins || i > 0);
+                    pair_commit(&bar.empty[slot]);
+                    pair_commit(&bar.o_done);
+                    ++x;
+                };
+                bool first = true, last_began = false;
+                for (int t = 0; t < tiles; ++t) {
+                    const bool ends = c.k + 1 >= c.span.count;
+                    if (first) {
+                        if (t > 0) values(t - 1, last_began);
+                        wait_cluster(&bar.q_full, segment & 1, abort_flag);
+                        ++segment;
+                    }
+                    scores(t, ends || t + 1 == tiles);
+                    if (t > 0 && !first) values(t - 1, last_began);
+                    last_began = first;
+                    first = ends;
+                    if (t + 1 < tiles) {
+                        if (ends) c.next_item(p); else ++c.k;
+                    }
+                }
+                values(tiles - 1, last_began);
+            }
+        } else {
+            // ------------------------------------------------------------------------------------------------- softmax
+            const int r = warp * 32 + lane, n = rank * 128 + r;          // row of the block, of the pair
+            const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+            const uint32_t o_addr = tmem + lanes;
+            float m = -INFINITY, l = 0.f, top = 0.f, qscale = fabsf(p.scale_log2);
+            bool begins = true;                                          // of this run's part of the item
+            int segment = 0;
+            int64_t at = run0;                                           // first tile of the segment
+            int began_k = c.k;
+            for (int t = 0; t < tiles; ++t, ++at) {
+                const int tok = n / p.group;
+                const int pos = c.pos0 + tok, meta = t % kMetaRing;
+                const int key0 = c.key0();
+                wait_cluster(&bar.keys_full[meta], (t / kMetaRing) & 1, abort_flag);
+                wait_cluster(&bar.s_full[t & 1], (t >> 1) & 1, abort_flag);
+                tc_fence_after_sync();
+                const uint32_t s_addr = tmem_s + lanes + (t & 1) * kTileKeys;
+                float s[kTileKeys];
+#pragma unroll
+                for (int i = 0; i < kTileKeys; i += 32) tmem_ld32(s_addr + i, s + i);
+                tmem_wait_ld();
+                if (begins) {
+                    m = -INFINITY;
+                    l = 0.f;
+                    top = 0.f;
+                    if (kCodes) qscale = query_scale[(segment & 3) * 128 + r];
+                    began_k = c.k;
+                }
+                if (kCodes) {
+                    const float4* ks = reinterpret_cast<const float4*>(key_scale + meta * kTileKeys);
+#pragma unroll
+                    for (int i = 0; i < kTileKeys / 4; ++i) {
+                        const float4 f = ks[i];
+                        s[4 * i] *= f.x; s[4 * i + 1] *= f.y; s[4 * i + 2] *= f.z; s[4 * i + 3] *= f.w;
+                    }
+                }
+                // ---- masks
+                const uint4 there = *reinterpret_cast<const uint4*>(key_mask + meta * 4);
+                const bool complete = (there.x & there.y & there.z & there.w) == 0xffffffffu;
+                if (!complete || !(key0 + kTileKeys - 1 <= c.pos0 && (p.window == 0 || key0 >= window_start(p, c.pos1) || key0 + kTileKeys <= p.sinks))) {
+                    const int hi = pos - key0, lo = p.window > 0 ? pos - p.window - key0 : -1, sink = p.window > 0 ? p.sinks - key0 : 0;
+                    const uint32_t bits[4] = {there.x, there.y, there.z, there.w};
+#pragma unroll
+                    for (int i = 0; i < kTileKeys; ++i) {
+                        const int k = key_of_column(i);
+                        if (!((bits[k >> 5] >> (k & 31)) & 1u) || k > hi || (k <= lo && k >= sink)) s[i] = -INFINITY;
+                    }
+                }
+                // ---- maximum; the base of the powers only moves when it has to
+                float most = s[0];
+#pragma unroll
+                for (int i = 1; i < kTileKeys; ++i) most = fmaxf(most, s[i]);
+                most *= qscale;
+                float alpha = 1.f;
+                const float m_new = most > m + kLazy ? most : m;
+                if (m_new > m) alpha = m == -INFINITY ? 0.f : tile_exp2(m - m_new);
+                m = m_new;
+                float unit = 1.f;
+                if (kCodes) {
+                    const float4 vt = *reinterpret_cast<const float4*>(value_top + meta * 4);
+                    const float tile_top = fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w));
+                    if (tile_top > 2.f * top) {                          // the same in all rows
+                        unit = top > 0.f ? top / tile_top : 0.f;
+                        top = tile_top;
+                    }
+                }
+                if (!begins) {
+                    const float factor = alpha * unit;
+                    if (__any_sync(kFull, factor != 1.f)) {
+                        wait_cluster(&bar.o_done, (t - 1) & 1, abort_flag);
+                        tc_fence_after_sync();
+#pragma unroll 1
+                        for (int i = 0; i < D; i += 32) {
+                            float o[32];
+                            tmem_ld32(o_addr + i, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] *= factor;
+                            tmem_st32(o_addr + i, reinterpret_cast<const uint32_t*>(o));
+                        }
+                    }
+                    l *= alpha;
+                }
+                // ---- weights
+                const float base = m == -INFINITY ? 0.f : m - kShift;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                uint32_t w[32];
+                const float inv_top = kCodes ? (top > 0.f ? 1.f / top : 1.f) : 1.f;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int e = half * 64 + 2 * i;
+                        float a = tile_exp2(fmaf(s[e], qscale, -base)), b = tile_exp2(fmaf(s[e + 1], qscale, -base));
+                        sum[i & 3] += a + b;
+                        if (kCodes) {
+                            const float2 vs = *reinterpret_cast<const float2*>(value_scale + meta * kTileKeys + e);
+                            a *= vs.x * inv_top;
+                            b *= vs.y * inv_top;
+                        }
+                        w[i] = tile_pack(a, b, OT{});
+                    }
+                    tmem_st32(s_addr + half * 32, w);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tmem_wait_st();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) arrive_first(&bar.p_full[t & 1]);
+                // ---- the end of the item, or of the run
+                const bool ends = c.k + 1 >= c.span.count;
+                if (ends || t + 1 == tiles) {
+                    wait_cluster(&bar.o_done, t & 1, abort_flag);
+                    tc_fence_after_sync();
+                    const int cols = c.tokens(p) * p.group, first_row = c.first_row(p);
+                    const bool whole = ends && began_k == 0;
+                    const float scale_out = kCodes ? (top > 0.f ? top : 1.f) : 1.f;
+                    const int which = at - (c.k - began_k) == run0 ? 0 : 1;
+                    float* part = parts + which * (int64_t)S::kPart;
+                    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first_row + tok) * p.os[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.os[1];
+                    const float inv = l == 0.f ? 0.f : scale_out / l;
+                    const bool failed = *abort_flag != 0;
+                    bool odd = false;
+                    const bool wide = (dim & 7) == 0 && ((p.os[0] | p.os[1]) & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+#pragma unroll 1
+                    for (int i = 0; i < D; i += 32) {
+                        float o[32];
+                        tmem_ld32(o_addr + i, o);
+                        tmem_wait_ld();
+                        if (n < cols && i < dim) {
+                            if (whole) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) {
+                                    o[e] = l == 0.f ? 0.f : o[e] * inv;
+                                    if (i + e < dim) odd |= !(fabsf(o[e]) < INFINITY);
+                                    if (failed) o[e] = NAN;
+                                }
+#pragma unroll
+                                for (int e = 0; e < 32; e += 8)
+                                    if (i + e < dim) {
+                                        const float (&v)[8] = *reinterpret_cast<const float (*)[8]>(o + e);
+                                        if (wide) store8<true>(out + i + e, 8, v); else store8<false>(out + i + e, dim - i - e, v);
+                                    }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 32; e += 4)
+                                    *reinterpret_cast<float4*>(part + 2 * kTileRows + (int64_t)n * D + i + e) =
+                                        failed ? make_float4(NAN, NAN, NAN, NAN) : make_float4(o[e] * scale_out, o[e + 1] * scale_out, o[e + 2] * scale_out, o[e + 3] * scale_out);
+                            }
+                        }
+                    }
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) arrive_first(&bar.o_empty);
+                    if (whole) {
+                        // `odd` rows of a tile with several tokens once more
+                        unsigned again = c.tokens(p) > 1 && !failed ? __ballot_sync(kFull, odd) : 0u;
+                        while (again) {
+                            const int i = __ffs(again) - 1;
+                            again &= again - 1;
+                            const int row = rank * 128 + warp * 32 + i, rt = row / p.group;
+                            row_again<T, TC>(p, c.seq, first_row + rt, c.pos0 + rt, c.head * p.group + row - rt * p.group);
+                        }
+                    } else {
+                        if (n < cols) { part[n] = m; part[kTileRows + n] = l; }
+                        if (rank == 0 && threadIdx.x == 0)
+                            heads[which] = PartHead{first_row, c.tokens(p), c.head, c.seq, c.pos0, began_k == 0, ends, runs.worker_of(at - c.k + c.span.count - 1)};
+                    }
+                    ++segment;
+                }
+                begins = ends;
+                if (t + 1 < tiles) {
+                    if (ends) c.next_item(p); else ++c.k;
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    cluster_sync();                                  // nothing more arrives at either block's barriers
+    if (warp == 8) {
+        tc_fence_after_sync();
+        pair_tmem_dealloc(tmem);
+    }
+}
+
+// Joins the parts of one tile: block (pair whose run has the tile's beginning, 8 rows), a warp per row.
+template <int D, typename T, typename TC>
+__global__ void __launch_bounds__(256) attention_tile_join_kernel(const __grid_constant__ AttnParams p) {
+    using S = TileShape<D, TC>;
+    pdl_trigger();
+    pdl_wait();
+    const int64_t pairs = gridDim.x;
+    const PartHead* heads = reinterpret_cast<const PartHead*>(p.part);
+    const float* parts = p.part + pairs * 2 * (sizeof(PartHead) / 4);
+    const int w0 = blockIdx.x, lane = threadIdx.x & 31, n = blockIdx.y * 8 + (threadIdx.x >> 5);
+    int which = -1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (heads[2 * w0 + i].begins == 1 && heads[2 * w0 + i].ends == 0) which = i;
+    if (which < 0) return;
+    const PartHead h = heads[2 * w0 + which];
+    if (n >= h.tokens * p.group) return;
+    const int count = h.last - w0 + 1;
+    auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * w0 + which : 2 * (w0 + i)) * S::kPart; };
+    float m = -INFINITY;
+    for (int i = lane; i < count; i += 32) m = fmaxf(m, part(i)[n]);
+    m = warp_max(m);
+    const float base = m == -INFINITY ? 0.f : m;
+    float l = 0.f, acc[D / 32] = {};
+    for (int i = 0; i < count; ++i) {
+        const float* one = part(i);
+        const float weight = tile_exp2(one[n] - base);
+        l = fmaf(weight, one[kTileRows + n], l);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+            if (c * 32 + lane < p.c.head_dim) acc[c] = fmaf(weight, one[2 * kTileRows + (int64_t)n * D + c * 32 + lane], acc[c]);
+    }
+    const int tok = n / p.group, qh = h.head * p.group + n - tok * p.group;
+    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(h.first_row + tok) * p.os[0] + (int64_t)qh * p.os[1];
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+        if (c * 32 + lane < p.c.head_dim) {
+            const float v = l == 0.f ? 0.f : acc[c] / l;
+            odd |= !(fabsf(v) < INFINITY);
+            store_elem(out + c * 32 + lane, v);
+        }
+    if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, h.first_row + tok, h.pos0 + tok, qh);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------
+template <int D, typename T, typename TC>
+static int tile(AttnParams p, size_t* need, cudaStream_t stream) {
+    using S = TileShape<D, TC>;
+    p.tile_tokens = kTileRows / p.group;
+    const int pairs = sm_count() / 2;
+    if (need) {
+        *need = (size_t)pairs * 2 * (sizeof(PartHead) + S::kPart * sizeof(float));
+        return FK_OK;
+    }
+    auto kern = attention_tile_kernel<D, T, TC>;
+    FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), "attention (tile) attr");
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(2 * pairs);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    FK_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p), "attention (tile) launch");
+    FK_LAUNCH_OK("attention (tile) launch");
+    FK_CUDA_OK(launch_pdl(attention_tile_join_kernel<D, T, TC>, dim3((unsigned)pairs, kTileRows / 8), dim3(256), 0, stream, p), "attention (tile) join launch");
+    FK_LAUNCH_OK("attention (tile) join launch");
+    return FK_OK;
+}
+
+template <typename T, typename TC>
+static int tile_dim(const AttnParams& p, size_t* need, cudaStream_t stream) {
+    return p.c.head_dim <= 128 ? tile<128, T, TC>(p, need, stream) : tile<256, T, TC>(p, need, stream);
+}
+
+bool attention_tile_supported(const AttnParams& p, int dtype) {
+    if (dtype != FK_BF16 && dtype != FK_F16) return false;
+    if (p.c.head_dim % 8 != 0 || p.group > kTileRows) return false;
+    const int cb = dtype_bytes(p.c.dtype), align = cb == 1 ? 8 : 16;
+    return groups_aligned(p.c.key, p.c.key_stride, 3, cb, align) && groups_aligned(p.c.value, p.c.value_stride, 3, cb, align) && groups_aligned(p.query, p.qs, 2, 2, 16);
+}
+
+// need != null: only the workspace's size
+int attention_tile(const AttnParams& p, int dtype, size_t* need, cudaStream_t stream) {
+    if (dtype == FK_BF16)
+        return p.c.dtype == FK_E4M3 ? tile_dim<__nv_bfloat16, __nv_fp8_e4m3>(p, need, stream) : tile_dim<__nv_bfloat16, __nv_bfloat16>(p, need, stream);
+    return p.c.dtype == FK_E4M3 ? tile_dim<__half, __nv_fp8_e4m3>(p, need, stream) : tile_dim<__half, __half>(p, need, stream);
+}
+
+}  // namespace fk
