@@ -23,6 +23,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 from typing import Any, Optional
 
 import torch
@@ -32,11 +33,39 @@ from ._lib import AttentionCall, KvCache, KvRows
 from .moe import _DTYPES
 
 _CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.FK_E4M3}
+_E4M3 = torch.float8_e4m3fn
+
+# The ABI's structs are filled with one pack each (setting their fields one by one costs more than the checks); the formats
+# are the fields of _lib.KvCache, KvRows and AttentionCall in order, without padding.
+_CACHE_FIELDS = "8i13q6Q"
+_ROW_FIELDS = "2Q4i4qQ"
+_CALL_FIELDS = "2Q4i4qQf3iIi2Q"
+_PACK_CACHE, _PACK_ROWS, _PACK_CALL = (struct.Struct("=" + f) for f in (_CACHE_FIELDS, _ROW_FIELDS, _CALL_FIELDS))
+_CACHE_BYTES = C.sizeof(KvCache)
+assert (_PACK_CACHE.size, _PACK_ROWS.size, _PACK_CALL.size) == (_CACHE_BYTES, C.sizeof(KvRows), C.sizeof(AttentionCall) - _CACHE_BYTES)
 
 
-def _on(device: torch.device):
-    """Context in which `device` is the current one; the stream to launch on is that device's current stream."""
-    return torch.cuda.device(device)
+def _stream(device: torch.device) -> int:
+    """The device's current stream, as the ABI takes it."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _On:
+    """Makes `device` the current one for a launch, at no cost where it is already (torch.cuda.device costs microseconds)."""
+
+    __slots__ = ("index", "before")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.before)
 
 
 def _check_index(t: Any, what: str, shape: tuple, device: torch.device) -> None:
@@ -44,69 +73,73 @@ def _check_index(t: Any, what: str, shape: tuple, device: torch.device) -> None:
         raise ValueError(f"{what} must be int32 with shape {list(shape)}, got {t.dtype} {list(t.shape)}")
     if t.device != device:
         raise ValueError(f"{what} must be on {device}")
-    if shape and shape[-1] > 1 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and shape[-1] > 1:
         raise ValueError(f"{what} must be contiguous in its last dimension")
 
 
-def _fill_cache(c: KvCache, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale) -> None:
-    """Checks the description of a cache and a ragged batch, and fills the ABI's struct."""
+def _pack_cache(into: Any, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale) -> tuple:
+    """Checks the description of a cache and a ragged batch and writes it to the front of a struct of the ABI; returns
+    (kv_heads, head_dim, seqs)."""
     if not key_cache.is_cuda:
         raise ValueError("key_cache must be a CUDA tensor")
-    if key_cache.ndim != 4 or value_cache.shape != key_cache.shape:
+    shape, device, dtype = key_cache.shape, key_cache.device, key_cache.dtype
+    if len(shape) != 4 or value_cache.shape != shape:
         raise ValueError("key_cache and value_cache must have the same shape [pages, kv_heads, page_size, head_dim]")
-    device, dtype = key_cache.device, key_cache.dtype
     if value_cache.device != device or value_cache.dtype != dtype:
         raise ValueError("key_cache and value_cache must have the same dtype and device")
     code = _CACHE_DTYPES.get(dtype)
     if code is None:
         raise ValueError(f"the cache must be float32, bfloat16, float16 or float8_e4m3fn, got {dtype}")
-    pages, heads, page_size, dim = key_cache.shape
+    pages, heads, page_size, dim = shape
     if pages < 1 or heads < 1 or page_size < 1:
         raise ValueError("the cache must have at least one page, head and row per page")
     if dim < 1 or dim > _lib.MAX_HEAD_DIM:
         raise ValueError(f"head_dim must be between 1 and {_lib.MAX_HEAD_DIM}")
-    ks, vs = key_cache.stride(), value_cache.stride()
-    if dim > 1 and (ks[3] != 1 or vs[3] != 1):
+    k0, k1, k2, k3 = key_cache.stride()
+    v0, v1, v2, v3 = value_cache.stride()
+    if dim > 1 and (k3 != 1 or v3 != 1):
         raise ValueError("key_cache and value_cache must be contiguous in their last dimension")
     if page_table.ndim != 2:
         raise ValueError("page_table must have shape [seqs, max_pages]")
-    seqs, max_pages = page_table.shape
-    _check_index(page_table, "page_table", (seqs, max_pages), device)
+    seqs, max_pages = table_shape = page_table.shape
+    _check_index(page_table, "page_table", table_shape, device)
     _check_index(lengths, "lengths", (seqs,), device)
     if max_pages * page_size >= 1 << 31:
         raise ValueError("page_table must hold less than 2^31 positions per sequence")
     if query_starts is not None:
         _check_index(query_starts, "query_starts", (seqs + 1,), device)
-    if dtype == torch.float8_e4m3fn:
+    if dtype == _E4M3:
         for name, t in (("key_scale", key_scale), ("value_scale", value_scale)):
             if t is None:
                 raise ValueError(f"{name} is required with a float8_e4m3fn cache")
-            if t.dtype != torch.float32 or t.shape != key_cache.shape[:3] or t.device != device:
+            if t.dtype != torch.float32 or t.shape != shape[:3] or t.device != device:
                 raise ValueError(f"{name} must be float32 [pages, kv_heads, page_size] on the cache's device")
-        c.key_scale_stride[:] = key_scale.stride()
-        c.value_scale_stride[:] = value_scale.stride()
-        c.key_scale, c.value_scale = key_scale.data_ptr(), value_scale.data_ptr()
-    elif key_scale is not None or value_scale is not None:
-        raise ValueError("key_scale and value_scale belong to a float8_e4m3fn cache")
-    c.pages, c.kv_heads, c.page_size, c.head_dim, c.dtype = pages, heads, page_size, dim, code
-    c.seqs, c.max_pages, c.table_stride = seqs, max_pages, page_table.stride(0)
-    c.key_stride[:] = ks[:3]
-    c.value_stride[:] = vs[:3]
-    c.key, c.value = key_cache.data_ptr(), value_cache.data_ptr()
-    c.page_table, c.lengths = page_table.data_ptr(), lengths.data_ptr()
+        scales = (*key_scale.stride(), *value_scale.stride())
+        scale_at = key_scale.data_ptr(), value_scale.data_ptr()
+    else:
+        if key_scale is not None or value_scale is not None:
+            raise ValueError("key_scale and value_scale belong to a float8_e4m3fn cache")
+        scales, scale_at = (0, 0, 0, 0, 0, 0), (0, 0)
+    _PACK_CACHE.pack_into(into, 0, pages, heads, page_size, dim, code, seqs, max_pages, 0, page_table.stride(0), k0, k1, k2, v0, v1, v2, *scales,
+                          key_cache.data_ptr(), value_cache.data_ptr(), *scale_at, page_table.data_ptr(), lengths.data_ptr())
+    return heads, dim, seqs
 
 
-def _check_rows(t: Any, what: str, rows: Optional[int], heads: int, key_cache) -> None:
-    if t.ndim != 3 or (rows is not None and t.shape[0] != rows) or t.shape[1] != heads or t.shape[2] != key_cache.shape[3]:
-        raise ValueError(f"{what} must have shape [{'rows' if rows is None else rows}, {heads}, {key_cache.shape[3]}], got {list(t.shape)}")
+def _check_rows(t: Any, what: str, rows: int, heads: int, dim: int, key_cache) -> int:
+    """Checks `[rows, heads, dim]` rows of a call against the cache; returns the code of their dtype."""
+    if t.shape != (rows, heads, dim):
+        raise ValueError(f"{what} must have shape [{rows}, {heads}, {dim}], got {list(t.shape)}")
     if t.device != key_cache.device:
         raise ValueError(f"{what} must be on the cache's device")
-    if t.dtype not in _DTYPES:
-        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
-    if key_cache.dtype != torch.float8_e4m3fn and t.dtype != key_cache.dtype:
-        raise ValueError(f"{what} must have the cache's dtype {key_cache.dtype}, got {t.dtype}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    dtype = t.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, got {dtype}")
+    if dtype != key_cache.dtype and key_cache.dtype != _E4M3:
+        raise ValueError(f"{what} must have the cache's dtype {key_cache.dtype}, got {dtype}")
+    if dim > 1 and t.stride(2) != 1:
         raise ValueError(f"{what} must be contiguous in its last dimension")
+    return code
 
 
 def _span(t: Any) -> tuple[int, int]:
@@ -132,11 +165,11 @@ def _overlap(a: Any, b: Any) -> bool:
     return True
 
 
-def _fill_rows(r: KvRows, key, value, query_starts, zero_rest: bool) -> None:
-    r.key, r.value, r.dtype, r.rows, r.zero_rest = key.data_ptr(), value.data_ptr(), _DTYPES[key.dtype], key.shape[0], zero_rest
-    r.key_stride[:] = key.stride()[:2]
-    r.value_stride[:] = value.stride()[:2]
-    r.starts = None if query_starts is None else query_starts.data_ptr()
+def _pack_rows(into: KvRows, key, value, code: int, query_starts, zero_rest: bool) -> None:
+    k0, k1, _ = key.stride()
+    v0, v1, _ = value.stride()
+    _PACK_ROWS.pack_into(into, 0, key.data_ptr(), value.data_ptr(), code, key.shape[0], zero_rest, 0, k0, k1, v0, v1,
+                         0 if query_starts is None else query_starts.data_ptr())
 
 
 def paged_kv_append(key: Any, value: Any, key_cache: Any, value_cache: Any, page_table: Any, lengths: Any, query_starts: Any = None, *,
@@ -149,14 +182,15 @@ def paged_kv_append(key: Any, value: Any, key_cache: Any, value_cache: Any, page
     x * 448 / max.  A row with an infinity or a NaN reads back as NaN.  Rows behind the last sequence are ignored.
     """
     c, r = KvCache(), KvRows()
-    _fill_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
-    _check_rows(key, "key", None, c.kv_heads, key_cache)
-    _check_rows(value, "value", key.shape[0], c.kv_heads, key_cache)
-    if key.dtype != value.dtype:
+    heads, dim, _ = _pack_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    rows = key.shape[0]
+    code = _check_rows(key, "key", rows, heads, dim, key_cache)
+    if code != _check_rows(value, "value", rows, heads, dim, key_cache):
         raise ValueError("key and value must have the same dtype")
-    _fill_rows(r, key, value, query_starts, False)
-    with _on(key_cache.device):
-        _lib.check(_lib.load().fk_kv_append(C.byref(c), C.byref(r), torch.cuda.current_stream().cuda_stream), "fk_kv_append")
+    _pack_rows(r, key, value, code, query_starts, False)
+    device = key_cache.device
+    with _On(device):
+        _lib.check(_lib.load().fk_kv_append(C.byref(c), C.byref(r), _stream(device)), "fk_kv_append")
 
 
 def paged_kv_gather(key_cache: Any, value_cache: Any, page_table: Any, lengths: Any, query_starts: Any, rows: int, *,
@@ -168,25 +202,26 @@ def paged_kv_gather(key_cache: Any, value_cache: Any, page_table: Any, lengths: 
     and keeps what it holds behind the last sequence; new tensors hold zeros there.
     """
     c, r = KvCache(), KvRows()
-    _fill_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    heads, dim, _ = _pack_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
     if rows < 0:
         raise ValueError("rows must not be negative")
     if dtype is None:
-        dtype = out[0].dtype if out is not None else torch.bfloat16 if key_cache.dtype == torch.float8_e4m3fn else key_cache.dtype
-    with _on(key_cache.device):
+        dtype = out[0].dtype if out is not None else torch.bfloat16 if key_cache.dtype == _E4M3 else key_cache.dtype
+    device = key_cache.device
+    with _On(device):
         if out is None:
-            key = torch.empty((rows, c.kv_heads, c.head_dim), device=key_cache.device, dtype=dtype)
-            value = torch.empty_like(key)
+            key = torch.empty((rows, heads, dim), device=device, dtype=dtype)
+            value = torch.empty((rows, heads, dim), device=device, dtype=dtype)
         else:
             key, value = out
-        _check_rows(key, "key" if out is None else "out[0]", rows, c.kv_heads, key_cache)
-        _check_rows(value, "value" if out is None else "out[1]", rows, c.kv_heads, key_cache)
+        code = _check_rows(key, "key" if out is None else "out[0]", rows, heads, dim, key_cache)
+        _check_rows(value, "value" if out is None else "out[1]", rows, heads, dim, key_cache)
         if key.dtype != dtype or value.dtype != dtype:
             raise ValueError(f"out must have dtype {dtype}")
         if out is not None and (_overlap(key, value) or any(_overlap(a, b) for a in out for b in (key_cache, value_cache))):
             raise ValueError("out must not overlap the cache, nor its two tensors each other")
-        _fill_rows(r, key, value, query_starts, out is None)
-        _lib.check(_lib.load().fk_kv_gather(C.byref(c), C.byref(r), torch.cuda.current_stream().cuda_stream), "fk_kv_gather")
+        _pack_rows(r, key, value, code, query_starts, out is None)
+        _lib.check(_lib.load().fk_kv_gather(C.byref(c), C.byref(r), _stream(device)), "fk_kv_gather")
     return key, value
 
 
@@ -206,13 +241,12 @@ def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: An
     Sums and softmax statistics are fp32.
     """
     call = AttentionCall()
-    c = call.cache
-    _fill_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
-    if query.ndim != 3 or query.shape[1] < 1 or query.shape[1] % c.kv_heads:
+    kv_heads, dim, seqs = _pack_cache(call, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    if query.ndim != 3 or query.shape[1] < 1 or query.shape[1] % kv_heads:
         raise ValueError("query must have shape [rows, q_heads, head_dim] with q_heads a multiple of the cache's kv_heads")
-    rows, q_heads, dim = query.shape
-    _check_rows(query, "query", rows, q_heads, key_cache)
-    if query_starts is None and rows > c.seqs:
+    rows, q_heads, _ = query.shape
+    code = _check_rows(query, "query", rows, q_heads, dim, key_cache)
+    if query_starts is None and rows > seqs:
         raise ValueError("query has more rows than there are sequences: query_starts is required")
     if window < 0 or sinks < 0 or max_query < 0:
         raise ValueError("window, sinks and max_query must not be negative")
@@ -224,29 +258,27 @@ def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: An
         scale = dim ** -0.5
     elif not math.isfinite(scale):
         raise ValueError("scale must be finite")
-    with _on(query.device):
-        call.zero_rest = out is None
-        if out is None:
-            out = torch.empty((rows, q_heads, dim), device=query.device, dtype=query.dtype)
+    device, fresh = query.device, out is None
+    lib = _lib.load()
+    with _On(device):
+        if fresh:
+            out = torch.empty((rows, q_heads, dim), device=device, dtype=query.dtype)
         else:
-            _check_rows(out, "out", rows, q_heads, key_cache)
-            if out.dtype != query.dtype:
+            if _check_rows(out, "out", rows, q_heads, dim, key_cache) != code:
                 raise ValueError("out must have the query's dtype")
             if any(_overlap(out, t) for t in (query, key_cache, value_cache)):
                 raise ValueError("out must not overlap the query or the cache")
-        call.query, call.out, call.dtype, call.rows, call.q_heads = query.data_ptr(), out.data_ptr(), _DTYPES[query.dtype], rows, q_heads
-        call.max_query = 1 if query_starts is None else min(max_query, rows)
-        call.query_stride[:] = query.stride()[:2]
-        call.out_stride[:] = out.stride()[:2]
-        call.starts = None if query_starts is None else query_starts.data_ptr()
-        call.scale, call.window, call.sinks, call.flags = scale, window, sinks, flags
-        lib = _lib.load()
-        need = lib.fk_paged_attention_workspace_bytes(C.byref(call))
-        # a new workspace per call: the allocator orders its reuse with the stream, and gives captured calls their own
-        ws = torch.empty(need, device=query.device, dtype=torch.uint8) if need else None
+        q0, q1, _ = query.stride()
+        o0, o1, _ = out.stride()
+        _PACK_CALL.pack_into(call, _CACHE_BYTES, query.data_ptr(), out.data_ptr(), code, rows, q_heads, 1 if query_starts is None else min(max_query, rows),
+                             q0, q1, o0, o1, 0 if query_starts is None else query_starts.data_ptr(), scale, window, sinks, fresh, flags, 0, 0, 0)
+        ref = C.byref(call)
+        need = lib.fk_paged_attention_workspace_bytes(ref)
         if need:
+            # a new workspace per call: the allocator orders its reuse with the stream, and gives captured calls their own
+            ws = torch.empty(need, device=device, dtype=torch.uint8)
             call.workspace, call.workspace_bytes = ws.data_ptr(), need
-        _lib.check(lib.fk_paged_attention(C.byref(call), torch.cuda.current_stream().cuda_stream), "fk_paged_attention")
+        _lib.check(lib.fk_paged_attention(ref, _stream(device)), "fk_paged_attention")
     return out
 
 
