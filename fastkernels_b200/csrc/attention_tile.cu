@@ -29,8 +29,9 @@
 namespace fk {
 
 constexpr int kTileRows = 256, kTileKeys = 128;
-constexpr int kTileThreads = 288;
+constexpr int kTileThreads = 448;       // 14 warps of up to 128 registers
 constexpr int kMetaRing = 8;
+constexpr int kMmaWarp = 12, kEdgeWarp = 13;
 
 template <int D, typename TC>
 struct TileShape {
@@ -39,21 +40,23 @@ struct TileShape {
     static constexpr int kSlot = 64 * D * 2;                         // 64 keys, or 128 values' half rows
     static constexpr int kSlots = D == 256 ? (kCodes ? 4 : 5) : (kCodes ? 10 : 11);
     static constexpr int kMeta = kMetaRing * (kCodes ? 2 * kTileKeys * 4 + 32 : 16);
-    static constexpr int kSmem = kQuery + kSlots * kSlot + kMeta + 4 * 128 * (kCodes ? 4 : 0) + 512;
+    static constexpr int kExchange = 2 * 2 * 128 * 4;                // between the two threads of a row
+    static constexpr int kSmem = kQuery + kSlots * kSlot + 640 + kMeta + kExchange + 4 * 128 * (kCodes ? 4 : 0);
+
     static constexpr int kPart = (D + 2) * kTileRows;                // floats of a partial result: m, l per row, [row][D]
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
     static_assert(2 * kMetaRing >= kSlots + 3, "a key tile's description outlives its softmax");
 };
 
 struct TileBarriers {
-    uint64_t full[12], empty[12];
+    uint64_t full[12], empty[12], landed[12];
     uint64_t q_full, q_empty, s_full[2], p_full[2], o_done, o_empty;
     uint64_t keys_full[kMetaRing];
     uint32_t tmem;
     int abort_flag;
     int64_t sums[kTileThreads / 32];
 };
-static_assert(sizeof(TileBarriers) <= 512, "fits behind the ring");
+static_assert(sizeof(TileBarriers) <= 640, "fits behind the ring");
 
 // ---- cluster-wide barriers and two-SM tensor-core instructions -----------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -64,27 +67,26 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// arrive at the barrier of the same offset in the pair's first block
+// Arrive at the barrier of the same offset in the pair's first block.  For what lies in tensor memory (ordered by the tcgen05 fences)
+// and for byte counts; a release at cluster scope would wait for all of the thread's memory accesses, some 1300 clocks here, which
+// doubled the time of a tile.
 __device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
+        "mbarrier.arrive.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)) : "memory");
+}
+// The same behind this thread's (or, after __syncwarp, warp's) writes to shared memory, which the products of the pair read.
+__device__ __forceinline__ void arrive_first_release(uint64_t* bar) {
     asm volatile(
         "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
         "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return ok != 0;
-}
 // bounded like mbar_wait, without its back-off: every waiter here has its own barrier and the next step depends on it
-__device__ __forceinline__ void wait_cluster(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    if (try_wait_cluster(bar, parity)) return;
+__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return;
     const long long limit = *abort_flag ? kWaitCyclesAfterAbort : kWaitCycles;
     const long long t0 = clock64();
-    while (!try_wait_cluster(bar, parity)) {
+    while (!mbar_try_wait(bar, parity)) {
         if (clock64() - t0 > limit) {
             *abort_flag = 1;
             return;
@@ -142,6 +144,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
           "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
           "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -175,13 +182,40 @@ __device__ __forceinline__ uint4 codes8_to_half(uint2 c) {
     return r;
 }
 
-// Key of column / value row n of a tile, relative to its first: producer warp w looks up keys 32 w .. 32 w + 31 and puts 16 of
-// them into each block's half of the columns.
-__device__ __forceinline__ constexpr int key_of_column(int n) { return ((n & 63) >> 4) * 32 + (n >> 6) * 16 + (n & 15); }
+// Key of column / value row n of a tile, relative to its first.  Where threads copy the rows, producer warp w looks up keys
+// 32 w .. 32 w + 31 and puts 16 of them into each block's half of the columns.
+template <bool TMA>
+__device__ __forceinline__ constexpr int key_of_column(int n) { return TMA ? n : ((n & 63) >> 4) * 32 + (n >> 6) * 16 + (n & 15); }
 
-// D: dimensions of the tiles, a multiple of 128 not below head_dim (the rest is zero).  T: type of queries and results, TC: of the cache.
-template <int D, typename T, typename TC>
-__global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ AttnParams p) {
+// Copies of a box of [unit rows][64 columns] out of one page into this block's shared memory, announced at the pair's first block's
+// barrier (address in the cluster's window).
+__device__ __forceinline__ void pair_tma_load(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int page, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(row), "r"(head), "r"(page)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t in_first_block(uint64_t* bar) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+    return a;
+}
+__device__ __forceinline__ void arrive_expect(uint32_t cluster_bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes) : "memory");
+}
+
+// Whether the cursor's key tile has keys that no row of the item sees.
+__device__ __forceinline__ bool edge_tile(const AttnParams& p, const ItemCursor<kTileKeys>& c) {
+    const int key0 = c.key0();
+    return !(key0 + kTileKeys <= c.span.end && (p.window == 0 || key0 >= window_start(p, c.pos0) || key0 + kTileKeys <= p.sinks));
+}
+
+// D: dimensions of the tiles, a multiple of 128 not below head_dim (the rest is zero).  T: type of queries and results, TC: of the
+// cache.  TMA: rows come by tensor copies of `unit` rows (a divisor of the page size), else by the producers' threads.
+template <int D, typename T, typename TC, bool TMA>
+__global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap key_map,
+                                                                         const __grid_constant__ CUtensorMap value_map, int unit) {
+    static_assert(!TMA || sizeof(TC) == 2, "codes are converted by threads");
     using S = TileShape<D, TC>;
     constexpr bool kCodes = S::kCodes;
     using OT = typename std::conditional<kCodes, __half, TC>::type;
@@ -192,27 +226,29 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + S::kQuery;
     unsigned char* tail = smem + S::kQuery + kSlots * S::kSlot;
     TileBarriers& bar = *reinterpret_cast<TileBarriers*>(tail);
-    uint32_t* key_mask = reinterpret_cast<uint32_t*>(tail + 512);                       // [kMetaRing][4]
-    float* key_scale = reinterpret_cast<float*>(tail + 512 + kMetaRing * 16);           // codes: [kMetaRing][128], by column
+    uint32_t* key_mask = reinterpret_cast<uint32_t*>(tail + 640);                       // [kMetaRing][4]
+    float* key_scale = reinterpret_cast<float*>(tail + 640 + kMetaRing * 16);           // codes: [kMetaRing][128], by column
     float* value_scale = key_scale + kMetaRing * kTileKeys;                             // codes: [kMetaRing][128], by value row
     float* value_top = value_scale + kMetaRing * kTileKeys;                             // codes: [kMetaRing][4]
-    float* query_scale = value_top + kMetaRing * 4;                                     // codes: [4][128], by row of the block
+    float* exchange = reinterpret_cast<float*>(tail + 640 + S::kMeta);                  // [2][2][128]
+    float* query_scale = exchange + 2 * 2 * 128;                                        // codes: [4][128], by row of the block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kSlots; ++i) { mbar_init(&bar.full[i], 8); mbar_init(&bar.empty[i], 1); }
+        for (int i = 0; i < kSlots; ++i) { mbar_init(&bar.full[i], TMA ? 2 : 8); mbar_init(&bar.empty[i], 1); }
+        for (int i = 0; i < kSlots; ++i) mbar_init(&bar.landed[i], 1);
         mbar_init(&bar.q_full, 8);
         mbar_init(&bar.q_empty, 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 8); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 16); }
         mbar_init(&bar.o_done, 1);
-        mbar_init(&bar.o_empty, 8);
-        for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], 4);
+        mbar_init(&bar.o_empty, 16);
+        for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], TMA ? 1 : 4);
         bar.abort_flag = 0;
         mbar_init_fence();
     }
-    if (warp == 8) pair_tmem_alloc(&bar.tmem);
+    if (warp == kMmaWarp) pair_tmem_alloc(&bar.tmem);
     pdl_trigger();
     tc_fence_before_sync();
     cluster_sync();                                  // barriers are there in both blocks
@@ -233,9 +269,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         ItemCursor<kTileKeys> c;
         locate(p, run0, c);
         const int dim = p.c.head_dim;
-        if (warp >= 4 && warp < 8) {
+        if (warp >= 8 && warp < kMmaWarp) {
             // ------------------------------------------------------------------------------------------------- producers
-            const int w = warp - 4;
+            const int w = warp - 8;
             int page = -1, in_page = 0;              // of key w * 32 + lane of the cursor's tile
             auto look = [&] {
                 page = -1;
@@ -249,47 +285,61 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 fence_async_proxy();
                 __syncwarp();
                 for (; arrived < upto; ++arrived)
-                    if (lane == 0) arrive_first(&bar.full[arrived % kSlots]);
+                    if (lane == 0) arrive_first_release(&bar.full[arrived % kSlots]);
             };
             auto load_query = [&](int segment) {     // 32 of the block's 128 rows per warp
-                if (!kCodes) asm volatile("cp.async.wait_group 0;" ::: "memory");
-                announce(x);                         // the products that read the old rows wait for these loads
-                wait_cluster(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
+                if (!kCodes && !TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
+                if (!TMA) announce(x);               // the products that read the old rows wait for these loads
                 const int cols = c.tokens(p) * p.group, first_row = c.first_row(p);
-                constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks < 1 ? 1 : 32 / kChunks;
-                const bool flip = p.scale_log2 < 0.f;              // the scale's sign goes into the query
-                for (int i = 0; i < 32 / kAtOnce; ++i) {
-                    const int r = w * 32 + i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks < 1 ? 1 : 32 / kChunks, kSteps = 32 / kAtOnce, kBatch = 8;
+                const int chunk = lane % kChunks;
+                const uint32_t to = q_smem + (chunk >> 3) * (128 * 128);
+                auto source = [&](int r) -> const T* {           // null: padding
                     const int n = rank * 128 + r, tok = n / p.group;
-                    float v[8] = {};
-                    if (n < cols && chunk * 8 < dim) {
-                        const T* q = reinterpret_cast<const T*>(p.query) + (int64_t)(first_row + tok) * p.qs[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.qs[1] + chunk * 8;
-                        load8<true>(q, 8, v);
+                    if (n >= cols || chunk * 8 >= dim) return nullptr;
+                    return reinterpret_cast<const T*>(p.query) + (int64_t)(first_row + tok) * p.qs[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.qs[1] + chunk * 8;
+                };
+                if (!kCodes) {
+                    wait_bar(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
+#pragma unroll 4
+                    for (int i = 0; i < kSteps; ++i) {
+                        const int r = w * 32 + i * kAtOnce + lane / kChunks;
+                        const T* q = source(r);
+                        tile_copy16(to + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), q ? q : p.query, q ? 16 : 0);
                     }
-                    if (kCodes) {
-                        float most = 0.f;
+                    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                } else {
+                    for (int i0 = 0; i0 < kSteps; i0 += kBatch) {
+                        uint4 raw[kBatch];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+                        for (int b = 0; b < kBatch; ++b) {
+                            const T* q = source(w * 32 + (i0 + b) * kAtOnce + lane / kChunks);
+                            raw[b] = q ? *reinterpret_cast<const uint4*>(q) : make_uint4(0, 0, 0, 0);
+                        }
+                        if (i0 == 0) wait_bar(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
 #pragma unroll
-                        for (int o = kChunks / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
-                        const int e2 = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
-                        const float down = ldexpf(1.f, -e2);
+                        for (int b = 0; b < kBatch; ++b) {
+                            const int r = w * 32 + (i0 + b) * kAtOnce + lane / kChunks;
+                            float v[8], most = 0.f;
+                            load8<true>(reinterpret_cast<const T*>(&raw[b]), 8, v);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] *= down;
-                        if (chunk == 0) query_scale[(segment & 3) * 128 + r] = fmaxf(ldexpf(fabsf(p.scale_log2), e2), FLT_MIN);
+                            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+#pragma unroll
+                            for (int o = kChunks / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
+                            const int e2 = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
+                            const float down = ldexpf(1.f, -e2);
+                            uint4 out;
+                            uint32_t* o = reinterpret_cast<uint32_t*>(&out);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[e] = tile_pack(v[2 * e] * down, v[2 * e + 1] * down, OT{});
+                            if (chunk == 0) query_scale[(segment & 3) * 128 + r] = fmaxf(ldexpf(fabsf(p.scale_log2), e2), FLT_MIN);
+                            sts16(to + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), out);
+                        }
                     }
-                    uint4 out;
-                    uint32_t* o = reinterpret_cast<uint32_t*>(&out);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        o[e] = tile_pack(v[2 * e], v[2 * e + 1], OT{});
-                        if (flip) o[e] ^= 0x80008000u;
-                    }
-                    sts16(q_smem + (chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4), out);
                 }
                 fence_async_proxy();
                 __syncwarp();
-                if (lane == 0) arrive_first(&bar.q_full);
+                if (lane == 0) arrive_first_release(&bar.q_full);
             };
             // rows of a slot: keys take 16 of this warp's 32 (those of this block's half), values all 32 with half of their columns
             constexpr int kKeyChunks = D / 8, kKeyAtOnce = 32 / kKeyChunks < 1 ? 1 : 32 / kKeyChunks;
@@ -304,7 +354,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             };
             auto load = [&](bool values, int64_t offset) {       // offset: bytes of this lane's row, < 0: no such row
                 const int slot = x % kSlots;
-                wait_cluster(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
+                if (!mbar_try_wait(&bar.empty[slot], ((x / kSlots) & 1) ^ 1)) {
+                    if (!kCodes) {                               // ahead of the products: announce what is on its way first
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        announce(x);
+                    }
+                    wait_bar(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
+                }
                 const uint32_t base = ring + slot * S::kSlot;
                 const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
                 if (!values) {
@@ -345,11 +401,77 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                 }
             };
-            look();
-            int64_t value_offset = -1;
             int segment = 0;
             bool first = true;
-            for (int t = 0; t < tiles; ++t) {
+            if (TMA) {
+                    // A copy takes its warp some 130 clocks to issue, so the four warps take every fourth one each
+                    const int units = kTileKeys / unit, key_units = units / 2;
+                    // lane i < units: unit i of the cursor's tile; its page, -1 where the table holds none, -2 where no row sees the unit.
+                    // Copies of no page are from behind the last one, which reads as zeros
+                    int page = 0, row = 0, page_v = 0, row_v = 0, head_v = 0;
+                    bool edge_v = false;
+                    auto look_unit = [&] {
+                        page = -2;
+                        const int j = c.key0() + lane * unit;
+                        if (lane < units && j < c.span.end && (p.window == 0 || j + unit > window_start(p, c.pos0) || j < p.sinks)) page = page_of(p.c, c.seq, j, row);
+                    };
+                    auto wait_slot = [&] { wait_bar(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag); };
+                    auto tma_values = [&] {
+                        constexpr int groups = D / 128;
+                        const int slot = x % kSlots;
+                        wait_slot();
+                        uint32_t to = in_first_block(&bar.full[slot]);
+                        if (edge_v) to = smem_u32(&bar.landed[slot]);
+                        if (lane == 0 && w == 0) {
+                            if (edge_v) asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(to), "r"((uint32_t)S::kSlot) : "memory");
+                            else arrive_expect(to, S::kSlot);
+                        }
+                        __syncwarp();
+                        const int u = lane / groups, g = lane % groups;
+                        const int pg = __shfl_sync(kFull, page_v, u), rw = __shfl_sync(kFull, row_v, u);
+                        if (u < units && (lane & 3) == w)
+                            pair_tma_load(ring + slot * S::kSlot + g * (128 * 128) + u * unit * 128, &value_map, (rank * groups + g) * 64, rw, head_v, pg < 0 ? p.c.pages : pg, to);
+                        ++x;
+                    };
+                    look_unit();
+                    for (int t = 0; t < tiles; ++t) {
+                        constexpr int groups = D / 64;
+                        if (first) {
+                            if (t > 0) tma_values();
+                            load_query(segment);
+                        }
+                        const int slot = x % kSlots, meta = t % kMetaRing, head = c.head;
+                        const bool edge = edge_tile(p, c), ends = c.k + 1 >= c.span.count, values_now = t > 0 && !first;
+                        wait_slot();                 // and with it for the last reader of this description (static_assert above)
+                        const uint32_t full = in_first_block(&bar.full[slot]);
+                        const unsigned there = __ballot_sync(kFull, page != -1) & (0xffffffffu >> (32 - units));
+                        if (lane == 0 && w == 0) {
+                            key_mask[meta * 4] = there;          // one bit per unit: not missing
+                            mbar_arrive(&bar.keys_full[meta]);
+                            arrive_expect(full, S::kSlot);
+                        }
+                        __syncwarp();
+                        const int u = lane / groups, g = lane % groups;
+                        const int pg = __shfl_sync(kFull, page, (rank * key_units + u) & 31), rw = __shfl_sync(kFull, row, (rank * key_units + u) & 31);
+                        if (u < key_units && (lane & 3) == w)
+                            pair_tma_load(ring + slot * S::kSlot + g * (64 * 128) + u * unit * 128, &key_map, g * 64, rw, head, pg < 0 ? p.c.pages : pg, full);
+                        ++x;
+                        // on to the next tile: its page numbers arrive while the previous tile's values are issued
+                        const int page_now = page, row_now = row;
+                        if (t + 1 < tiles) {
+                            if (ends) c.next_item(p); else ++c.k;
+                            look_unit();
+                        }
+                        if (values_now) tma_values();
+                        page_v = page_now; row_v = row_now; head_v = head; edge_v = edge;
+                        first = ends;
+                        if (ends) ++segment;
+                    }
+                    tma_values();
+            }
+            int64_t value_offset = -1;
+            if (!TMA) look();
+            for (int t = TMA ? tiles : 0; t < tiles; ++t) {
                 if (first) {
                     if (t > 0) load(true, value_offset);
                     load_query(segment);
@@ -361,7 +483,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const int meta = t % kMetaRing;
                 // a description is written anew only when its last reader has passed: the key slot of this tile, waited for below,
                 // was freed later than that (static_assert above); so wait for the slot first
-                wait_cluster(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
+                if (!mbar_try_wait(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1)) {
+                    if (!kCodes) {
+                        asm volatile("cp.async.wait_group 0;" ::: "memory");
+                        announce(x);
+                    }
+                    wait_bar(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
+                }
                 if (lane == 0) key_mask[meta * 4 + w] = rows;
                 if (kCodes) {
                     const float ks = page < 0 ? 0.f : p.c.key_scale[row_offset(p.c.key_scale_stride, page, c.head, in_page)];
@@ -388,10 +516,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 first = ends;
                 if (ends) ++segment;
             }
-            load(true, value_offset);
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            announce(x);
-        } else if (warp == 8) {
+            if (!TMA) {
+                load(true, value_offset);
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                announce(x);
+            }
+        } else if (warp == kEdgeWarp) {
+            // ------------------------------------------------------------------------------------------------- edges
+            // A tile of values with rows that nobody may see (behind the sequence's end, outside of the window) is copied to a barrier of
+            // its own: here those rows are zeroed, which can hold anything (0 * infinity is no zero), and the slot is announced.
+            if (TMA) {
+                uint32_t landed = 0;                     // per slot: parity of its next such copy
+                for (int t = 0; t < tiles; ++t) {
+                    const bool ends = c.k + 1 >= c.span.count;
+                    if (edge_tile(p, c)) {
+                        // order of the loads: K(0), then [K(t + 1), V(t)] inside an item and [V(t), K(t + 1)] where t ends one
+                        const int slot = (ends || t + 1 == tiles ? 2 * t + 1 : 2 * t + 2) % kSlots, key0 = c.key0(), lo = window_start(p, c.pos0);
+                        const uint32_t base = ring + slot * S::kSlot;
+                        wait_bar(&bar.landed[slot], (landed >> slot) & 1, abort_flag);
+                        landed ^= 1u << slot;
+                        for (int r = lane; r < kTileKeys; r += 32) {
+                            const int j = key0 + r;
+                            if (j < c.span.end && (p.window == 0 || j >= lo || j < p.sinks)) continue;
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i) sts16(base + (i >> 3) * (128 * 128) + r * 128 + ((i & 7) << 4), make_uint4(0, 0, 0, 0));
+                        }
+                        fence_async_proxy();
+                        __syncwarp();
+                        if (lane == 0) arrive_first_release(&bar.full[slot]);
+                    }
+                    if (t + 1 < tiles) {
+                        if (ends) c.next_item(p); else ++c.k;
+                    }
+                }
+            }
+        } else if (warp == kMmaWarp) {
             // ------------------------------------------------------------------------------------------------- products
             if (rank == 0 && lane == 0) {
                 constexpr uint32_t s_idesc = pair_idesc<OT>(kTileKeys, false), o_idesc = pair_idesc<OT>(D, true);
@@ -399,7 +558,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 int x = 0, segment = 0, o_segment = 0;
                 auto scores = [&](int t, bool ends) {
                     const int slot = x % kSlots;
-                    wait_cluster(&bar.full[slot], (x / kSlots) & 1, abort_flag);
+                    wait_bar(&bar.full[slot], (x / kSlots) & 1, abort_flag);
                     tc_fence_after_sync();
                     const uint32_t k = ring + slot * S::kSlot;
                     for (int i = 0; i < key_steps; ++i)
@@ -411,13 +570,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     ++x;
                 };
                 auto values = [&](int t, bool begins) {
-                    wait_cluster(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
+                    wait_bar(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
                     if (begins) {
-                        if (o_segment > 0) wait_cluster(&bar.o_empty, (o_segment - 1) & 1, abort_flag);
+                        if (o_segment > 0) wait_bar(&bar.o_empty, (o_segment - 1) & 1, abort_flag);
                         ++o_segment;
                     }
                     const int slot = x % kSlots;
-                    wait_cluster(&bar.full[slot], (x / kSlots) & 1, abort_flag);
+                    wait_bar(&bar.full[slot], (x / kSlots) & 1, abort_flag);
                     tc_fence_after_sync();
                     const uint32_t v = ring + slot * S::kSlot;
 #pragma unroll
@@ -432,7 +591,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     const bool ends = c.k + 1 >= c.span.count;
                     if (first) {
                         if (t > 0) values(t - 1, last_began);
-                        wait_cluster(&bar.q_full, segment & 1, abort_flag);
+                        wait_bar(&bar.q_full, segment & 1, abort_flag);
                         ++segment;
                     }
                     scores(t, ends || t + 1 == tiles);
@@ -447,25 +606,45 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
         } else {
             // ------------------------------------------------------------------------------------------------- softmax
-            const int r = warp * 32 + lane, n = rank * 128 + r;          // row of the block, of the pair
-            const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+            // two threads per row, 64 columns each: warps w and w + 4
+            const int quarter = warp & 3, half = warp >> 2;
+            const int r = quarter * 32 + lane, n = rank * 128 + r;       // row of the block, of the pair
+            const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
             const uint32_t o_addr = tmem + lanes;
             float m = -INFINITY, l = 0.f, top = 0.f, qscale = fabsf(p.scale_log2);
             bool begins = true;                                          // of this run's part of the item
             int segment = 0;
-            int64_t at = run0;                                           // first tile of the segment
+            int64_t at = run0;                                           // tile of the order
             int began_k = c.k;
+            const int tok = n / p.group;
+            const bool negative = p.scale_log2 < 0.f;
+            auto meet = [&] { named_bar_sync(1 + quarter, 64); };
             for (int t = 0; t < tiles; ++t, ++at) {
-                const int tok = n / p.group;
                 const int pos = c.pos0 + tok, meta = t % kMetaRing;
                 const int key0 = c.key0();
-                wait_cluster(&bar.keys_full[meta], (t / kMetaRing) & 1, abort_flag);
-                wait_cluster(&bar.s_full[t & 1], (t >> 1) & 1, abort_flag);
+                const bool inside = key0 + kTileKeys - 1 <= c.pos0 && (p.window == 0 || key0 >= window_start(p, c.pos1) || key0 + kTileKeys <= p.sinks);
+                wait_bar(&bar.keys_full[meta], (t / kMetaRing) & 1, abort_flag);
+                uint32_t there[2] = {0xffffffffu, 0xffffffffu};          // one bit per key: its page is not missing
+                bool complete;
+                if (TMA) {
+                    const uint32_t bits = key_mask[meta * 4];
+                    complete = bits == 0xffffffffu >> (32 - kTileKeys / unit);
+                    if (!complete)
+                        for (int k = 0; k < 64; ++k)
+                            if (!((bits >> ((half * 64 + k) / unit)) & 1u)) there[k >> 5] &= ~(1u << (k & 31));
+                } else {
+                    const uint4 v = *reinterpret_cast<const uint4*>(key_mask + meta * 4);
+                    complete = (v.x & v.y & v.z & v.w) == 0xffffffffu;
+                    // columns 16 i .. 16 i + 15 of this half are the half's 16 keys of producer warp i
+                    there[0] = ((v.x >> (16 * half)) & 0xffffu) | ((v.y >> (16 * half)) << 16);
+                    there[1] = ((v.z >> (16 * half)) & 0xffffu) | ((v.w >> (16 * half)) << 16);
+                }
+                wait_bar(&bar.s_full[t & 1], (t >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
                 const uint32_t s_addr = tmem_s + lanes + (t & 1) * kTileKeys;
-                float s[kTileKeys];
-#pragma unroll
-                for (int i = 0; i < kTileKeys; i += 32) tmem_ld32(s_addr + i, s + i);
+                float s[64];
+                tmem_ld32(s_addr + half * 64, s);
+                tmem_ld32(s_addr + half * 64 + 32, s + 32);
                 tmem_wait_ld();
                 if (begins) {
                     m = -INFINITY;
@@ -475,56 +654,64 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     began_k = c.k;
                 }
                 if (kCodes) {
-                    const float4* ks = reinterpret_cast<const float4*>(key_scale + meta * kTileKeys);
+                    const float4* ks = reinterpret_cast<const float4*>(key_scale + meta * kTileKeys + half * 64);
 #pragma unroll
-                    for (int i = 0; i < kTileKeys / 4; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         const float4 f = ks[i];
                         s[4 * i] *= f.x; s[4 * i + 1] *= f.y; s[4 * i + 2] *= f.z; s[4 * i + 3] *= f.w;
                     }
                 }
-                // ---- masks
-                const uint4 there = *reinterpret_cast<const uint4*>(key_mask + meta * 4);
-                const bool complete = (there.x & there.y & there.z & there.w) == 0xffffffffu;
-                if (!complete || !(key0 + kTileKeys - 1 <= c.pos0 && (p.window == 0 || key0 >= window_start(p, c.pos1) || key0 + kTileKeys <= p.sinks))) {
-                    const int hi = pos - key0, lo = p.window > 0 ? pos - p.window - key0 : -1, sink = p.window > 0 ? p.sinks - key0 : 0;
-                    const uint32_t bits[4] = {there.x, there.y, there.z, there.w};
+                if (negative)
 #pragma unroll
-                    for (int i = 0; i < kTileKeys; ++i) {
-                        const int k = key_of_column(i);
-                        if (!((bits[k >> 5] >> (k & 31)) & 1u) || k > hi || (k <= lo && k >= sink)) s[i] = -INFINITY;
+                    for (int i = 0; i < 64; ++i) s[i] = -s[i];
+                if (!complete || !inside) {
+                    // keys relative to this half's first: column i is key i (tensor copies), or 32 (i / 16) + i % 16
+                    const int first = key0 + (TMA ? 64 : 16) * half;
+                    const int hi = pos - first, lo = p.window > 0 ? pos - p.window - first : -1000, sink = p.window > 0 ? p.sinks - first : 0;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        const int k = TMA ? i : (i >> 4) * 32 + (i & 15);
+                        if (!((there[i >> 5] >> (i & 31)) & 1u) || k > hi || (k <= lo && k >= sink)) s[i] = -INFINITY;
                     }
                 }
-                // ---- maximum; the base of the powers only moves when it has to
-                float most = s[0];
+                // ---- the row's maximum; the base of the powers only moves when it has to
+                float tops[8];
 #pragma unroll
-                for (int i = 1; i < kTileKeys; ++i) most = fmaxf(most, s[i]);
-                most *= qscale;
+                for (int e = 0; e < 8; ++e) tops[e] = fmaxf(s[e], s[e + 8]);
+#pragma unroll
+                for (int i = 16; i < 64; i += 16)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) tops[e] = fmaxf(tops[e], fmaxf(s[i + e], s[i + 8 + e]));
+                float most = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+                float* ex = exchange + (t & 1) * 256;
+                ex[half * 128 + r] = most;
+                meet();                                                  // also: both have read their scores
+                most = qscale * fmaxf(most, ex[(half ^ 1) * 128 + r]);
                 float alpha = 1.f;
                 const float m_new = most > m + kLazy ? most : m;
                 if (m_new > m) alpha = m == -INFINITY ? 0.f : tile_exp2(m - m_new);
                 m = m_new;
-                float unit = 1.f;
+                float unit_scale = 1.f;
                 if (kCodes) {
                     const float4 vt = *reinterpret_cast<const float4*>(value_top + meta * 4);
                     const float tile_top = fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w));
                     if (tile_top > 2.f * top) {                          // the same in all rows
-                        unit = top > 0.f ? top / tile_top : 0.f;
+                        unit_scale = top > 0.f ? top / tile_top : 0.f;
                         top = tile_top;
                     }
                 }
                 if (!begins) {
-                    const float factor = alpha * unit;
-                    if (__any_sync(kFull, factor != 1.f)) {
-                        wait_cluster(&bar.o_done, (t - 1) & 1, abort_flag);
+                    const float factor = alpha * unit_scale;
+                    if (__any_sync(kFull, factor != 1.f)) {              // the same in both warps of a row
+                        wait_bar(&bar.o_done, (t - 1) & 1, abort_flag);
                         tc_fence_after_sync();
 #pragma unroll 1
-                        for (int i = 0; i < D; i += 32) {
-                            float o[32];
-                            tmem_ld32(o_addr + i, o);
-                            tmem_wait_ld();
+                        for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 16) {
+                            float o[16];
+                            tmem_ld16(o_addr + i, o);
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] *= factor;
-                            tmem_st32(o_addr + i, reinterpret_cast<const uint32_t*>(o));
+                            for (int e = 0; e < 16; ++e) o[e] *= factor;
+                            tmem_st16(o_addr + i, reinterpret_cast<const uint32_t*>(o));
                         }
                     }
                     l *= alpha;
@@ -532,23 +719,23 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 // ---- weights
                 const float base = m == -INFINITY ? 0.f : m - kShift;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                uint32_t w[32];
                 const float inv_top = kCodes ? (top > 0.f ? 1.f / top : 1.f) : 1.f;
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int part = 0; part < 2; ++part) {
+                    uint32_t w[16];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int e = half * 64 + 2 * i;
+                    for (int i = 0; i < 16; ++i) {
+                        const int e = part * 32 + 2 * i;
                         float a = tile_exp2(fmaf(s[e], qscale, -base)), b = tile_exp2(fmaf(s[e + 1], qscale, -base));
                         sum[i & 3] += a + b;
                         if (kCodes) {
-                            const float2 vs = *reinterpret_cast<const float2*>(value_scale + meta * kTileKeys + e);
+                            const float2 vs = *reinterpret_cast<const float2*>(value_scale + meta * kTileKeys + half * 64 + e);
                             a *= vs.x * inv_top;
                             b *= vs.y * inv_top;
                         }
                         w[i] = tile_pack(a, b, OT{});
                     }
-                    tmem_st32(s_addr + half * 32, w);
+                    tmem_st16(s_addr + half * 32 + part * 16, w);        // over scores that both threads have read
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 tmem_wait_st();
@@ -558,9 +745,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 // ---- the end of the item, or of the run
                 const bool ends = c.k + 1 >= c.span.count;
                 if (ends || t + 1 == tiles) {
-                    wait_cluster(&bar.o_done, t & 1, abort_flag);
+                    // the row's sum; the buffer is the one that the next tile's maxima do not use
+                    float* sums = exchange + ((t + 1) & 1) * 256;
+                    sums[half * 128 + r] = l;
+                    meet();
+                    l = sums[r] + sums[128 + r];                         // in this order in both threads
+                    wait_bar(&bar.o_done, t & 1, abort_flag);
                     tc_fence_after_sync();
-                    const int cols = c.tokens(p) * p.group, first_row = c.first_row(p);
+                    const int tokens = c.tokens(p), cols = tokens * p.group, first_row = c.first_row(p);
                     const bool whole = ends && began_k == 0;
                     const float scale_out = kCodes ? (top > 0.f ? top : 1.f) : 1.f;
                     const int which = at - (c.k - began_k) == run0 ? 0 : 1;
@@ -571,27 +763,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     bool odd = false;
                     const bool wide = (dim & 7) == 0 && ((p.os[0] | p.os[1]) & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll 1
-                    for (int i = 0; i < D; i += 32) {
-                        float o[32];
-                        tmem_ld32(o_addr + i, o);
-                        tmem_wait_ld();
+                    for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 16) {
+                        float o[16];
+                        tmem_ld16(o_addr + i, o);
                         if (n < cols && i < dim) {
                             if (whole) {
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) {
+                                for (int e = 0; e < 16; ++e) {
                                     o[e] = l == 0.f ? 0.f : o[e] * inv;
                                     if (i + e < dim) odd |= !(fabsf(o[e]) < INFINITY);
                                     if (failed) o[e] = NAN;
                                 }
 #pragma unroll
-                                for (int e = 0; e < 32; e += 8)
+                                for (int e = 0; e < 16; e += 8)
                                     if (i + e < dim) {
-                                        const float (&v)[8] = *reinterpret_cast<const float (*)[8]>(o + e);
+                                        const float v[8] = {o[e], o[e + 1], o[e + 2], o[e + 3], o[e + 4], o[e + 5], o[e + 6], o[e + 7]};
                                         if (wide) store8<true>(out + i + e, 8, v); else store8<false>(out + i + e, dim - i - e, v);
                                     }
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 32; e += 4)
+                                for (int e = 0; e < 16; e += 4)
                                     *reinterpret_cast<float4*>(part + 2 * kTileRows + (int64_t)n * D + i + e) =
                                         failed ? make_float4(NAN, NAN, NAN, NAN) : make_float4(o[e] * scale_out, o[e + 1] * scale_out, o[e + 2] * scale_out, o[e + 3] * scale_out);
                             }
@@ -601,20 +792,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     __syncwarp();
                     if (lane == 0) arrive_first(&bar.o_empty);
                     if (whole) {
-                        // `odd` rows of a tile with several tokens once more
-                        unsigned again = c.tokens(p) > 1 && !failed ? __ballot_sync(kFull, odd) : 0u;
+                        // rows of a tile with several tokens whose result is not finite: once more, when both halves are written
+                        float* flags = exchange + (t & 1) * 256;
+                        flags[half * 128 + r] = odd ? 1.f : 0.f;
+                        meet();
+                        unsigned again = half == 0 && tokens > 1 && !failed ? __ballot_sync(kFull, flags[r] + flags[128 + r] != 0.f) : 0u;
                         while (again) {
                             const int i = __ffs(again) - 1;
                             again &= again - 1;
-                            const int row = rank * 128 + warp * 32 + i, rt = row / p.group;
+                            const int row = rank * 128 + quarter * 32 + i, rt = row / p.group;
                             row_again<T, TC>(p, c.seq, first_row + rt, c.pos0 + rt, c.head * p.group + row - rt * p.group);
                         }
                     } else {
-                        if (n < cols) { part[n] = m; part[kTileRows + n] = l; }
+                        if (n < cols && half == 0) { part[n] = m; part[kTileRows + n] = l; }
                         if (rank == 0 && threadIdx.x == 0)
-                            heads[which] = PartHead{first_row, c.tokens(p), c.head, c.seq, c.pos0, began_k == 0, ends, runs.worker_of(at - c.k + c.span.count - 1)};
+                            heads[which] = PartHead{first_row, tokens, c.head, c.seq, c.pos0, began_k == 0, ends, runs.worker_of(at - c.k + c.span.count - 1)};
                     }
                     ++segment;
+                    meet();                                              // the exchange is free again
                 }
                 begins = ends;
                 if (t + 1 < tiles) {
@@ -626,7 +821,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     __syncwarp();
     tc_fence_before_sync();
     cluster_sync();                                  // nothing more arrives at either block's barriers
-    if (warp == 8) {
+    if (warp == kMmaWarp) {
         tc_fence_after_sync();
         pair_tmem_dealloc(tmem);
     }
@@ -680,18 +875,29 @@ __global__ void __launch_bounds__(256) attention_tile_join_kernel(const __grid_c
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
-template <int D, typename T, typename TC>
-static int tile(AttnParams p, size_t* need, cudaStream_t stream) {
+// Rows per tensor copy: the largest power of two up to 64 that divides the page size (a copy stays within a page, and copies start
+// at its multiples); 0 below 8, the height of the swizzle's pattern.
+static int unit_rows(int page_size) {
+    int unit = 64;
+    while (unit >= 8 && page_size % unit) unit >>= 1;
+    return unit >= 8 ? unit : 0;
+}
+
+// Box of [unit rows][64 columns] of one head of one page; columns beyond head_dim and pages beyond the last read as zeros.
+static bool page_map(const void* base, const fk_kv_cache& c, const int64_t* stride, int unit, CUtensorMap* out) {
+    const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_size, (uint64_t)c.kv_heads, (uint64_t)c.pages};
+    const uint64_t strides[3] = {(uint64_t)stride[2] * 2, (uint64_t)stride[1] * 2, (uint64_t)stride[0] * 2};
+    const uint32_t box[4] = {64, (uint32_t)unit, 1, 1};
+    return paged_tensor_map(base, c.dtype == FK_BF16, dims, strides, box, out);
+}
+
+template <int D, typename T, typename TC, bool TMA>
+static int launch_tile(const AttnParams& p, const CUtensorMap& key_map, const CUtensorMap& value_map, int unit, cudaStream_t stream) {
     using S = TileShape<D, TC>;
-    p.tile_tokens = kTileRows / p.group;
-    const int pairs = sm_count() / 2;
-    if (need) {
-        *need = (size_t)pairs * 2 * (sizeof(PartHead) + S::kPart * sizeof(float));
-        return FK_OK;
-    }
-    auto kern = attention_tile_kernel<D, T, TC>;
+    auto kern = attention_tile_kernel<D, T, TC, TMA>;
     FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), "attention (tile) attr");
     cudaLaunchConfig_t cfg{};
+    const int pairs = sm_count() / 2;
     cfg.gridDim = dim3(2 * pairs);
     cfg.blockDim = dim3(kTileThreads);
     cfg.dynamicSmemBytes = S::kSmem;
@@ -704,11 +910,28 @@ static int tile(AttnParams p, size_t* need, cudaStream_t stream) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    FK_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p), "attention (tile) launch");
+    FK_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, key_map, value_map, unit), "attention (tile) launch");
     FK_LAUNCH_OK("attention (tile) launch");
     FK_CUDA_OK(launch_pdl(attention_tile_join_kernel<D, T, TC>, dim3((unsigned)pairs, kTileRows / 8), dim3(256), 0, stream, p), "attention (tile) join launch");
     FK_LAUNCH_OK("attention (tile) join launch");
     return FK_OK;
+}
+
+template <int D, typename T, typename TC>
+static int tile(AttnParams p, size_t* need, cudaStream_t stream) {
+    p.tile_tokens = kTileRows / p.group;
+    if (need) {
+        *need = (size_t)(sm_count() / 2) * 2 * (sizeof(PartHead) + TileShape<D, TC>::kPart * sizeof(float));
+        return FK_OK;
+    }
+    CUtensorMap key_map{}, value_map{};
+    if constexpr (sizeof(TC) == 2) {
+        // Tensor copies wherever pages and strides allow them (2048 tokens at 16384: with rows copied by threads 785 us)
+        const int unit = unit_rows(p.c.page_size);
+        if (unit > 0 && page_map(p.c.key, p.c, p.c.key_stride, unit, &key_map) && page_map(p.c.value, p.c, p.c.value_stride, unit, &value_map))
+            return launch_tile<D, T, TC, true>(p, key_map, value_map, unit, stream);
+    }
+    return launch_tile<D, T, TC, false>(p, key_map, value_map, 0, stream);
 }
 
 template <typename T, typename TC>

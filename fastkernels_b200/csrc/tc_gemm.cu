@@ -373,6 +373,16 @@ bool column_pair_map(const void* base, uint64_t rows, uint64_t cols, uint32_t bo
     return true;
 }
 
+bool paged_tensor_map(const void* base, bool bf16, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMap* out) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t d[4], s[3];
+    cuuint32_t b[4], elem[4] = {1, 1, 1, 1};
+    for (int i = 0; i < 4; ++i) { d[i] = dims[i]; b[i] = box[i]; if (i < 3) s[i] = strides[i]; }
+    return fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), d, s, b, elem,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool tc_path_supported(const ExpertParams& p, int weight_dtype) {
     if (weight_dtype != FK_BF16) return false;
     if (p.H % 128 != 0 || p.I % 64 != 0 || p.H < 128 || p.I < 64) return false;
