@@ -100,27 +100,30 @@ __device__ __forceinline__ void pair_tmem_alloc(uint32_t* dst) {
 __device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr) {
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
 }
-__device__ __forceinline__ void pair_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Descriptors of operands in shared memory, 128-byte swizzle, 8-row (8-k) groups 1024 bytes apart: the low word (address, distance of
+// 64-column groups for MN-major operands) moves, the high one is the same for all.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t group) { return (addr >> 4) | ((group >> 4) << 16); }
+// K-major a and b: rows of 64 elements (128 bytes)
+__device__ __forceinline__ void pair_mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d), "r"(a_low), "r"(b_low), "r"(idesc), "r"((uint32_t)accumulate), "n"(kDescHigh) : "memory");
 }
-__device__ __forceinline__ void pair_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// a in tensor memory; b MN-major: 64 columns (128 bytes) per k
+__device__ __forceinline__ void pair_mma_ts(uint32_t d, uint32_t a, uint32_t b_low, uint32_t idesc, bool accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b_low), "r"(idesc), "r"((uint32_t)accumulate), "n"(kDescHigh) : "memory");
+}
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 // arrive at the barrier of this offset in both blocks when all products issued so far are done
 __device__ __forceinline__ void pair_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_u32(bar)), "h"((uint16_t)3) : "memory");
-}
-// K-major operand with rows of 64 elements (128 bytes, swizzled), 8-row groups 1024 bytes apart
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t addr) {
-    return ((uint64_t)(addr >> 4) & 0x3fffull) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// MN-major operand: rows of 64 columns (128 bytes, swizzled) per k, 8-k groups 1024 bytes apart, 64-column groups `group` bytes apart
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t addr, uint32_t group) {
-    return ((uint64_t)(addr >> 4) & 0x3fffull) | ((uint64_t)(group >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 template <typename OT>
 __device__ __forceinline__ constexpr uint32_t pair_idesc(uint32_t n, bool b_mn_major) {
@@ -552,39 +555,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
         } else if (warp == kMmaWarp) {
             // ------------------------------------------------------------------------------------------------- products
-            if (rank == 0 && lane == 0) {
+            // The whole warp walks and waits, one lane issues: what the instructions need is then the same for all lanes and lies in uniform
+            // registers, and the issuing thread's own instructions are not what bounds a tile (with all of it in one lane's branch, a tile
+            // took 4000 clocks for 2050 of products)
+            if (rank == 0) {
                 constexpr uint32_t s_idesc = pair_idesc<OT>(kTileKeys, false), o_idesc = pair_idesc<OT>(D, true);
-                const int key_steps = (dim + 15) / 16;
-                int x = 0, segment = 0, o_segment = 0;
+                const uint32_t q_low = desc_low(q_smem, 16), k_low = desc_low(ring, 16), v_low = desc_low(ring, 128 * 128);
+                const bool leader = elect_lane();
+                int slot = 0, segment = 0, o_segment = 0;
+                uint32_t phase = 0;                  // of the ring
+                auto next = [&] {
+                    if (++slot == kSlots) { slot = 0; phase ^= 1; }
+                };
                 auto scores = [&](int t, bool ends) {
-                    const int slot = x % kSlots;
-                    wait_bar(&bar.full[slot], (x / kSlots) & 1, abort_flag);
+                    wait_bar(&bar.full[slot], phase, abort_flag);
                     tc_fence_after_sync();
-                    const uint32_t k = ring + slot * S::kSlot;
-                    for (int i = 0; i < key_steps; ++i)
-                        pair_mma_ss(tmem_s + (t & 1) * kTileKeys, desc_k_major(q_smem + (i >> 2) * (128 * 128) + (i & 3) * 32),
-                                    desc_k_major(k + (i >> 2) * (64 * 128) + (i & 3) * 32), s_idesc, i > 0);
-                    pair_commit(&bar.empty[slot]);
-                    pair_commit(&bar.s_full[t & 1]);
-                    if (ends) pair_commit(&bar.q_empty);
-                    ++x;
+                    if (leader) {
+                        const uint32_t d = tmem_s + (t & 1) * kTileKeys, k = k_low + slot * (S::kSlot >> 4);
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i)
+                            if (i * 16 < dim) pair_mma_ss(d, q_low + (((i >> 2) * (128 * 128) + (i & 3) * 32) >> 4), k + (((i >> 2) * (64 * 128) + (i & 3) * 32) >> 4), s_idesc, i > 0);
+                        pair_commit(&bar.s_full[t & 1]);
+                        pair_commit(&bar.empty[slot]);
+                        if (ends) pair_commit(&bar.q_empty);
+                    }
+                    __syncwarp();
+                    next();
                 };
                 auto values = [&](int t, bool begins) {
-                    wait_bar(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
+                    wait_bar(&bar.full[slot], phase, abort_flag);
                     if (begins) {
                         if (o_segment > 0) wait_bar(&bar.o_empty, (o_segment - 1) & 1, abort_flag);
                         ++o_segment;
                     }
-                    const int slot = x % kSlots;
-                    wait_bar(&bar.full[slot], (x / kSlots) & 1, abort_flag);
+                    wait_bar(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
                     tc_fence_after_sync();
-                    const uint32_t v = ring + slot * S::kSlot;
+                    if (leader) {
+                        const uint32_t a = tmem_s + (t & 1) * kTileKeys, v = v_low + slot * (S::kSlot >> 4);
 #pragma unroll
-                    for (int i = 0; i < kTileKeys / 16; ++i)
-                        pair_mma_ts(tmem, tmem_s + (t & 1) * kTileKeys + i * 8, desc_mn_major(v + i * 2048, 128 * 128), o_idesc, !begins || i > 0);
-                    pair_commit(&bar.empty[slot]);
-                    pair_commit(&bar.o_done);
-                    ++x;
+                        for (int i = 0; i < kTileKeys / 16; ++i) pair_mma_ts(tmem, a + i * 8, v + i * (2048 >> 4), o_idesc, !begins || i > 0);
+                        pair_commit(&bar.o_done);
+                        pair_commit(&bar.empty[slot]);
+                    }
+                    __syncwarp();
+                    next();
                 };
                 bool first = true, last_began = false;
                 for (int t = 0; t < tiles; ++t) {
