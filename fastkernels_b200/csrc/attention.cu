@@ -98,12 +98,12 @@ static int check_attention(const fk_attention_call* a) {
     return FK_OK;
 }
 
-// Pieces of the key axis: enough warps for the whole chip (16 per SM) where there are few rows, none shorter than 128 keys.
+// Pieces of the key axis: enough warps for the whole chip (16 per SM) where there are few rows, none shorter than 64 keys.
 static int any_splits(const fk_attention_call& a) {
     const int64_t rows = (int64_t)a.rows * a.q_heads;
     const int64_t longest = (int64_t)a.cache.max_pages * a.cache.page_size;
     int64_t want = (148 * 16 + rows - 1) / rows;
-    if (want > (longest + 127) / 128) want = (longest + 127) / 128;
+    if (want > (longest + 63) / 64) want = (longest + 63) / 64;
     if (want > 64) want = 64;
     return want < 1 ? 1 : (int)want;
 }
@@ -138,7 +138,7 @@ static AttnParams attn_params(const fk_attention_call& a) {
 
 enum class Path { any, few, tile };
 
-// Few rows per key/value head (up to 16: decode and short continuations) are a stream of the cache; more, and head sizes that
+// Few rows per key/value head (up to 16, 8 at 256 dimensions: decode and short continuations) are a stream of the cache; more, and head sizes that
 // the stream has no form for, go to the tensor cores; fp32, head sizes off a multiple of 8 and rows off 16-byte boundaries take
 // the shape-agnostic kernel.
 static Path path_of(const fk_attention_call& a, const AttnParams& p) {

@@ -51,16 +51,24 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const Q& q, int se
     for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] = 0.f;
     const TC* keys = reinterpret_cast<const TC*>(p.c.key) + head * p.c.key_stride[1];
     const TC* values = reinterpret_cast<const TC*>(p.c.value) + head * p.c.value_stride[1];
+    // where the key of this lane in the group at k0 is; looked up one group ahead of its use
+    int next_page = -1, next_row = 0;
+    auto look = [&](int64_t k0) {
+        next_page = -1;
+        const int64_t k = k0 + lane;
+        if (k < count) next_page = page_of(p.c, seq, (int)(k < n_sinks ? k : lo + k - n_sinks), next_row);
+    };
+    look((int64_t)first * 32);
     for (int64_t k0 = (int64_t)first * 32; k0 < count; k0 += (int64_t)step * 32) {
-        const int k = (int)k0 + lane;
-        int in_page = 0, page = -1;
-        if (k < count) page = page_of(p.c, seq, k < n_sinks ? k : lo + k - n_sinks, in_page);
+        const int page = next_page, in_page = next_row;
+        look(k0 + (int64_t)step * 32);
         float s = -INFINITY, vscale = 1.f;
         int64_t voff = 0;
         if (page >= 0) {
             const TC* row = keys + page * p.c.key_stride[0] + in_page * p.c.key_stride[2];
             voff = page * p.c.value_stride[0] + in_page * p.c.value_stride[2];
             float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
             for (int d = 0; d < D; d += 8) {
                 float v[8];
                 load8<WIDE>(row + d, D - d, v);
@@ -83,13 +91,25 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const Q& q, int se
         r.l = r.l * alpha + warp_sum(w);
 #pragma unroll
         for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] *= alpha;
-        for (int i = 0; i < 32; ++i) {
-            const int64_t off = __shfl_sync(kFull, voff, i);
-            const float wi = __shfl_sync(kFull, w * vscale, i);
-            if (!((seen >> i) & 1u) || wi == 0.f) continue;
+        const float weight = page >= 0 && w != 0.f ? w * vscale : 0.f;
+        const unsigned adds = __ballot_sync(kFull, page >= 0 && w != 0.f);
+        constexpr int kRows = 4;                            // value rows in flight
+#pragma unroll 2
+        for (int i0 = 0; i0 < 32; i0 += kRows) {
+            float v[kRows][FK_MAX_HEAD_DIM / 32];
 #pragma unroll
-            for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
-                if (c * 32 + lane < D) r.acc[c] = fmaf(wi, load_elem(values + off + c * 32 + lane), r.acc[c]);
+            for (int i = 0; i < kRows; ++i) {
+                const int64_t off = __shfl_sync(kFull, voff, i0 + i);
+#pragma unroll
+                for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
+                    v[i][c] = ((adds >> (i0 + i)) & 1u) && c * 32 + lane < D ? load_elem(values + off + c * 32 + lane) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const float wi = __shfl_sync(kFull, weight, i0 + i);
+#pragma unroll
+                for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] = fmaf(wi, v[i][c], r.acc[c]);
+            }
         }
     }
 }

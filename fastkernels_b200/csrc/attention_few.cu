@@ -9,8 +9,8 @@
 // Every warp works alone: it takes 16 keys at a time through its own ring of shared-memory slots (cp.async, a slot of keys, then
 // one of values), keeps its own running maximum and sum, and never waits for another warp.  The groups of 16 keys of all
 // (sequence, head) items, in order, are dealt to the warps of the grid in equal contiguous runs, so uneven sequences need no
-// schedule.  A run covers some items whole (written out at once) and at most two in part; those are joined by
-// attention_few_join_kernel in key order, so the result does not depend on timing.
+// schedule.  A run covers some items whole (written out at once) and at most two in part; the parts of a block's warps are joined at
+// the block's end, what crosses blocks by attention_few_join_kernel, in key order, so the result does not depend on timing.
 //
 // 8-bit caches: the codes go to fp16 exactly; a query row is scaled by a power of two into fp16's range (exact for what is
 // within 2^-14 of its largest element, to 2^-25 of it below), scores are multiplied by their key's scale, and the weights by
@@ -106,7 +106,8 @@ struct FewShape {
     static constexpr int kSlots = kFit > 8 ? 8 : kFit;
     static constexpr int kCols = 8 * NT;
     static constexpr int kPart = (D + 2) * kCols;                      // floats of a partial result: m, l per column, [column][D]
-    static constexpr int kSmem = kWarps * kSlots * (kSlot + 16) + 256;
+    static constexpr int kHeads = kWarps * 2 * (int)sizeof(PartHead);
+    static constexpr int kSmem = kWarps * kSlots * (kSlot + 16) + 256 + kHeads;
     static_assert(kSlots >= 3, "a slot being read and two on their way");
 };
 
@@ -119,6 +120,64 @@ __device__ __forceinline__ int slot_chunk(int row, int chunk) {
     if (!VALUES) return D >= 128 ? chunk ^ ((row & 1) << 2) : chunk;
     return D >= 128 ? chunk ^ (((row >> 2) & 3) << 1) : chunk ^ ((row >> 2) & 3);
 }
+
+// Column n of an item joined from `count` parts, by one warp: lane l has dimensions 4 l .. 4 l + 3 (and 128 more each), or 2 l, 2 l + 1
+// at 64.  part(i) is the address of the i-th part.
+template <int D>
+struct Joined {
+    static constexpr int kVec = D >= 128 ? 4 : 2, kParts = D / (32 * kVec);
+    float m, l, acc[kParts][kVec];
+    __device__ __forceinline__ static int dim(int lane, int c, int e) { return c * 32 * kVec + lane * kVec + e; }
+    template <int COLS, typename Part>
+    __device__ __forceinline__ void join(const Part& part, int first, int count, int step, int n) {
+        const int lane = threadIdx.x & 31;
+        m = -INFINITY;
+        for (int i = first + lane * step; i < count; i += 32 * step) m = fmaxf(m, part(i)[n]);
+        m = warp_max(m);
+        const float base = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+#pragma unroll
+        for (int c = 0; c < kParts; ++c)
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) acc[c][e] = 0.f;
+#pragma unroll 4
+        for (int i = first; i < count; i += step) {
+            const float* one = part(i);
+            const float weight = exp2_fast(one[n] - base);
+            l = fmaf(weight, one[COLS + n], l);
+#pragma unroll
+            for (int c = 0; c < kParts; ++c) {
+                const float* from = one + 2 * COLS + n * D + dim(lane, c, 0);
+                float v[kVec];
+                if (kVec == 4) {
+                    const float4 f = *reinterpret_cast<const float4*>(from);
+                    v[0] = f.x; v[1] = f.y; v[kVec - 2] = f.z; v[kVec - 1] = f.w;
+                } else {
+                    const float2 f = *reinterpret_cast<const float2*>(from);
+                    v[0] = f.x; v[1] = f.y;
+                }
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) acc[c][e] = fmaf(weight, v[e], acc[c][e]);
+            }
+        }
+    }
+    // the finished row
+    template <typename T, typename TC>
+    __device__ __forceinline__ void finish(const AttnParams& p, const PartHead& h, int n) const {
+        const int lane = threadIdx.x & 31, tok = n / p.group, row = h.first_row + tok, qh = h.head * p.group + n - tok * p.group;
+        T* out = reinterpret_cast<T*>(p.out) + (int64_t)row * p.os[0] + (int64_t)qh * p.os[1];
+        bool odd = false;
+#pragma unroll
+        for (int c = 0; c < kParts; ++c)
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) {
+                const float v = l == 0.f ? 0.f : acc[c][e] / l;
+                odd |= !(fabsf(v) < INFINITY);
+                store_elem(out + dim(lane, c, e), v);
+            }
+        if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, row, h.pos0 + tok, qh);
+    }
+};
 
 template <int D, int NT, typename T, typename TC>
 __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention_few_kernel(const __grid_constant__ AttnParams p) {
@@ -138,14 +197,20 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     Runs runs{total_tiles<kFewKeys>(p, reinterpret_cast<int64_t*>(smem)), (int64_t)gridDim.x * S::kWarps, kFewLeast};
     zero_blind_rows<T>(p);
     const int64_t me = (int64_t)blockIdx.x * S::kWarps + warp;
-    PartHead* heads = reinterpret_cast<PartHead*>(p.part) + me * 2;
-    float* parts = p.part + runs.workers * 2 * (sizeof(PartHead) / 4) + me * 2 * S::kPart;
+    // workspace: heads of the blocks' parts, blocks' parts, warps' parts
+    PartHead* block_heads = reinterpret_cast<PartHead*>(p.part) + blockIdx.x * 2;
+    float* block_parts = p.part + gridDim.x * 2 * (sizeof(PartHead) / 4) + (int64_t)blockIdx.x * 2 * S::kPart;
+    float* warp_parts = p.part + gridDim.x * 2 * (sizeof(PartHead) / 4) + ((int64_t)gridDim.x + (int64_t)blockIdx.x * S::kWarps) * 2 * S::kPart;
+    PartHead* warp_heads = reinterpret_cast<PartHead*>(smem + 256 + S::kWarps * kSlots * (S::kSlot + 16));
+    PartHead* heads = warp_heads + warp * 2;
+    float* parts = warp_parts + warp * 2 * S::kPart;
     const int64_t run0 = runs.begin(me), run1 = runs.begin(me + 1);
     if (lane < 2) heads[lane].begins = heads[lane].ends = -1;
-    if (run0 >= run1) return;
+    if (threadIdx.x < 2) block_heads[threadIdx.x].begins = block_heads[threadIdx.x].ends = -1;
+    __syncwarp();
 
     ItemCursor<kFewKeys> cur, ahead;
-    locate(p, run0, cur);
+    if (run0 < run1) locate(p, run0, cur);
     ahead = cur;
 
     // ---- issue side: keys and values of one group after the other into the ring
@@ -191,7 +256,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (++issue_slot == kSlots) issue_slot = 0;
     };
-    look();
+    if (run0 < run1) look();
 #pragma unroll
     for (int i = 0; i < kSlots - 1; ++i) issue(i & 1);
     int slot = 0;
@@ -473,14 +538,57 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                         for (int h = 0; h < 2; ++h) part[2 * S::kCols + n * D + dim_of(i, h)] = acc[nt][i][c + 2 * h] * unit;
                 }
             if (lane == 0)
-                heads[which] = PartHead{first_row, tokens, cur.head, cur.seq, cur.pos0, begins, ends, runs.worker_of(at - cur.k + cur.span.count - 1)};
+                heads[which] = PartHead{first_row, tokens, cur.head, cur.seq, cur.pos0, begins, ends, runs.worker_of(at - cur.k + cur.span.count - 1) / S::kWarps};
         }
         at += steps;
         if (at < run1) cur.next_item(p);
     }
+
+    // ---- the parts of the block's warps: one that does not begin its item continues the one before it
+    __syncthreads();
+    int group = -1, task = 0;
+    for (int e = 0; e < 2 * S::kWarps;) {
+        if (warp_heads[e].begins < 0) { ++e; continue; }
+        ++group;
+        int entries[2] = {e, e};                 // first and last part
+        int count = 1;
+        for (int f = e + 1; f < 2 * S::kWarps; ++f) {
+            if (warp_heads[f].begins < 0) continue;
+            if (warp_heads[f].begins == 1) break;
+            entries[1] = f;
+            ++count;
+        }
+        e = entries[1] + 1;
+        const PartHead h = warp_heads[entries[0]];
+        const bool begins = h.begins == 1, ends = warp_heads[entries[1]].ends == 1;
+        // a first part may be either of its warp's two, all others are the first of theirs
+        auto part = [&](int i) { return warp_parts + (i == 0 ? entries[0] : (entries[0] / 2 + i) * 2) * (int64_t)S::kPart; };
+        const int cols = h.tokens * p.group;
+        for (int n = 0; n < cols; ++n, ++task) {
+            if (task % S::kWarps != warp) continue;
+            Joined<D> j;
+            j.template join<S::kCols>(part, 0, count, 1, n);
+            if (begins && ends) {
+                j.template finish<T, TC>(p, h, n);
+            } else {
+                float* to = block_parts + (group == 0 ? 0 : 1) * S::kPart;
+                if (lane == 0) { to[n] = j.m; to[S::kCols + n] = j.l; }
+#pragma unroll
+                for (int c = 0; c < Joined<D>::kParts; ++c)
+#pragma unroll
+                    for (int x = 0; x < Joined<D>::kVec; ++x) to[2 * S::kCols + n * D + Joined<D>::dim(lane, c, x)] = j.acc[c][x];
+            }
+        }
+        if (!(begins && ends) && threadIdx.x == 0) {
+            PartHead b = h;
+            b.begins = begins;
+            b.ends = ends;
+            block_heads[group == 0 ? 0 : 1] = b;
+        }
+    }
 }
 
-// Joins the parts of one item, a block per (warp of the grid above whose run has the item's beginning, column).
+// Joins the parts of one item from several blocks: a block per (block of the grid above whose run has the item's beginning, column).
 constexpr int kJoinWarps = 4;
 
 template <int D, int NT, typename T, typename TC>
@@ -489,9 +597,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_few_join_kernel(con
     __shared__ float sums[kJoinWarps][D + 2];
     pdl_trigger();
     pdl_wait();
-    const int64_t warps = gridDim.x;
     const PartHead* heads = reinterpret_cast<const PartHead*>(p.part);
-    const float* parts = p.part + warps * 2 * (sizeof(PartHead) / 4);
+    const float* parts = p.part + gridDim.x * 2 * (sizeof(PartHead) / 4);
     const int w0 = blockIdx.x, n = blockIdx.y;
     int which = -1;
 #pragma unroll
@@ -502,41 +609,35 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_few_join_kernel(con
     if (n >= h.tokens * p.group) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, count = h.last - w0 + 1;
     auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * w0 + which : 2 * (w0 + i)) * S::kPart; };
-    float m = -INFINITY;
-    for (int i = threadIdx.x; i < count; i += blockDim.x) m = fmaxf(m, part(i)[n]);
-    m = warp_max(m);
-    if (lane == 0) sums[warp][0] = m;
-    __syncthreads();
-    for (int i = 0; i < kJoinWarps; ++i) m = fmaxf(m, sums[i][0]);
-    __syncthreads();
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, acc[D / 32] = {};
-    for (int i = warp; i < count; i += kJoinWarps) {
-        const float* one = part(i);
-        const float weight = exp2_fast(one[n] - base);
-        l = fmaf(weight, one[S::kCols + n], l);
+    Joined<D> j;
+    j.template join<S::kCols>(part, warp, count, kJoinWarps, n);
+    if (count > 1) {                             // the warps' shares, in order
+        if (lane == 0) { sums[warp][D] = j.m; sums[warp][D + 1] = j.l; }
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(weight, one[2 * S::kCols + n * D + c * 32 + lane], acc[c]);
+        for (int c = 0; c < Joined<D>::kParts; ++c)
+#pragma unroll
+            for (int x = 0; x < Joined<D>::kVec; ++x) sums[warp][Joined<D>::dim(lane, c, x)] = j.acc[c][x];
+        __syncthreads();
+        if (warp != 0) return;
+        for (int w = 0; w < kJoinWarps; ++w) j.m = fmaxf(j.m, sums[w][D]);
+        const float base = j.m == -INFINITY ? 0.f : j.m;
+        j.l = 0.f;
+#pragma unroll
+        for (int c = 0; c < Joined<D>::kParts; ++c)
+#pragma unroll
+            for (int x = 0; x < Joined<D>::kVec; ++x) j.acc[c][x] = 0.f;
+        for (int w = 0; w < kJoinWarps; ++w) {
+            const float weight = exp2_fast(sums[w][D] - base);
+            j.l = fmaf(weight, sums[w][D + 1], j.l);
+#pragma unroll
+            for (int c = 0; c < Joined<D>::kParts; ++c)
+#pragma unroll
+                for (int x = 0; x < Joined<D>::kVec; ++x) j.acc[c][x] = fmaf(weight, sums[w][Joined<D>::dim(lane, c, x)], j.acc[c][x]);
+        }
+    } else if (warp != 0) {
+        return;
     }
-    if (lane == 0) sums[warp][D] = l;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) sums[warp][c * 32 + lane] = acc[c];
-    __syncthreads();
-    if (warp != 0) return;
-    l = 0.f;
-    for (int i = 0; i < kJoinWarps; ++i) l += sums[i][D];
-    const int row = h.first_row + n / p.group, qh = h.head * p.group + n % p.group;
-    T* out = reinterpret_cast<T*>(p.out) + (int64_t)row * p.os[0] + (int64_t)qh * p.os[1];
-    bool odd = false;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-        float v = 0.f;
-        for (int i = 0; i < kJoinWarps; ++i) v += sums[i][c * 32 + lane];
-        v = l == 0.f ? 0.f : v / l;
-        odd |= !(fabsf(v) < INFINITY);
-        store_elem(out + c * 32 + lane, v);
-    }
-    if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, row, h.pos0 + n / p.group, qh);
+    j.template finish<T, TC>(p, h, n);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -547,9 +648,8 @@ static int few(AttnParams p, int max_warps, size_t* need, cudaStream_t stream) {
     using S = FewShape<D, NT, TC>;
     p.tile_tokens = S::kCols / p.group;
     const int blocks = (int)min((int64_t)sm_count(), ((int64_t)max_warps + S::kWarps - 1) / S::kWarps);
-    const int64_t warps = (int64_t)blocks * S::kWarps;
     if (need) {
-        *need = warps * 2 * (sizeof(PartHead) + S::kPart * sizeof(float));
+        *need = (size_t)blocks * 2 * (sizeof(PartHead) + (1 + S::kWarps) * S::kPart * sizeof(float));
         return FK_OK;
     }
     auto kern = attention_few_kernel<D, NT, T, TC>;
@@ -557,15 +657,16 @@ static int few(AttnParams p, int max_warps, size_t* need, cudaStream_t stream) {
     FK_CUDA_OK(launch_pdl(kern, dim3(blocks), dim3(32 * S::kWarps), (size_t)S::kSmem, stream, p), "attention (few) launch");
     FK_LAUNCH_OK("attention (few) launch");
     const int cols = (int)min((int64_t)S::kCols, (int64_t)p.tile_tokens * p.group);
-    FK_CUDA_OK(launch_pdl(attention_few_join_kernel<D, NT, T, TC>, dim3((unsigned)warps, cols), dim3(32 * kJoinWarps), 0, stream, p), "attention (few) join launch");
+    FK_CUDA_OK(launch_pdl(attention_few_join_kernel<D, NT, T, TC>, dim3((unsigned)blocks, cols), dim3(32 * kJoinWarps), 0, stream, p), "attention (few) join launch");
     FK_LAUNCH_OK("attention (few) join launch");
     return FK_OK;
 }
 
 template <int D, typename T, typename TC>
 static int few_columns(const AttnParams& p, int cols, int max_warps, size_t* need, cudaStream_t stream) {
-    if (cols <= 8) return few<D, 1, T, TC>(p, max_warps, need, stream);
-    return few<D, 2, T, TC>(p, max_warps, need, stream);
+    if constexpr (D < 256)
+        if (cols > 8) return few<D, 2, T, TC>(p, max_warps, need, stream);
+    return few<D, 1, T, TC>(p, max_warps, need, stream);
 }
 
 template <typename T, typename TC>
@@ -580,7 +681,8 @@ static int few_dim(const AttnParams& p, int cols, int max_warps, size_t* need, c
 bool attention_few_supported(const AttnParams& p, int dtype, int max_query) {
     if (dtype != FK_BF16 && dtype != FK_F16) return false;
     if (p.c.head_dim != 64 && p.c.head_dim != 128 && p.c.head_dim != 256) return false;
-    if (max_query < 1 || (int64_t)max_query * p.group > 16) return false;
+    // two groups of 8 columns do not fit the registers at 256 dimensions
+    if (max_query < 1 || (int64_t)max_query * p.group > (p.c.head_dim == 256 ? 8 : 16)) return false;
     const int cb = dtype_bytes(p.c.dtype);
     return groups_aligned(p.c.key, p.c.key_stride, 3, cb, 16) && groups_aligned(p.c.value, p.c.value_stride, 3, cb, 16) && groups_aligned(p.query, p.qs, 2, 2, 4);
 }
