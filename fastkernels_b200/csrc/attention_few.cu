@@ -21,7 +21,7 @@
 
 #include "attention_items.cuh"
 #include "kernels.cuh"
-#include "tma.cuh"
+#include "tcgen05.cuh"
 
 namespace fk {
 
@@ -75,11 +75,6 @@ __device__ __forceinline__ uint2 lds8(uint32_t addr) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ float lds_float(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-    return v;
-}
 // `bytes` (0 or all) are copied, the rest of the destination becomes zero
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -93,33 +88,47 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int row, int group, int head, int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(group), "r"(head), "r"(page)
+        : "memory");
+}
+
 constexpr int kFewKeys = 16;                    // keys of a group
 constexpr int kFewLeast = 2;                    // shortest run of a warp, in groups
 
 template <int D, int NT, typename TC>
 struct FewShape {
     static constexpr bool kCodes = FewOps<TC>::kCodes;
-    static constexpr int kPitch = D * (int)sizeof(TC);                 // bytes of a row in a slot
-    static constexpr int kSlot = 16 * kPitch + (kCodes ? 128 : 0);     // rows, then their 16 scales
-    static constexpr int kWarps = kCodes && NT == 1 && D <= 128 ? 16 : 8;      // as many as the registers hold
+    static constexpr int kPitch = D * (int)sizeof(TC);                 // bytes of a row
+    static constexpr int kSlot = 16 * kPitch;
+    static constexpr int kGroups = kPitch >= 128 ? kPitch / 128 : 1;   // a slot is [groups of 128 bytes][16 rows]
+    static constexpr int kWarps = kCodes && NT == 1 && D <= 128 ? 12 : 8;      // as many as the registers hold
     static constexpr int kFit = 192 * 1024 / kWarps / kSlot;           // slots per warp in 192 KB
     static constexpr int kSlots = kFit > 8 ? 8 : kFit;
     static constexpr int kCols = 8 * NT;
     static constexpr int kPart = (D + 2) * kCols;                      // floats of a partial result: m, l per column, [column][D]
-    static constexpr int kHeads = kWarps * 2 * (int)sizeof(PartHead);
-    static constexpr int kSmem = kWarps * kSlots * (kSlot + 16) + 256 + kHeads;
+    // behind the ring, per slot: first key and row mask, scales of its rows, barrier
+    static constexpr int kSide = 8 + (kCodes ? 64 : 0) + 8;
+    static constexpr int kRing = kWarps * kSlots * kSlot;
+    static constexpr int kSmem = kRing + kWarps * kSlots * kSide + kWarps * 2 * (int)sizeof(PartHead) + 256;
     static_assert(kSlots >= 3, "a slot being read and two on their way");
+    static_assert(kSmem <= 227 * 1024, "shared memory of a block");
 };
 
-// 16-byte chunk of a slot's row in which a chunk of the source row is kept.  16-bit rows: ldmatrix reads eight rows of one
-// chunk.  Codes: a quarter of a warp reads chunks t = 0..3 of two neighbouring rows (keys), or two neighbouring chunks (units of 8
-// bytes at 64 dimensions) of rows four apart (values).
-template <int D, typename TC, bool VALUES>
-__device__ __forceinline__ int slot_chunk(int row, int chunk) {
-    if (!FewOps<TC>::kCodes) return chunk ^ (row & 7);
-    if (!VALUES) return D >= 128 ? chunk ^ ((row & 1) << 2) : chunk;
-    return D >= 128 ? chunk ^ (((row >> 2) & 3) << 1) : chunk ^ ((row >> 2) & 3);
+// Byte of a slot at which 16-byte chunk `chunk` of row `row` is kept: the layout of a tensor copy with 128-byte swizzle.  ldmatrix
+// reads eight rows of one chunk; with codes, a quarter of a warp reads chunks 0..3 (or 4..7) of two key rows that differ in bit 2, or
+// two neighbouring chunks of four value rows that differ in bits 1 and 2 (key_row below): no conflicts.  Rows of 64 bytes: two reads
+// of the values for one.
+template <int D, typename TC>
+__device__ __forceinline__ int slot_at(int row, int chunk) {
+    if (D * sizeof(TC) >= 128) return (chunk >> 3) * (16 * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+    return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
+// Key (row of the group) of row i < 8 of S^T, + 8 for the others.
+template <typename TC>
+__device__ __forceinline__ int key_row(int i) { return FewOps<TC>::kCodes ? ((i & 6) ^ ((i & 1) << 2)) | (i & 1) : i; }
 
 // Column n of an item joined from `count` parts, by one warp: lane l has dimensions 4 l .. 4 l + 3 (and 128 more each), or 2 l, 2 l + 1
 // at 64.  part(i) is the address of the i-th part.
@@ -179,29 +188,43 @@ struct Joined {
     }
 };
 
-template <int D, int NT, typename T, typename TC>
-__global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention_few_kernel(const __grid_constant__ AttnParams p) {
+// TMA: the 16 rows of a group lie in one page and come by one tensor copy (and one bulk copy of their scales); else by cp.async.
+template <int D, int NT, typename T, typename TC, bool TMA>
+__global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention_few_kernel(const __grid_constant__ AttnParams p, const __grid_constant__ CUtensorMap key_map,
+                                                                                         const __grid_constant__ CUtensorMap value_map) {
     using S = FewShape<D, NT, TC>;
     using OT = typename FewOps<TC>::T;
     constexpr bool kCodes = S::kCodes;
     constexpr int kMT = D / 16, kSlots = S::kSlots;
     constexpr float kShift = std::is_same<OT, __half>::value ? 14.f : 0.f;
-    extern __shared__ __align__(128) unsigned char smem[];
+    extern __shared__ __align__(1024) unsigned char smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    unsigned char* mine = smem + 256 + warp * kSlots * (S::kSlot + 16);
-    const uint32_t ring = smem_u32(mine);
-    int2* meta = reinterpret_cast<int2*>(mine + kSlots * S::kSlot);
+    const uint32_t ring = smem_u32(smem) + warp * kSlots * S::kSlot;
+    unsigned char* side = smem + S::kRing;
+    uint64_t* landed = reinterpret_cast<uint64_t*>(side) + warp * kSlots;                                               // tensor copies' barriers
+    int2* meta = reinterpret_cast<int2*>(side + S::kWarps * kSlots * 8) + warp * kSlots;
+    float* scales = reinterpret_cast<float*>(side + S::kWarps * kSlots * 16) + warp * kSlots * 16;                      // codes
+    PartHead* warp_heads = reinterpret_cast<PartHead*>(side + S::kWarps * kSlots * S::kSide);
+    int64_t* scratch = reinterpret_cast<int64_t*>(warp_heads + S::kWarps * 2);
+    int* abort_flag = reinterpret_cast<int*>(scratch + S::kWarps);
+    if (TMA) {
+        if (lane == 0) {
+            for (int i = 0; i < kSlots; ++i) mbar_init(&landed[i], 1);
+            mbar_init_fence();
+        }
+        __syncwarp();
+    }
+    if (threadIdx.x == 0) *abort_flag = 0;
     pdl_trigger();
     pdl_wait();
 
-    Runs runs{total_tiles<kFewKeys>(p, reinterpret_cast<int64_t*>(smem)), (int64_t)gridDim.x * S::kWarps, kFewLeast};
+    Runs runs{total_tiles<kFewKeys>(p, scratch), (int64_t)gridDim.x * S::kWarps, kFewLeast};
     zero_blind_rows<T>(p);
     const int64_t me = (int64_t)blockIdx.x * S::kWarps + warp;
     // workspace: heads of the blocks' parts, blocks' parts, warps' parts
     PartHead* block_heads = reinterpret_cast<PartHead*>(p.part) + blockIdx.x * 2;
     float* block_parts = p.part + gridDim.x * 2 * (sizeof(PartHead) / 4) + (int64_t)blockIdx.x * 2 * S::kPart;
     float* warp_parts = p.part + gridDim.x * 2 * (sizeof(PartHead) / 4) + ((int64_t)gridDim.x + (int64_t)blockIdx.x * S::kWarps) * 2 * S::kPart;
-    PartHead* warp_heads = reinterpret_cast<PartHead*>(smem + 256 + S::kWarps * kSlots * (S::kSlot + 16));
     PartHead* heads = warp_heads + warp * 2;
     float* parts = warp_parts + warp * 2 * S::kPart;
     const int64_t run0 = runs.begin(me), run1 = runs.begin(me + 1);
@@ -215,37 +238,54 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 
     // ---- issue side: keys and values of one group after the other into the ring
     int64_t left = run1 - run0;
-    int page = -1, in_page = 0;                  // of this lane's row (lanes 0..15) of the next group
-    int64_t koff = -1, voff = -1;                // bytes
+    int page = -1, in_page = 0;                  // of this lane's row (lanes 0..15) of the next group; tensor copies: of its first
+    bool seen = false;                           // some row sees this lane's key
+    int64_t koff = -1, voff = -1;                // bytes; cp.async only
     int issue_slot = 0;
     auto look = [&] {                            // the page table is read one group ahead of its use
         page = -1;
+        seen = false;
+        if (left <= 0) return;
         const int j = ahead.key0() + (lane & 15);
-        if (left > 0 && ahead.some_row_sees(p, j)) page = page_of(p.c, ahead.seq, j, in_page);
+        seen = ahead.some_row_sees(p, j);
+        if (TMA || seen) page = page_of(p.c, ahead.seq, TMA ? ahead.key0() : j, in_page);
     };
     auto issue = [&](bool values) {
         if (left > 0) {
             const uint32_t base = ring + issue_slot * S::kSlot;
             if (!values) {
-                koff = page < 0 ? -1 : row_offset(p.c.key_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
-                voff = page < 0 ? -1 : row_offset(p.c.value_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
-                const unsigned rows = __ballot_sync(kFull, page >= 0) & 0xffffu;
-                if (lane == 0) meta[issue_slot * 2] = make_int2(ahead.key0(), (int)rows);
+                if (!TMA) {
+                    koff = page < 0 ? -1 : row_offset(p.c.key_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
+                    voff = page < 0 ? -1 : row_offset(p.c.value_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
+                }
+                const unsigned rows = __ballot_sync(kFull, page >= 0 && seen) & 0xffffu;
+                if (lane == 0) meta[issue_slot] = make_int2(ahead.key0(), (int)rows);
             }
-            const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
-            constexpr int kChunks = S::kPitch / 16, kAtOnce = 32 / kChunks;
+            if (TMA) {
+                if (lane == 0) {
+                    uint64_t* bar = &landed[issue_slot];
+                    mbar_expect_tx(bar, S::kSlot + (kCodes && page >= 0 ? 64 : 0));
+                    tma_load_5d(base, values ? &value_map : &key_map, 0, in_page, 0, ahead.head, page < 0 ? p.c.pages : page, bar);
+                    if (kCodes && page >= 0)
+                        bulk_load(scales + issue_slot * 16,
+                                  (values ? p.c.value_scale : p.c.key_scale) + row_offset(values ? p.c.value_scale_stride : p.c.key_scale_stride, page, ahead.head, in_page), 64, bar);
+                }
+                __syncwarp();
+            } else {
+                const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
+                constexpr int kChunks = S::kPitch / 16, kAtOnce = 32 / kChunks;
 #pragma unroll
-            for (int i = 0; i < 16 / kAtOnce; ++i) {
-                const int row = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
-                const int64_t off = __shfl_sync(kFull, values ? voff : koff, row);
-                const int to = values ? slot_chunk<D, TC, true>(row, chunk) : slot_chunk<D, TC, false>(row, chunk);
-                copy16(base + row * S::kPitch + to * 16, off < 0 ? from : from + off + chunk * 16, off < 0 ? 0 : 16);
-            }
-            if (kCodes && lane < 16) {
-                const float* s = values ? p.c.value_scale : p.c.key_scale;
-                copy4(base + 16 * S::kPitch + lane * 4,
-                      page < 0 ? s : s + (values ? row_offset(p.c.value_scale_stride, page, ahead.head, in_page) : row_offset(p.c.key_scale_stride, page, ahead.head, in_page)),
-                      page < 0 ? 0 : 4);
+                for (int i = 0; i < 16 / kAtOnce; ++i) {
+                    const int row = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+                    const int64_t off = __shfl_sync(kFull, values ? voff : koff, row);
+                    copy16(base + slot_at<D, TC>(row, chunk), off < 0 ? from : from + off + chunk * 16, off < 0 ? 0 : 16);
+                }
+                if (kCodes && lane < 16) {
+                    const float* s = values ? p.c.value_scale : p.c.key_scale;
+                    copy4(smem_u32(scales + issue_slot * 16 + lane),
+                          page < 0 ? s : s + (values ? row_offset(p.c.value_scale_stride, page, ahead.head, in_page) : row_offset(p.c.key_scale_stride, page, ahead.head, in_page)),
+                          page < 0 ? 0 : 4);
+                }
             }
             if (values) {
                 --left;
@@ -253,24 +293,29 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 look();
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (!TMA) asm volatile("cp.async.commit_group;" ::: "memory");
         if (++issue_slot == kSlots) issue_slot = 0;
     };
     if (run0 < run1) look();
 #pragma unroll
     for (int i = 0; i < kSlots - 1; ++i) issue(i & 1);
     int slot = 0;
+    uint32_t phase = 0;
+    bool zeroed = false;                         // threads wrote to the slot that is read
     // the oldest slot has landed for the whole warp, and the one before it is free
     auto next_slot = [&](bool issue_values) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+        if (TMA) mbar_wait_spin(&landed[slot], phase, abort_flag);
+        else asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+        if (TMA && zeroed) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        zeroed = false;
         __syncwarp();
         issue(issue_values);
         const int now = slot;
-        if (++slot == kSlots) slot = 0;
+        if (++slot == kSlots) { slot = 0; phase ^= 1; }
         return now;
     };
 
-    const int row_lo = kCodes ? 4 * (g >> 1) + (g & 1) : g, row_hi = kCodes ? row_lo + 2 : g + 8;      // this thread's key rows of S^T
+    const int row_lo = key_row<TC>(g), row_hi = row_lo + 8;      // this thread's key rows of S^T
     int64_t at = run0;
     while (at < run1) {
         const int steps = (int)min((int64_t)(cur.span.count - cur.k), run1 - at);
@@ -333,15 +378,15 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
             // ---- scores
             const int ks = next_slot((kSlots - 1) & 1);
             const uint32_t kbase = ring + ks * S::kSlot;
-            const int2 what = meta[ks * 2];
+            const int2 what = meta[ks];
             float s[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
             if (kCodes) {
 #pragma unroll
                 for (int i = 0; i < D / 64; ++i) {
-                    const uint4 lo = lds16(kbase + row_lo * S::kPitch + slot_chunk<D, TC, false>(row_lo, 4 * i + t) * 16);
-                    const uint4 hi = lds16(kbase + row_hi * S::kPitch + slot_chunk<D, TC, false>(row_hi, 4 * i + t) * 16);
+                    const uint4 lo = lds16(kbase + slot_at<D, TC>(row_lo, 4 * i + t));
+                    const uint4 hi = lds16(kbase + slot_at<D, TC>(row_hi, 4 * i + t));
                     const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -350,7 +395,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                         for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a, qf[nt][4 * i + j], OT{});
                     }
                 }
-                const float k0 = lds_float(kbase + 16 * S::kPitch + row_lo * 4), k1 = lds_float(kbase + 16 * S::kPitch + row_hi * 4);
+                const float k0 = scales[ks * 16 + row_lo], k1 = scales[ks * 16 + row_hi];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     s[nt][0] *= qscale[nt][0] * k0; s[nt][1] *= qscale[nt][1] * k0;
@@ -364,7 +409,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 #pragma unroll
                 for (int kk = 0; kk < kMT; ++kk) {
                     uint32_t a[4];
-                    ldmatrix4(a, kbase + row * S::kPitch + slot_chunk<D, TC, false>(row, 2 * kk + (lane >> 4)) * 16);
+                    ldmatrix4(a, kbase + slot_at<D, TC>(row, 2 * kk + (lane >> 4)));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(kk & 1 ? s2[nt] : s[nt], a, qf[nt][kk], OT{});
                 }
@@ -421,8 +466,17 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
             // ---- values
             const int vs = next_slot(((kSlots - 1) & 1) ^ 1);
             const uint32_t vbase = ring + vs * S::kSlot;
+            if (TMA && what.y != 0xffff) {
+                // rows that nobody may see can hold anything, and 0 * infinity is no zero
+                for (int i = lane; i < 16 * S::kPitch / 16; i += 32) {
+                    const int row = (i >> 3) & 15;
+                    if (!((what.y >> row) & 1)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vbase + i * 16), "r"(0) : "memory");
+                }
+                __syncwarp();
+                zeroed = true;
+            }
             if (kCodes) {
-                float v0 = lds_float(vbase + 16 * S::kPitch + row_lo * 4), v1 = lds_float(vbase + 16 * S::kPitch + row_hi * 4);
+                float v0 = (what.y >> row_lo) & 1 ? scales[vs * 16 + row_lo] : 0.f, v1 = (what.y >> row_hi) & 1 ? scales[vs * 16 + row_hi] : 0.f;
                 float most = fmaxf(fabsf(v0), fabsf(v1));
                 most = fmaxf(most, __shfl_xor_sync(kFull, most, 4));
                 most = fmaxf(most, __shfl_xor_sync(kFull, most, 8));
@@ -454,12 +508,12 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                     uint32_t w[4][4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const int row = 4 * t + i;
+                        const int row = key_row<TC>(2 * t + (i & 1)) + 4 * (i & 2);
                         if (D >= 128) {
-                            const uint4 x = lds16(vbase + row * S::kPitch + slot_chunk<D, TC, true>(row, g + 8 * u) * 16);
+                            const uint4 x = lds16(vbase + slot_at<D, TC>(row, g + 8 * u));
                             w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
                         } else {
-                            const uint2 x = lds8(vbase + row * S::kPitch + slot_chunk<D, TC, true>(row, g >> 1) * 16 + (g & 1) * 8);
+                            const uint2 x = lds8(vbase + slot_at<D, TC>(row, g >> 1) + (g & 1) * 8);
                             w[i][0] = x.x; w[i][1] = x.y;
                         }
                     }
@@ -481,7 +535,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 #pragma unroll
                 for (int i = 0; i < kMT; ++i) {
                     uint32_t a[4];
-                    ldmatrix4_trans(a, vbase + row * S::kPitch + slot_chunk<D, TC, true>(row, 2 * i + ((lane >> 3) & 1)) * 16);
+                    ldmatrix4_trans(a, vbase + slot_at<D, TC>(row, 2 * i + ((lane >> 3) & 1)));
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][i], a, pf[nt], OT{});
                 }
@@ -498,6 +552,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 4);
                 l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 8);
                 l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 16);
+                if (TMA && *reinterpret_cast<volatile int*>(abort_flag)) l[nt][c] = NAN;       // a copy that never came: no number is right
             }
         if (begins && ends) {
             bool odd = false;
@@ -643,6 +698,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_few_join_kernel(con
 // ---------------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------------
+// One head's 16 rows of a page as [128-byte groups of columns][16 rows][128 bytes]
+static bool group_map(const void* base, const fk_kv_cache& c, const int64_t* stride, CUtensorMap* out) {
+    const int bytes = dtype_bytes(c.dtype), cols = 128 / bytes;
+    const uint64_t dims[5] = {(uint64_t)cols, (uint64_t)c.page_size, (uint64_t)(c.head_dim / cols), (uint64_t)c.kv_heads, (uint64_t)c.pages};
+    const uint64_t strides[4] = {(uint64_t)(stride[2] * bytes), 128, (uint64_t)(stride[1] * bytes), (uint64_t)(stride[0] * bytes)};
+    const uint32_t box[5] = {(uint32_t)cols, (uint32_t)kFewKeys, (uint32_t)(c.head_dim / cols), 1, 1};
+    return cache_tensor_map(base, c.dtype, 5, dims, strides, box, out);
+}
+
 template <int D, int NT, typename T, typename TC>
 static int few(AttnParams p, int max_warps, size_t* need, cudaStream_t stream) {
     using S = FewShape<D, NT, TC>;
@@ -652,10 +716,23 @@ static int few(AttnParams p, int max_warps, size_t* need, cudaStream_t stream) {
         *need = (size_t)blocks * 2 * (sizeof(PartHead) + (1 + S::kWarps) * S::kPart * sizeof(float));
         return FK_OK;
     }
-    auto kern = attention_few_kernel<D, NT, T, TC>;
-    FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), "attention (few) attr");
-    FK_CUDA_OK(launch_pdl(kern, dim3(blocks), dim3(32 * S::kWarps), (size_t)S::kSmem, stream, p), "attention (few) launch");
-    FK_LAUNCH_OK("attention (few) launch");
+    CUtensorMap key_map{}, value_map{};
+    auto launch = [&](auto kern) -> int {
+        FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), "attention (few) attr");
+        FK_CUDA_OK(launch_pdl(kern, dim3(blocks), dim3(32 * S::kWarps), (size_t)S::kSmem, stream, p, key_map, value_map), "attention (few) launch");
+        FK_LAUNCH_OK("attention (few) launch");
+        return FK_OK;
+    };
+    int st = -1;
+    if constexpr (S::kPitch >= 128) {
+        // Tensor copies where a group's rows lie in one page and its scales on 16 bytes: one instruction for what takes a warp 40 to 100
+        auto scales_ok = [&](const float* s, const int64_t* stride) { return stride[2] == 1 && groups_aligned(s, stride, 2, 4, 16); };
+        if (p.c.page_size % kFewKeys == 0 && (!S::kCodes || (scales_ok(p.c.key_scale, p.c.key_scale_stride) && scales_ok(p.c.value_scale, p.c.value_scale_stride))) &&
+            group_map(p.c.key, p.c, p.c.key_stride, &key_map) && group_map(p.c.value, p.c, p.c.value_stride, &value_map))
+            st = launch(attention_few_kernel<D, NT, T, TC, true>);
+    }
+    if (st < 0) st = launch(attention_few_kernel<D, NT, T, TC, false>);
+    if (st != FK_OK) return st;
     const int cols = (int)min((int64_t)S::kCols, (int64_t)p.tile_tokens * p.group);
     FK_CUDA_OK(launch_pdl(attention_few_join_kernel<D, NT, T, TC>, dim3((unsigned)blocks, cols), dim3(32 * kJoinWarps), 0, stream, p), "attention (few) join launch");
     FK_LAUNCH_OK("attention (few) join launch");

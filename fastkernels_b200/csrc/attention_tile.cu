@@ -81,18 +81,6 @@ __device__ __forceinline__ void arrive_first_release(uint64_t* bar) {
         "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\t"
         "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(smem_u32(bar)) : "memory");
 }
-// bounded like mbar_wait, without its back-off: every waiter here has its own barrier and the next step depends on it
-__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    if (mbar_try_wait(bar, parity)) return;
-    const long long limit = *abort_flag ? kWaitCyclesAfterAbort : kWaitCycles;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (clock64() - t0 > limit) {
-            *abort_flag = 1;
-            return;
-        }
-    }
-}
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t* dst) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(dst)) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -303,7 +291,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     return reinterpret_cast<const T*>(p.query) + (int64_t)(first_row + tok) * p.qs[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.qs[1] + chunk * 8;
                 };
                 if (!kCodes) {
-                    wait_bar(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
+                    mbar_wait_spin(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
 #pragma unroll 4
                     for (int i = 0; i < kSteps; ++i) {
                         const int r = w * 32 + i * kAtOnce + lane / kChunks;
@@ -319,7 +307,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             const T* q = source(w * 32 + (i0 + b) * kAtOnce + lane / kChunks);
                             raw[b] = q ? *reinterpret_cast<const uint4*>(q) : make_uint4(0, 0, 0, 0);
                         }
-                        if (i0 == 0) wait_bar(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
+                        if (i0 == 0) mbar_wait_spin(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
 #pragma unroll
                         for (int b = 0; b < kBatch; ++b) {
                             const int r = w * 32 + (i0 + b) * kAtOnce + lane / kChunks;
@@ -362,7 +350,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         asm volatile("cp.async.wait_group 0;" ::: "memory");
                         announce(x);
                     }
-                    wait_bar(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
+                    mbar_wait_spin(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
                 }
                 const uint32_t base = ring + slot * S::kSlot;
                 const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
@@ -418,7 +406,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         const int j = c.key0() + lane * unit;
                         if (lane < units && j < c.span.end && (p.window == 0 || j + unit > window_start(p, c.pos0) || j < p.sinks)) page = page_of(p.c, c.seq, j, row);
                     };
-                    auto wait_slot = [&] { wait_bar(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag); };
+                    auto wait_slot = [&] { mbar_wait_spin(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag); };
                     auto tma_values = [&] {
                         constexpr int groups = D / 128;
                         const int slot = x % kSlots;
@@ -491,7 +479,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         asm volatile("cp.async.wait_group 0;" ::: "memory");
                         announce(x);
                     }
-                    wait_bar(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
+                    mbar_wait_spin(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
                 }
                 if (lane == 0) key_mask[meta * 4 + w] = rows;
                 if (kCodes) {
@@ -536,7 +524,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         // order of the loads: K(0), then [K(t + 1), V(t)] inside an item and [V(t), K(t + 1)] where t ends one
                         const int slot = (ends || t + 1 == tiles ? 2 * t + 1 : 2 * t + 2) % kSlots, key0 = c.key0(), lo = window_start(p, c.pos0);
                         const uint32_t base = ring + slot * S::kSlot;
-                        wait_bar(&bar.landed[slot], (landed >> slot) & 1, abort_flag);
+                        mbar_wait_spin(&bar.landed[slot], (landed >> slot) & 1, abort_flag);
                         landed ^= 1u << slot;
                         for (int r = lane; r < kTileKeys; r += 32) {
                             const int j = key0 + r;
@@ -568,7 +556,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     if (++slot == kSlots) { slot = 0; phase ^= 1; }
                 };
                 auto scores = [&](int t, bool ends) {
-                    wait_bar(&bar.full[slot], phase, abort_flag);
+                    mbar_wait_spin(&bar.full[slot], phase, abort_flag);
                     tc_fence_after_sync();
                     if (leader) {
                         const uint32_t d = tmem_s + (t & 1) * kTileKeys, k = k_low + slot * (S::kSlot >> 4);
@@ -583,12 +571,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     next();
                 };
                 auto values = [&](int t, bool begins) {
-                    wait_bar(&bar.full[slot], phase, abort_flag);
+                    mbar_wait_spin(&bar.full[slot], phase, abort_flag);
                     if (begins) {
-                        if (o_segment > 0) wait_bar(&bar.o_empty, (o_segment - 1) & 1, abort_flag);
+                        if (o_segment > 0) mbar_wait_spin(&bar.o_empty, (o_segment - 1) & 1, abort_flag);
                         ++o_segment;
                     }
-                    wait_bar(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
+                    mbar_wait_spin(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
                     tc_fence_after_sync();
                     if (leader) {
                         const uint32_t a = tmem_s + (t & 1) * kTileKeys, v = v_low + slot * (S::kSlot >> 4);
@@ -605,7 +593,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     const bool ends = c.k + 1 >= c.span.count;
                     if (first) {
                         if (t > 0) values(t - 1, last_began);
-                        wait_bar(&bar.q_full, segment & 1, abort_flag);
+                        mbar_wait_spin(&bar.q_full, segment & 1, abort_flag);
                         ++segment;
                     }
                     scores(t, ends || t + 1 == tiles);
@@ -637,7 +625,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const int pos = c.pos0 + tok, meta = t % kMetaRing;
                 const int key0 = c.key0();
                 const bool inside = key0 + kTileKeys - 1 <= c.pos0 && (p.window == 0 || key0 >= window_start(p, c.pos1) || key0 + kTileKeys <= p.sinks);
-                wait_bar(&bar.keys_full[meta], (t / kMetaRing) & 1, abort_flag);
+                mbar_wait_spin(&bar.keys_full[meta], (t / kMetaRing) & 1, abort_flag);
                 uint32_t there[2] = {0xffffffffu, 0xffffffffu};          // one bit per key: its page is not missing
                 bool complete;
                 if (TMA) {
@@ -653,7 +641,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     there[0] = ((v.x >> (16 * half)) & 0xffffu) | ((v.y >> (16 * half)) << 16);
                     there[1] = ((v.z >> (16 * half)) & 0xffffu) | ((v.w >> (16 * half)) << 16);
                 }
-                wait_bar(&bar.s_full[t & 1], (t >> 1) & 1, abort_flag);
+                mbar_wait_spin(&bar.s_full[t & 1], (t >> 1) & 1, abort_flag);
                 tc_fence_after_sync();
                 const uint32_t s_addr = tmem_s + lanes + (t & 1) * kTileKeys;
                 float s[64];
@@ -717,7 +705,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 if (!begins) {
                     const float factor = alpha * unit_scale;
                     if (__any_sync(kFull, factor != 1.f)) {              // the same in both warps of a row
-                        wait_bar(&bar.o_done, (t - 1) & 1, abort_flag);
+                        mbar_wait_spin(&bar.o_done, (t - 1) & 1, abort_flag);
                         tc_fence_after_sync();
 #pragma unroll 1
                         for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 16) {
@@ -764,7 +752,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     sums[half * 128 + r] = l;
                     meet();
                     l = sums[r] + sums[128 + r];                         // in this order in both threads
-                    wait_bar(&bar.o_done, t & 1, abort_flag);
+                    mbar_wait_spin(&bar.o_done, t & 1, abort_flag);
                     tc_fence_after_sync();
                     const int tokens = c.tokens(p), cols = tokens * p.group, first_row = c.first_row(p);
                     const bool whole = ends && began_k == 0;
@@ -902,7 +890,7 @@ static bool page_map(const void* base, const fk_kv_cache& c, const int64_t* stri
     const uint64_t dims[4] = {(uint64_t)c.head_dim, (uint64_t)c.page_size, (uint64_t)c.kv_heads, (uint64_t)c.pages};
     const uint64_t strides[3] = {(uint64_t)stride[2] * 2, (uint64_t)stride[1] * 2, (uint64_t)stride[0] * 2};
     const uint32_t box[4] = {64, (uint32_t)unit, 1, 1};
-    return paged_tensor_map(base, c.dtype == FK_BF16, dims, strides, box, out);
+    return cache_tensor_map(base, c.dtype, 4, dims, strides, box, out);
 }
 
 template <int D, typename T, typename TC, bool TMA>

@@ -373,14 +373,15 @@ bool column_pair_map(const void* base, uint64_t rows, uint64_t cols, uint32_t bo
     return true;
 }
 
-bool paged_tensor_map(const void* base, bool bf16, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMap* out) {
+bool cache_tensor_map(const void* base, int dtype, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMap* out) {
     EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    cuuint64_t d[4], s[3];
-    cuuint32_t b[4], elem[4] = {1, 1, 1, 1};
-    for (int i = 0; i < 4; ++i) { d[i] = dims[i]; b[i] = box[i]; if (i < 3) s[i] = strides[i]; }
-    return fn(out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base), d, s, b, elem,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    if (!fn || rank > 5) return false;
+    const CUtensorMapDataType type = dtype == FK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : dtype == FK_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    cuuint64_t d[5], s[4];
+    cuuint32_t b[5], elem[5] = {1, 1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) { d[i] = dims[i]; b[i] = box[i]; if (i + 1 < rank) s[i] = strides[i]; }
+    return fn(out, type, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, elem, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool tc_path_supported(const ExpertParams& p, int weight_dtype) {

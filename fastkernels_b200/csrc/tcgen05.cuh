@@ -106,8 +106,8 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
 bool weight_tensor_map(const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, CUtensorMap* out);
 bool column_pair_map(const void* base, uint64_t rows, uint64_t cols, uint32_t box_rows, CUtensorMap* out);
 bool gate_up_pair_map(const void* base, uint64_t experts, uint64_t half_rows, uint64_t cols, uint32_t box_rows, CUtensorMap* out);
-// Map of a 4-D tensor of bf16 or fp16 (dims and box innermost first, strides in bytes of dims 1..3), 128-byte swizzle, zeros outside;
-// not cached.  False where the encoder refuses it.
-bool paged_tensor_map(const void* base, bool bf16, const uint64_t (&dims)[4], const uint64_t (&strides)[3], const uint32_t (&box)[4], CUtensorMap* out);
+// Map of a tensor of `rank` dimensions (dims and box innermost first, strides in bytes of dims 1 ..) of an fk_dtype other than fp32,
+// 128-byte swizzle, zeros outside; not cached.  False where the encoder refuses it.
+bool cache_tensor_map(const void* base, int dtype, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMap* out);
 
 }  // namespace fk

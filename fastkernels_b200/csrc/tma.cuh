@@ -71,6 +71,19 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
+// The same without the back-off, for warps whose next step is what everything waits for.
+__device__ __forceinline__ void mbar_wait_spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    if (mbar_try_wait(bar, parity)) return;
+    const long long limit = *abort_flag ? kWaitCyclesAfterAbort : kWaitCycles;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (clock64() - t0 > limit) {
+            *abort_flag = 1;
+            return;
+        }
+    }
+}
+
 // Contiguous global -> shared copy of `bytes` (multiple of 16, both addresses 16-byte aligned);
 // completion is signalled on `bar` as transaction bytes.
 __device__ __forceinline__ void bulk_load(void* dst_smem, const void* src_gmem, uint32_t bytes, uint64_t* bar) {
