@@ -61,10 +61,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t codes_to_half2(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(two & 0xffffu), __NV_E4M3);
-    return (uint32_t)h.x | ((uint32_t)h.y << 16);
-}
 __device__ __forceinline__ uint4 lds16(uint32_t addr) {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
@@ -390,7 +386,9 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                     const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint32_t a[4] = {codes_to_half2(wl[j]), codes_to_half2(wh[j]), codes_to_half2(wl[j] >> 16), codes_to_half2(wh[j] >> 16)};
+                        uint32_t a[4];
+                        codes4_to_half(wl[j], a[0], a[2]);
+                        codes4_to_half(wh[j], a[1], a[3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a, qf[nt][4 * i + j], OT{});
                     }
@@ -518,17 +516,19 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                         }
                     }
 #pragma unroll
-                    for (int j = 0; j < kWords; ++j)
+                    for (int j = 0; j < kWords; ++j) {
+                        uint32_t both[2][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) codes4_to_half(w[i][j], both[0][i], both[1][i]);
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            uint32_t c[4];
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) c[i] = codes_to_half2(w[i][j] >> (16 * h));
+                            const uint32_t (&c)[4] = both[h];
                             const uint32_t a[4] = {__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[0], c[1], 0x7632), __byte_perm(c[2], c[3], 0x5410),
                                                    __byte_perm(c[2], c[3], 0x7632)};
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][u * 8 + j * 2 + h], a, pf[nt], OT{});
                         }
+                    }
                 }
             } else {
                 const int row = (lane & 7) + ((lane >> 4) << 3);

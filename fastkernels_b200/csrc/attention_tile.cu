@@ -164,12 +164,8 @@ __device__ __forceinline__ uint32_t tile_pack(float lo, float hi, __half) {
 }
 __device__ __forceinline__ uint4 codes8_to_half(uint2 c) {
     uint4 r;
-    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(((i < 2 ? c.x : c.y) >> (16 * (i & 1))) & 0xffffu), __NV_E4M3);
-        w[i] = (uint32_t)h.x | ((uint32_t)h.y << 16);
-    }
+    codes4_to_half(c.x, r.x, r.y);
+    codes4_to_half(c.y, r.z, r.w);
     return r;
 }
 

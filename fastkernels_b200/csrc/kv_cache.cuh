@@ -87,17 +87,21 @@ __device__ __forceinline__ void load8(const __half* p, int n, float (&v)[8]) {
         for (int i = 0; i < 8; ++i) v[i] = i < n ? __half2float(p[i]) : 0.f;
     }
 }
-__device__ __forceinline__ float2 e4m3x2_to_float2(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
-    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+// Four codes -> two pairs of fp16 (exact): one conversion per pair and nothing else; the conversion of the fp8 header's type costs four
+// instructions per pair, which bound the kernels that read codes.
+__device__ __forceinline__ void codes4_to_half(uint32_t four, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(four));
 }
 template <bool WIDE>
 __device__ __forceinline__ void load8(const __nv_fp8_e4m3* p, int n, float (&v)[8]) {
     if (WIDE) {
         const uint2 a = *reinterpret_cast<const uint2*>(p);
+        uint32_t h[4];
+        codes4_to_half(a.x, h[0], h[1]);
+        codes4_to_half(a.y, h[2], h[3]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float2 f = e4m3x2_to_float2(((i < 2 ? a.x : a.y) >> (16 * (i & 1))) & 0xffffu);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
             v[2 * i] = f.x; v[2 * i + 1] = f.y;
         }
     } else {
