@@ -91,22 +91,26 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-constexpr int kFewKeys = 16;                    // keys of a group
+constexpr int kFewKeys = 16;                    // keys of one product, rows of a tensor copy
 constexpr int kFewLeast = 2;                    // shortest run of a warp, in groups
 
 template <int D, int NT, typename TC>
 struct FewShape {
     static constexpr bool kCodes = FewOps<TC>::kCodes;
     static constexpr int kPitch = D * (int)sizeof(TC);                 // bytes of a row
-    static constexpr int kSlot = 16 * kPitch;
-    static constexpr int kGroups = kPitch >= 128 ? kPitch / 128 : 1;   // a slot is [groups of 128 bytes][16 rows]
+    // Keys of a group: 32 where rows are short, so that what a group costs beside its bytes (waits, maxima, page numbers) is spread over more
+    // of them (128 dimensions in 8 bits, 128 x 8000: 16 keys 335 us)
+    static constexpr int kTiles = kPitch <= 128 ? 2 : 1, kKeys = 16 * kTiles;
+    static constexpr uint32_t kAllRows = 0xffffffffu >> (32 - kKeys);
+    static constexpr int kSlot = kKeys * kPitch;
+    static constexpr int kGroups = kPitch >= 128 ? kPitch / 128 : 1;   // a slot is [groups of 128 bytes][keys]
     static constexpr int kWarps = kCodes && NT == 1 && D <= 128 ? 12 : 8;      // as many as the registers hold
     static constexpr int kFit = 192 * 1024 / kWarps / kSlot;           // slots per warp in 192 KB
     static constexpr int kSlots = kFit > 8 ? 8 : kFit;
     static constexpr int kCols = 8 * NT;
     static constexpr int kPart = (D + 2) * kCols;                      // floats of a partial result: m, l per column, [column][D]
     // behind the ring, per slot: first key and row mask, scales of its rows, barrier
-    static constexpr int kSide = 8 + (kCodes ? 64 : 0) + 8;
+    static constexpr int kSide = 8 + (kCodes ? 4 * kKeys : 0) + 8;
     static constexpr int kRing = kWarps * kSlots * kSlot;
     static constexpr int kSmem = kRing + kWarps * kSlots * kSide + kWarps * 2 * (int)sizeof(PartHead) + 256;
     static_assert(kSlots >= 3, "a slot being read and two on their way");
@@ -199,7 +203,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     unsigned char* side = smem + S::kRing;
     uint64_t* landed = reinterpret_cast<uint64_t*>(side) + warp * kSlots;                                               // tensor copies' barriers
     int2* meta = reinterpret_cast<int2*>(side + S::kWarps * kSlots * 8) + warp * kSlots;
-    float* scales = reinterpret_cast<float*>(side + S::kWarps * kSlots * 16) + warp * kSlots * 16;                      // codes
+    float* scales = reinterpret_cast<float*>(side + S::kWarps * kSlots * 16) + warp * kSlots * S::kKeys;                // codes
     PartHead* warp_heads = reinterpret_cast<PartHead*>(side + S::kWarps * kSlots * S::kSide);
     int64_t* scratch = reinterpret_cast<int64_t*>(warp_heads + S::kWarps * 2);
     int* abort_flag = reinterpret_cast<int*>(scratch + S::kWarps);
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     pdl_trigger();
     pdl_wait();
 
-    Runs runs{total_tiles<kFewKeys>(p, scratch), (int64_t)gridDim.x * S::kWarps, kFewLeast};
+    Runs runs{total_tiles<S::kKeys>(p, scratch), (int64_t)gridDim.x * S::kWarps, kFewLeast};
     zero_blind_rows<T>(p);
     const int64_t me = (int64_t)blockIdx.x * S::kWarps + warp;
     // workspace: heads of the blocks' parts, blocks' parts, warps' parts
@@ -228,13 +232,13 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     if (threadIdx.x < 2) block_heads[threadIdx.x].begins = block_heads[threadIdx.x].ends = -1;
     __syncwarp();
 
-    ItemCursor<kFewKeys> cur, ahead;
+    ItemCursor<S::kKeys> cur, ahead;
     if (run0 < run1) locate(p, run0, cur);
     ahead = cur;
 
     // ---- issue side: keys and values of one group after the other into the ring
     int64_t left = run1 - run0;
-    int page = -1, in_page = 0;                  // of this lane's row (lanes 0..15) of the next group; tensor copies: of its first
+    int page = -1, in_page = 0;                  // of this lane's row of the next group; tensor copies: of the first of its 16 rows
     bool seen = false;                           // some row sees this lane's key
     int64_t koff = -1, voff = -1;                // bytes; cp.async only
     int issue_slot = 0;
@@ -242,9 +246,9 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
         page = -1;
         seen = false;
         if (left <= 0) return;
-        const int j = ahead.key0() + (lane & 15);
+        const int j = ahead.key0() + (lane & (S::kKeys - 1));
         seen = ahead.some_row_sees(p, j);
-        if (TMA || seen) page = page_of(p.c, ahead.seq, TMA ? ahead.key0() : j, in_page);
+        if (TMA || seen) page = page_of(p.c, ahead.seq, TMA ? j & ~15 : j, in_page);
     };
     auto issue = [&](bool values) {
         if (left > 0) {
@@ -254,16 +258,17 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                     koff = page < 0 ? -1 : row_offset(p.c.key_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
                     voff = page < 0 ? -1 : row_offset(p.c.value_stride, page, ahead.head, in_page) * (int64_t)sizeof(TC);
                 }
-                const unsigned rows = __ballot_sync(kFull, page >= 0 && seen) & 0xffffu;
+                const unsigned rows = __ballot_sync(kFull, page >= 0 && seen) & S::kAllRows;
                 if (lane == 0) meta[issue_slot] = make_int2(ahead.key0(), (int)rows);
             }
             if (TMA) {
-                if (lane == 0) {
-                    uint64_t* bar = &landed[issue_slot];
-                    mbar_expect_tx(bar, S::kSlot + (kCodes && page >= 0 ? 64 : 0));
-                    tma_load_5d(base, values ? &value_map : &key_map, 0, in_page, 0, ahead.head, page < 0 ? p.c.pages : page, bar);
+                uint64_t* bar = &landed[issue_slot];
+                const unsigned there = __ballot_sync(kFull, page >= 0);
+                if (lane == 0) mbar_expect_tx(bar, S::kSlot + (kCodes ? 64 * ((there & 1) + (S::kTiles > 1 ? (there >> 16) & 1 : 0)) : 0));
+                if ((lane & 15) == 0 && lane < S::kKeys) {
+                    tma_load_5d(base + lane * 128, values ? &value_map : &key_map, 0, in_page, 0, ahead.head, page < 0 ? p.c.pages : page, bar);
                     if (kCodes && page >= 0)
-                        bulk_load(scales + issue_slot * 16,
+                        bulk_load(scales + issue_slot * S::kKeys + lane,
                                   (values ? p.c.value_scale : p.c.key_scale) + row_offset(values ? p.c.value_scale_stride : p.c.key_scale_stride, page, ahead.head, in_page), 64, bar);
                 }
                 __syncwarp();
@@ -271,14 +276,14 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
                 constexpr int kChunks = S::kPitch / 16, kAtOnce = 32 / kChunks;
 #pragma unroll
-                for (int i = 0; i < 16 / kAtOnce; ++i) {
+                for (int i = 0; i < S::kKeys / kAtOnce; ++i) {
                     const int row = i * kAtOnce + lane / kChunks, chunk = lane % kChunks;
                     const int64_t off = __shfl_sync(kFull, values ? voff : koff, row);
                     copy16(base + slot_at<D, TC>(row, chunk), off < 0 ? from : from + off + chunk * 16, off < 0 ? 0 : 16);
                 }
-                if (kCodes && lane < 16) {
+                if (kCodes && lane < S::kKeys) {
                     const float* s = values ? p.c.value_scale : p.c.key_scale;
-                    copy4(smem_u32(scales + issue_slot * 16 + lane),
+                    copy4(smem_u32(scales + issue_slot * S::kKeys + lane),
                           page < 0 ? s : s + (values ? row_offset(p.c.value_scale_stride, page, ahead.head, in_page) : row_offset(p.c.key_scale_stride, page, ahead.head, in_page)),
                           page < 0 ? 0 : 4);
                 }
@@ -360,7 +365,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 qscale[nt][0] = qscale[nt][1] = p.scale_log2;
             }
         }
-        float acc[NT][kMT][4], m[NT][2], l[NT][2], top = 0.f;
+        float acc[NT][kMT][4], m[NT][2], l[NT][2], top = 0.f, inv_top = 1.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -375,57 +380,62 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
             const int ks = next_slot((kSlots - 1) & 1);
             const uint32_t kbase = ring + ks * S::kSlot;
             const int2 what = meta[ks];
-            float s[NT][4];
+            float s[S::kTiles][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-            if (kCodes) {
+            for (int kt = 0; kt < S::kTiles; ++kt) {
 #pragma unroll
-                for (int i = 0; i < D / 64; ++i) {
-                    const uint4 lo = lds16(kbase + slot_at<D, TC>(row_lo, 4 * i + t));
-                    const uint4 hi = lds16(kbase + slot_at<D, TC>(row_hi, 4 * i + t));
-                    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+                for (int nt = 0; nt < NT; ++nt) s[kt][nt][0] = s[kt][nt][1] = s[kt][nt][2] = s[kt][nt][3] = 0.f;
+                if (kCodes) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t a[4];
-                        codes4_to_half(wl[j], a[0], a[2]);
-                        codes4_to_half(wh[j], a[1], a[3]);
+                    for (int i = 0; i < D / 64; ++i) {
+                        const uint4 lo = lds16(kbase + slot_at<D, TC>(row_lo + 16 * kt, 4 * i + t)), hi = lds16(kbase + slot_at<D, TC>(row_hi + 16 * kt, 4 * i + t));
+                        const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-                        for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a, qf[nt][4 * i + j], OT{});
+                        for (int j = 0; j < 4; ++j) {
+                            uint32_t a[4];
+                            codes4_to_half(wl[j], a[0], a[2]);
+                            codes4_to_half(wh[j], a[1], a[3]);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) mma16816(s[kt][nt], a, qf[nt][4 * i + j], OT{});
+                        }
                     }
+                    const float k0 = scales[ks * S::kKeys + row_lo + 16 * kt], k1 = scales[ks * S::kKeys + row_hi + 16 * kt];
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        s[kt][nt][0] *= qscale[nt][0] * k0; s[kt][nt][1] *= qscale[nt][1] * k0;
+                        s[kt][nt][2] *= qscale[nt][0] * k1; s[kt][nt][3] *= qscale[nt][1] * k1;
+                    }
+                } else {
+                    float s2[NT][4];                  // two chains of products
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
+                    const int row = (lane & 15) + 16 * kt;
+#pragma unroll
+                    for (int kk = 0; kk < kMT; ++kk) {
+                        uint32_t a[4];
+                        ldmatrix4(a, kbase + slot_at<D, TC>(row, 2 * kk + (lane >> 4)));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816(kk & 1 ? s2[nt] : s[kt][nt], a, qf[nt][kk], OT{});
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kt][nt][i] = (s[kt][nt][i] + s2[nt][i]) * p.scale_log2;
                 }
-                const float k0 = scales[ks * 16 + row_lo], k1 = scales[ks * 16 + row_hi];
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    s[nt][0] *= qscale[nt][0] * k0; s[nt][1] *= qscale[nt][1] * k0;
-                    s[nt][2] *= qscale[nt][0] * k1; s[nt][3] *= qscale[nt][1] * k1;
-                }
-            } else {
-                float s2[NT][4];                  // two chains of products
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) s2[nt][0] = s2[nt][1] = s2[nt][2] = s2[nt][3] = 0.f;
-                const int row = lane & 15;
-#pragma unroll
-                for (int kk = 0; kk < kMT; ++kk) {
-                    uint32_t a[4];
-                    ldmatrix4(a, kbase + slot_at<D, TC>(row, 2 * kk + (lane >> 4)));
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816(kk & 1 ? s2[nt] : s[nt], a, qf[nt][kk], OT{});
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[nt][i] = (s[nt][i] + s2[nt][i]) * p.scale_log2;
             }
             // ---- masks: rows that are not there, and keys that only some of the tokens see
-            const bool all = tokens == 1 || (what.x + 15 <= cur.pos0 && (p.window == 0 || what.x >= sure_lo || what.x + 15 < p.sinks));
-            if (what.y != 0xffff || !all) {
+            const bool all = tokens == 1 || (what.x + S::kKeys - 1 <= cur.pos0 && (p.window == 0 || what.x >= sure_lo || what.x + S::kKeys <= p.sinks));
+            const bool all_rows = (uint32_t)what.y == S::kAllRows;
+            if (!all_rows || !all) {
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int kt = 0; kt < S::kTiles; ++kt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = i < 2 ? row_lo : row_hi, n = nt * 8 + 2 * t + (i & 1);
-                        if (!((what.y >> row) & 1) || (!all && !sees(p, cur.pos0 + n / p.group, what.x + row))) s[nt][i] = -INFINITY;
-                    }
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int row = (i < 2 ? row_lo : row_hi) + 16 * kt, n = nt * 8 + 2 * t + (i & 1);
+                            if (!(((uint32_t)what.y >> row) & 1) || (!all && !sees(p, cur.pos0 + n / p.group, what.x + row))) s[kt][nt][i] = -INFINITY;
+                        }
             }
             // ---- running maximum, weights
             bool grew = false;
@@ -434,7 +444,8 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float x = fmaxf(s[nt][c], s[nt][c + 2]);
+                    float x = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+                    if (S::kTiles > 1) x = fmaxf(x, fmaxf(s[S::kTiles - 1][nt][c], s[S::kTiles - 1][nt][c + 2]));
                     x = fmaxf(x, __shfl_xor_sync(kFull, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(kFull, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(kFull, x, 16));
@@ -456,32 +467,46 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float base = m[nt][i & 1] == -INFINITY ? 0.f : m[nt][i & 1] - kShift;
-                    s[nt][i] = exp2_fast(s[nt][i] - base);
-                    l[nt][i & 1] += s[nt][i];
+                for (int c = 0; c < 2; ++c) {
+                    const float base = m[nt][c] == -INFINITY ? 0.f : m[nt][c] - kShift;
+#pragma unroll
+                    for (int kt = 0; kt < S::kTiles; ++kt) {
+                        s[kt][nt][c] = exp2_fast(s[kt][nt][c] - base);
+                        s[kt][nt][c + 2] = exp2_fast(s[kt][nt][c + 2] - base);
+                        l[nt][c] += s[kt][nt][c] + s[kt][nt][c + 2];
+                    }
                 }
             // ---- values
             const int vs = next_slot(((kSlots - 1) & 1) ^ 1);
             const uint32_t vbase = ring + vs * S::kSlot;
-            if (TMA && what.y != 0xffff) {
+            if (TMA && !all_rows) {
                 // rows that nobody may see can hold anything, and 0 * infinity is no zero
-                for (int i = lane; i < 16 * S::kPitch / 16; i += 32) {
-                    const int row = (i >> 3) & 15;
-                    if (!((what.y >> row) & 1)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vbase + i * 16), "r"(0) : "memory");
+                for (int i = lane; i < S::kSlot / 16; i += 32) {
+                    const int row = (i >> 3) & (S::kKeys - 1);
+                    if (!(((uint32_t)what.y >> row) & 1)) asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vbase + i * 16), "r"(0) : "memory");
                 }
                 __syncwarp();
                 zeroed = true;
             }
             if (kCodes) {
-                float v0 = (what.y >> row_lo) & 1 ? scales[vs * 16 + row_lo] : 0.f, v1 = (what.y >> row_hi) & 1 ? scales[vs * 16 + row_hi] : 0.f;
-                float most = fmaxf(fabsf(v0), fabsf(v1));
+                float v[S::kTiles][2], most = 0.f;
+#pragma unroll
+                for (int kt = 0; kt < S::kTiles; ++kt) {
+                    v[kt][0] = scales[vs * S::kKeys + row_lo + 16 * kt];
+                    v[kt][1] = scales[vs * S::kKeys + row_hi + 16 * kt];
+                    if (!all_rows) {
+                        if (!(((uint32_t)what.y >> (row_lo + 16 * kt)) & 1)) v[kt][0] = 0.f;
+                        if (!(((uint32_t)what.y >> (row_hi + 16 * kt)) & 1)) v[kt][1] = 0.f;
+                    }
+                    most = fmaxf(most, fmaxf(fabsf(v[kt][0]), fabsf(v[kt][1])));
+                }
                 most = fmaxf(most, __shfl_xor_sync(kFull, most, 4));
                 most = fmaxf(most, __shfl_xor_sync(kFull, most, 8));
                 most = fmaxf(most, __shfl_xor_sync(kFull, most, 16));
                 if (most > top) {                 // the same in all lanes
                     const float a = top / most;
                     top = most;
+                    inv_top = 1.f / top;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -489,55 +514,61 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 #pragma unroll
                             for (int c = 0; c < 4; ++c) acc[nt][i][c] *= a;
                 }
-                if (top > 0.f) { v0 /= top; v1 /= top; }
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) { s[nt][0] *= v0; s[nt][1] *= v0; s[nt][2] *= v1; s[nt][3] *= v1; }
-            }
-            uint32_t pf[NT][2];
+                for (int kt = 0; kt < S::kTiles; ++kt) {
+                    const float v0 = v[kt][0] * inv_top, v1 = v[kt][1] * inv_top;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                pf[nt][0] = transpose8x8(pack2(s[nt][0], s[nt][1], OT{}));
-                pf[nt][1] = transpose8x8(pack2(s[nt][2], s[nt][3], OT{}));
-            }
-            if (kCodes) {
-                constexpr int kUnits = D >= 128 ? D / 128 : 1, kWords = D >= 128 ? 4 : 2;
-#pragma unroll
-                for (int u = 0; u < kUnits; ++u) {
-                    uint32_t w[4][4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = key_row<TC>(2 * t + (i & 1)) + 4 * (i & 2);
-                        if (D >= 128) {
-                            const uint4 x = lds16(vbase + slot_at<D, TC>(row, g + 8 * u));
-                            w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
-                        } else {
-                            const uint2 x = lds8(vbase + slot_at<D, TC>(row, g >> 1) + (g & 1) * 8);
-                            w[i][0] = x.x; w[i][1] = x.y;
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < kWords; ++j) {
-                        uint32_t both[2][4];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) codes4_to_half(w[i][j], both[0][i], both[1][i]);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t (&c)[4] = both[h];
-                            const uint32_t a[4] = {__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[0], c[1], 0x7632), __byte_perm(c[2], c[3], 0x5410),
-                                                   __byte_perm(c[2], c[3], 0x7632)};
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][u * 8 + j * 2 + h], a, pf[nt], OT{});
-                        }
-                    }
+                    for (int nt = 0; nt < NT; ++nt) { s[kt][nt][0] *= v0; s[kt][nt][1] *= v0; s[kt][nt][2] *= v1; s[kt][nt][3] *= v1; }
                 }
-            } else {
-                const int row = (lane & 7) + ((lane >> 4) << 3);
+            }
 #pragma unroll
-                for (int i = 0; i < kMT; ++i) {
-                    uint32_t a[4];
-                    ldmatrix4_trans(a, vbase + slot_at<D, TC>(row, 2 * i + ((lane >> 3) & 1)));
+            for (int kt = 0; kt < S::kTiles; ++kt) {
+                uint32_t pf[NT][2];
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][i], a, pf[nt], OT{});
+                for (int nt = 0; nt < NT; ++nt) {
+                    pf[nt][0] = transpose8x8(pack2(s[kt][nt][0], s[kt][nt][1], OT{}));
+                    pf[nt][1] = transpose8x8(pack2(s[kt][nt][2], s[kt][nt][3], OT{}));
+                }
+                if (kCodes) {
+                    constexpr int kUnits = D >= 128 ? D / 128 : 1, kWords = D >= 128 ? 4 : 2;
+#pragma unroll
+                    for (int u = 0; u < kUnits; ++u) {
+                        uint32_t w[4][4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int row = key_row<TC>(2 * t + (i & 1)) + 4 * (i & 2) + 16 * kt;
+                            if (D >= 128) {
+                                const uint4 x = lds16(vbase + slot_at<D, TC>(row, g + 8 * u));
+                                w[i][0] = x.x; w[i][1] = x.y; w[i][2] = x.z; w[i][3] = x.w;
+                            } else {
+                                const uint2 x = lds8(vbase + slot_at<D, TC>(row, g >> 1) + (g & 1) * 8);
+                                w[i][0] = x.x; w[i][1] = x.y;
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < kWords; ++j) {
+                            uint32_t both[2][4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) codes4_to_half(w[i][j], both[0][i], both[1][i]);
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                const uint32_t (&c)[4] = both[h];
+                                const uint32_t a[4] = {__byte_perm(c[0], c[1], 0x5410), __byte_perm(c[0], c[1], 0x7632), __byte_perm(c[2], c[3], 0x5410),
+                                                       __byte_perm(c[2], c[3], 0x7632)};
+#pragma unroll
+                                for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][u * 8 + j * 2 + h], a, pf[nt], OT{});
+                            }
+                        }
+                    }
+                } else {
+                    const int row = (lane & 7) + ((lane >> 4) << 3) + 16 * kt;
+#pragma unroll
+                    for (int i = 0; i < kMT; ++i) {
+                        uint32_t a[4];
+                        ldmatrix4_trans(a, vbase + slot_at<D, TC>(row, 2 * i + ((lane >> 3) & 1)));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma16816(acc[nt][i], a, pf[nt], OT{});
+                    }
                 }
             }
         }
