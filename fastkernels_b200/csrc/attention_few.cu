@@ -112,7 +112,7 @@ struct FewShape {
     // behind the ring, per slot: first key and row mask, scales of its rows, barrier
     static constexpr int kSide = 8 + (kCodes ? 4 * kKeys : 0) + 8;
     static constexpr int kRing = kWarps * kSlots * kSlot;
-    static constexpr int kSmem = kRing + kWarps * kSlots * kSide + kWarps * 2 * (int)sizeof(PartHead) + 256;
+    static constexpr int kSmem = kRing + kWarps * kSlots * kSide + kWarps * 2 * (int)sizeof(PartHead) + kWarps * 16 + 16;
     static_assert(kSlots >= 3, "a slot being read and two on their way");
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
 };
@@ -206,7 +206,9 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     float* scales = reinterpret_cast<float*>(side + S::kWarps * kSlots * 16) + warp * kSlots * S::kKeys;                // codes
     PartHead* warp_heads = reinterpret_cast<PartHead*>(side + S::kWarps * kSlots * S::kSide);
     int64_t* scratch = reinterpret_cast<int64_t*>(warp_heads + S::kWarps * 2);
-    int* abort_flag = reinterpret_cast<int*>(scratch + S::kWarps);
+    int* abort_flag = reinterpret_cast<int*>(scratch + 2 * S::kWarps);
+    int64_t* upto = reinterpret_cast<int64_t*>(smem);              // over the ring, before its first copy
+    const int room = S::kRing / 8;
     if (TMA) {
         if (lane == 0) {
             for (int i = 0; i < kSlots; ++i) mbar_init(&landed[i], 1);
@@ -218,8 +220,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     pdl_trigger();
     pdl_wait();
 
-    Runs runs{total_tiles<S::kKeys>(p, scratch), (int64_t)gridDim.x * S::kWarps, kFewLeast};
-    zero_blind_rows<T>(p);
+    Runs runs{plan_tiles<S::kKeys>(p, scratch, upto, room), (int64_t)gridDim.x * S::kWarps, kFewLeast};
     const int64_t me = (int64_t)blockIdx.x * S::kWarps + warp;
     // workspace: heads of the blocks' parts, blocks' parts, warps' parts
     PartHead* block_heads = reinterpret_cast<PartHead*>(p.part) + blockIdx.x * 2;
@@ -233,7 +234,8 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     __syncwarp();
 
     ItemCursor<S::kKeys> cur, ahead;
-    if (run0 < run1) locate(p, run0, cur);
+    if (run0 < run1) locate(p, run0, upto, room, cur);
+    __syncthreads();                             // the plan's memory is the ring's from here on
     ahead = cur;
 
     // ---- issue side: keys and values of one group after the other into the ring
@@ -683,6 +685,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) attention_few_join_kernel(con
     __shared__ float sums[kJoinWarps][D + 2];
     pdl_trigger();
     pdl_wait();
+    if (blockIdx.y == 0) zero_blind_rows<T>(p);
     const PartHead* heads = reinterpret_cast<const PartHead*>(p.part);
     const float* parts = p.part + gridDim.x * 2 * (sizeof(PartHead) / 4);
     const int w0 = blockIdx.x, n = blockIdx.y;

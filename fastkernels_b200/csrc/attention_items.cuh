@@ -50,6 +50,14 @@ __device__ __forceinline__ bool sees(const AttnParams& p, int pos, int j) {
     return j <= pos && (p.window == 0 || j > pos - p.window || j < p.sinks);
 }
 
+// Bits of 32 consecutive positions from j0 on that a token at position pos sees.
+__device__ __forceinline__ uint32_t seen_bits(const AttnParams& p, int pos, int j0) {
+    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; };       // positions j0 .. j0 + n - 1
+    const uint32_t past = below(pos - j0 + 1);
+    if (p.window == 0) return past;
+    return past & (~below(pos - p.window - j0 + 1) | below(p.sinks - j0));
+}
+
 // A position in the order (sequence, head, tile of tokens, key tile).  All lanes of a warp hold the same.
 template <int KT>
 struct ItemCursor {
@@ -107,48 +115,69 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
     return v;
 }
 
-// All items' key tiles; every thread of the block calls it, `scratch` holds a word per warp.
+// The order's extent and, in shared memory, where each sequence ends in it: upto[s] key tiles up to and with sequence s, for as many
+// sequences as `room` holds (others are counted again by locate).  Every thread of the block calls it; `scratch` holds two words
+// per warp.
 template <int KT>
-__device__ __forceinline__ int64_t total_tiles(const AttnParams& p, int64_t* scratch) {
-    int64_t sum = 0;
-    for (int s = threadIdx.x; s < p.c.seqs; s += blockDim.x) {
-        const SeqRows r = rows_of_seq(p, s);
-        if (r.n > 0) sum += seq_tiles<KT>(p, r);
-    }
-    sum = warp_sum64(sum);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = sum;
-    __syncthreads();
+__device__ __forceinline__ int64_t plan_tiles(const AttnParams& p, int64_t* scratch, int64_t* upto, int room) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     int64_t all = 0;
-    for (int i = 0; i < (int)(blockDim.x >> 5); ++i) all += scratch[i];
-    return all * p.c.kv_heads;
-}
-
-// Cursor at key tile `target` of the order (target < total_tiles); a whole warp calls it.
-template <int KT>
-__device__ __forceinline__ void locate(const AttnParams& p, int64_t target, ItemCursor<KT>& c) {
-    const int lane = threadIdx.x & 31;
-    int64_t before = 0;
-    for (int s0 = 0; s0 < p.c.seqs; s0 += 32) {
-        const int s = s0 + lane;
+    for (int s0 = 0, turn = 0; s0 < p.c.seqs; s0 += blockDim.x, turn ^= 1) {
+        const int s = s0 + threadIdx.x;
         int64_t mine = 0;
         if (s < p.c.seqs) {
             const SeqRows r = rows_of_seq(p, s);
             if (r.n > 0) mine = seq_tiles<KT>(p, r) * p.c.kv_heads;
         }
-        int64_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t up = __shfl_up_sync(kFull, upto, o);
-            if (lane >= o) upto += up;
+            const int64_t up = __shfl_up_sync(kFull, mine, o);
+            if (lane >= o) mine += up;
         }
-        const unsigned past = __ballot_sync(kFull, before + upto > target);
+        if (lane == 31) scratch[turn * warps + warp] = mine;
+        __syncthreads();
+        int64_t before = all;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) before += scratch[turn * warps + w];
+            all += scratch[turn * warps + w];
+        }
+        if (s < p.c.seqs && s < room) upto[s] = before + mine;
+    }
+    __syncthreads();
+    return all;
+}
+
+// Cursor at key tile `target` of the order (target < the extent); a whole warp calls it.
+template <int KT>
+__device__ __forceinline__ void locate(const AttnParams& p, int64_t target, const int64_t* upto, int room, ItemCursor<KT>& c) {
+    const int lane = threadIdx.x & 31;
+    int64_t before = 0;
+    for (int s0 = 0; s0 < p.c.seqs; s0 += 32) {
+        const int s = s0 + lane;
+        int64_t end = 0;                         // of this lane's sequence
+        if (s0 + 32 <= room || p.c.seqs <= room) {
+            if (s < p.c.seqs) end = upto[s];
+        } else {
+            if (s < p.c.seqs) {
+                const SeqRows r = rows_of_seq(p, s);
+                if (r.n > 0) end = seq_tiles<KT>(p, r) * p.c.kv_heads;
+            }
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t up = __shfl_up_sync(kFull, end, o);
+                if (lane >= o) end += up;
+            }
+            end += before;
+        }
+        const unsigned past = __ballot_sync(kFull, s < p.c.seqs && end > target);
         if (past == 0) {
-            before += __shfl_sync(kFull, upto, 31);
+            before = __shfl_sync(kFull, end, min(31, p.c.seqs - s0 - 1));
             continue;
         }
         const int at = __ffs(past) - 1;
-        int64_t rest = target - before - __shfl_sync(kFull, upto - mine, at);
-        const int64_t per_head = __shfl_sync(kFull, mine, at) / p.c.kv_heads;
+        const int64_t start = at > 0 ? __shfl_sync(kFull, end, at > 0 ? at - 1 : 0) : before;
+        int64_t rest = target - start;
+        const int64_t per_head = (__shfl_sync(kFull, end, at) - start) / p.c.kv_heads;
         c.seq = s0 + at;
         c.rows = rows_of_seq(p, c.seq);
         c.head = (int)(rest / per_head);

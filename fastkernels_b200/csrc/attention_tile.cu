@@ -38,10 +38,11 @@ struct TileShape {
     static constexpr bool kCodes = sizeof(TC) == 1;
     static constexpr int kQuery = 128 * D * 2;                       // bytes of a block's query rows
     static constexpr int kSlot = 64 * D * 2;                         // 64 keys, or 128 values' half rows
-    static constexpr int kSlots = D == 256 ? (kCodes ? 4 : 5) : (kCodes ? 10 : 11);
+    static constexpr int kQueries = D == 256 ? 1 : 2;                // buffers of query rows: where they fit, the next item's come early
+    static constexpr int kSlots = D == 256 ? (kCodes ? 4 : 5) : (kCodes ? 8 : 9);
     static constexpr int kMeta = kMetaRing * (kCodes ? 2 * kTileKeys * 4 + 32 : 16);
     static constexpr int kExchange = 2 * 2 * 128 * 4;                // between the two threads of a row
-    static constexpr int kSmem = kQuery + kSlots * kSlot + 640 + kMeta + kExchange + 4 * 128 * (kCodes ? 4 : 0);
+    static constexpr int kSmem = kQueries * kQuery + kSlots * kSlot + 640 + kMeta + kExchange + 4 * 128 * (kCodes ? 4 : 0);
 
     static constexpr int kPart = (D + 2) * kTileRows;                // floats of a partial result: m, l per row, [row][D]
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
@@ -50,11 +51,10 @@ struct TileShape {
 
 struct TileBarriers {
     uint64_t full[12], empty[12], landed[12];
-    uint64_t q_full, q_empty, s_full[2], p_full[2], o_done, o_empty;
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done, o_empty;
     uint64_t keys_full[kMetaRing];
     uint32_t tmem;
     int abort_flag;
-    int64_t sums[kTileThreads / 32];
 };
 static_assert(sizeof(TileBarriers) <= 640, "fits behind the ring");
 
@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     constexpr float kShift = kHalf ? 7.f : 0.f, kLazy = 8.f - (kCodes ? 1.f : 0.f);
     constexpr int kSlots = S::kSlots;
     extern __shared__ __align__(1024) unsigned char smem[];
-    const uint32_t q_smem = smem_u32(smem), ring = q_smem + S::kQuery;
-    unsigned char* tail = smem + S::kQuery + kSlots * S::kSlot;
+    const uint32_t q_smem = smem_u32(smem), ring = q_smem + S::kQueries * S::kQuery;
+    unsigned char* tail = smem + S::kQueries * S::kQuery + kSlots * S::kSlot;
     TileBarriers& bar = *reinterpret_cast<TileBarriers*>(tail);
     uint32_t* key_mask = reinterpret_cast<uint32_t*>(tail + 640);                       // [kMetaRing][4]
     float* key_scale = reinterpret_cast<float*>(tail + 640 + kMetaRing * 16);           // codes: [kMetaRing][128], by column
@@ -226,9 +226,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     if (threadIdx.x == 0) {
         for (int i = 0; i < kSlots; ++i) { mbar_init(&bar.full[i], TMA ? 2 : 8); mbar_init(&bar.empty[i], 1); }
         for (int i = 0; i < kSlots; ++i) mbar_init(&bar.landed[i], 1);
-        mbar_init(&bar.q_full, 8);
-        mbar_init(&bar.q_empty, 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 16); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&bar.q_full[i], 8);
+            mbar_init(&bar.q_empty[i], 1); mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 16); }
         mbar_init(&bar.o_done, 1);
         mbar_init(&bar.o_empty, 16);
         for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], TMA ? 1 : 4);
@@ -244,17 +244,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     volatile int* abort_flag = &bar.abort_flag;
     pdl_wait();
 
-    const Runs runs{total_tiles<kTileKeys>(p, bar.sums), pairs, 1};
-    zero_blind_rows<T>(p);
+    int64_t* upto = reinterpret_cast<int64_t*>(smem);              // over the queries and the ring, before their first copy
+    const int room = (S::kQueries * S::kQuery + kSlots * S::kSlot) / 8;
+    const Runs runs{plan_tiles<kTileKeys>(p, reinterpret_cast<int64_t*>(exchange), upto, room), pairs, 1};
     const int64_t run0 = runs.begin(pair), run1 = runs.begin(pair + 1);
     const int tiles = (int)(run1 - run0);
     PartHead* heads = reinterpret_cast<PartHead*>(p.part) + 2 * (int64_t)pair;
     float* parts = p.part + runs.workers * 2 * (sizeof(PartHead) / 4) + 2 * (int64_t)pair * S::kPart;
     if (threadIdx.x == 0 && rank == 0) heads[0].begins = heads[0].ends = heads[1].begins = heads[1].ends = -1;
 
+    ItemCursor<kTileKeys> c;
+    if (tiles > 0) locate(p, run0, upto, room, c);
+    fence_async_proxy();                             // the plan's memory is the copies' from here on
+    __syncthreads();
     if (tiles > 0) {
-        ItemCursor<kTileKeys> c;
-        locate(p, run0, c);
         const int dim = p.c.head_dim;
         if (warp >= 8 && warp < kMmaWarp) {
             // ------------------------------------------------------------------------------------------------- producers
@@ -280,14 +283,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const int cols = c.tokens(p) * p.group, first_row = c.first_row(p);
                 constexpr int kChunks = D / 8, kAtOnce = 32 / kChunks < 1 ? 1 : 32 / kChunks, kSteps = 32 / kAtOnce, kBatch = 8;
                 const int chunk = lane % kChunks;
-                const uint32_t to = q_smem + (chunk >> 3) * (128 * 128);
+                const int buffer = segment % S::kQueries;
+                const uint32_t to = q_smem + buffer * S::kQuery + (chunk >> 3) * (128 * 128);
                 auto source = [&](int r) -> const T* {           // null: padding
                     const int n = rank * 128 + r, tok = n / p.group;
                     if (n >= cols || chunk * 8 >= dim) return nullptr;
                     return reinterpret_cast<const T*>(p.query) + (int64_t)(first_row + tok) * p.qs[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.qs[1] + chunk * 8;
                 };
                 if (!kCodes) {
-                    mbar_wait_spin(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
+                    mbar_wait_spin(&bar.q_empty[buffer], ((segment / S::kQueries) & 1) ^ 1, abort_flag);
 #pragma unroll 4
                     for (int i = 0; i < kSteps; ++i) {
                         const int r = w * 32 + i * kAtOnce + lane / kChunks;
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             const T* q = source(w * 32 + (i0 + b) * kAtOnce + lane / kChunks);
                             raw[b] = q ? *reinterpret_cast<const uint4*>(q) : make_uint4(0, 0, 0, 0);
                         }
-                        if (i0 == 0) mbar_wait_spin(&bar.q_empty, (segment & 1) ^ 1, abort_flag);
+                        if (i0 == 0) mbar_wait_spin(&bar.q_empty[buffer], ((segment / S::kQueries) & 1) ^ 1, abort_flag);
 #pragma unroll
                         for (int b = 0; b < kBatch; ++b) {
                             const int r = w * 32 + (i0 + b) * kAtOnce + lane / kChunks;
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 }
                 fence_async_proxy();
                 __syncwarp();
-                if (lane == 0) arrive_first_release(&bar.q_full);
+                if (lane == 0) arrive_first_release(&bar.q_full[buffer]);
             };
             // rows of a slot: keys take 16 of this warp's 32 (those of this block's half), values all 32 with half of their columns
             constexpr int kKeyChunks = D / 8, kKeyAtOnce = 32 / kKeyChunks < 1 ? 1 : 32 / kKeyChunks;
@@ -423,10 +427,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     look_unit();
                     for (int t = 0; t < tiles; ++t) {
                         constexpr int groups = D / 64;
-                        if (first) {
-                            if (t > 0) tma_values();
-                            load_query(segment);
-                        }
+                        if (first && t > 0) tma_values();
                         const int slot = x % kSlots, meta = t % kMetaRing, head = c.head;
                         const bool edge = edge_tile(p, c), ends = c.k + 1 >= c.span.count, values_now = t > 0 && !first;
                         wait_slot();                 // and with it for the last reader of this description (static_assert above)
@@ -443,6 +444,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         if (u < key_units && (lane & 3) == w)
                             pair_tma_load(ring + slot * S::kSlot + g * (64 * 128) + u * unit * 128, &key_map, g * 64, rw, head, pg < 0 ? p.c.pages : pg, full);
                         ++x;
+                        if (first) load_query(segment);
                         // on to the next tile: its page numbers arrive while the previous tile's values are issued
                         const int page_now = page, row_now = row;
                         if (t + 1 < tiles) {
@@ -551,17 +553,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 auto next = [&] {
                     if (++slot == kSlots) { slot = 0; phase ^= 1; }
                 };
-                auto scores = [&](int t, bool ends) {
+                auto scores = [&](int t, bool ends, int buffer) {
                     mbar_wait_spin(&bar.full[slot], phase, abort_flag);
                     tc_fence_after_sync();
                     if (leader) {
-                        const uint32_t d = tmem_s + (t & 1) * kTileKeys, k = k_low + slot * (S::kSlot >> 4);
+                        const uint32_t d = tmem_s + (t & 1) * kTileKeys, k = k_low + slot * (S::kSlot >> 4), q = q_low + buffer * (S::kQuery >> 4);
 #pragma unroll
                         for (int i = 0; i < D / 16; ++i)
-                            if (i * 16 < dim) pair_mma_ss(d, q_low + (((i >> 2) * (128 * 128) + (i & 3) * 32) >> 4), k + (((i >> 2) * (64 * 128) + (i & 3) * 32) >> 4), s_idesc, i > 0);
+                            if (i * 16 < dim) pair_mma_ss(d, q + (((i >> 2) * (128 * 128) + (i & 3) * 32) >> 4), k + (((i >> 2) * (64 * 128) + (i & 3) * 32) >> 4), s_idesc, i > 0);
                         pair_commit(&bar.s_full[t & 1]);
                         pair_commit(&bar.empty[slot]);
-                        if (ends) pair_commit(&bar.q_empty);
+                        if (ends) pair_commit(&bar.q_empty[buffer]);
                     }
                     __syncwarp();
                     next();
@@ -589,10 +591,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     const bool ends = c.k + 1 >= c.span.count;
                     if (first) {
                         if (t > 0) values(t - 1, last_began);
-                        mbar_wait_spin(&bar.q_full, segment & 1, abort_flag);
+                        mbar_wait_spin(&bar.q_full[segment % S::kQueries], (segment / S::kQueries) & 1, abort_flag);
                         ++segment;
                     }
-                    scores(t, ends || t + 1 == tiles);
+                    scores(t, ends || t + 1 == tiles, (segment - 1) % S::kQueries);
                     if (t > 0 && !first) values(t - 1, last_began);
                     last_began = first;
                     first = ends;
@@ -663,14 +665,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
 #pragma unroll
                     for (int i = 0; i < 64; ++i) s[i] = -s[i];
                 if (!complete || !inside) {
-                    // keys relative to this half's first: column i is key i (tensor copies), or 32 (i / 16) + i % 16
-                    const int first = key0 + (TMA ? 64 : 16) * half;
-                    const int hi = pos - first, lo = p.window > 0 ? pos - p.window - first : -1000, sink = p.window > 0 ? p.sinks - first : 0;
+                    // column i of this half is key i (tensor copies), or 32 (i / 16) + i % 16 of those from 16 half on
+                    uint32_t bits[2];
+                    if (TMA) {
+                        bits[0] = seen_bits(p, pos, key0 + half * 64);
+                        bits[1] = seen_bits(p, pos, key0 + half * 64 + 32);
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) {
-                        const int k = TMA ? i : (i >> 4) * 32 + (i & 15);
-                        if (!((there[i >> 5] >> (i & 31)) & 1u) || k > hi || (k <= lo && k >= sink)) s[i] = -INFINITY;
+                        for (int i = 0; i < 2; ++i)
+                            bits[i] = (seen_bits(p, pos, key0 + 64 * i + 16 * half) & 0xffffu) | (seen_bits(p, pos, key0 + 64 * i + 32 + 16 * half) << 16);
                     }
+                    bits[0] &= there[0];
+                    bits[1] &= there[1];
+#pragma unroll
+                    for (int i = 0; i < 64; ++i)
+                        if (!((bits[i >> 5] >> (i & 31)) & 1u)) s[i] = -INFINITY;
                 }
                 // ---- the row's maximum; the base of the powers only moves when it has to
                 float tops[8];
@@ -825,49 +834,78 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     }
 }
 
-// Joins the parts of one tile: block (pair whose run has the tile's beginning, 8 rows), a warp per row.
+// Joins the parts of one tile: block (pair whose run has the tile's beginning, 32 rows), four rows per warp, four dimensions per lane.
 template <int D, typename T, typename TC>
-__global__ void __launch_bounds__(256) attention_tile_join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(256, 4) attention_tile_join_kernel(const __grid_constant__ AttnParams p) {
     using S = TileShape<D, TC>;
+    constexpr int kRows = 4, kVec = D / 128;
     pdl_trigger();
     pdl_wait();
+    if (blockIdx.y == 0) zero_blind_rows<T>(p);
     const int64_t pairs = gridDim.x;
     const PartHead* heads = reinterpret_cast<const PartHead*>(p.part);
     const float* parts = p.part + pairs * 2 * (sizeof(PartHead) / 4);
-    const int w0 = blockIdx.x, lane = threadIdx.x & 31, n = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int w0 = blockIdx.x, lane = threadIdx.x & 31, n0 = blockIdx.y * 8 * kRows + (threadIdx.x >> 5) * kRows;
     int which = -1;
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         if (heads[2 * w0 + i].begins == 1 && heads[2 * w0 + i].ends == 0) which = i;
     if (which < 0) return;
     const PartHead h = heads[2 * w0 + which];
-    if (n >= h.tokens * p.group) return;
+    const int rows = min(kRows, h.tokens * p.group - n0);
+    if (rows <= 0) return;
     const int count = h.last - w0 + 1;
     auto part = [&](int i) { return parts + (int64_t)(i == 0 ? 2 * w0 + which : 2 * (w0 + i)) * S::kPart; };
-    float m = -INFINITY;
-    for (int i = lane; i < count; i += 32) m = fmaxf(m, part(i)[n]);
-    m = warp_max(m);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, acc[D / 32] = {};
+    float m[kRows], l[kRows] = {};
+    float4 acc[kRows][kVec];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        m[r] = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) acc[r][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int i = lane; i < count; i += 32)
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+            if (r < rows) m[r] = fmaxf(m[r], part(i)[n0 + r]);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) m[r] = warp_max(m[r]);
     for (int i = 0; i < count; ++i) {
         const float* one = part(i);
-        const float weight = tile_exp2(one[n] - base);
-        l = fmaf(weight, one[kTileRows + n], l);
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c)
-            if (c * 32 + lane < p.c.head_dim) acc[c] = fmaf(weight, one[2 * kTileRows + (int64_t)n * D + c * 32 + lane], acc[c]);
-    }
-    const int tok = n / p.group, qh = h.head * p.group + n - tok * p.group;
-    T* out = reinterpret_cast<T*>(p.out) + (int64_t)(h.first_row + tok) * p.os[0] + (int64_t)qh * p.os[1];
-    bool odd = false;
+        for (int r = 0; r < kRows; ++r) {
+            if (r >= rows) continue;
+            const float weight = tile_exp2(one[n0 + r] - (m[r] == -INFINITY ? 0.f : m[r]));
+            l[r] = fmaf(weight, one[kTileRows + n0 + r], l[r]);
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c)
-        if (c * 32 + lane < p.c.head_dim) {
-            const float v = l == 0.f ? 0.f : acc[c] / l;
-            odd |= !(fabsf(v) < INFINITY);
-            store_elem(out + c * 32 + lane, v);
+            for (int c = 0; c < kVec; ++c) {
+                if (c * 128 + lane * 4 >= p.c.head_dim) continue;
+                const float4 v = *reinterpret_cast<const float4*>(one + 2 * kTileRows + (int64_t)(n0 + r) * D + c * 128 + lane * 4);
+                acc[r][c].x = fmaf(weight, v.x, acc[r][c].x); acc[r][c].y = fmaf(weight, v.y, acc[r][c].y);
+                acc[r][c].z = fmaf(weight, v.z, acc[r][c].z); acc[r][c].w = fmaf(weight, v.w, acc[r][c].w);
+            }
         }
-    if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, h.first_row + tok, h.pos0 + tok, qh);
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        if (r >= rows) continue;
+        const int n = n0 + r, tok = n / p.group, qh = h.head * p.group + n - tok * p.group;
+        T* out = reinterpret_cast<T*>(p.out) + (int64_t)(h.first_row + tok) * p.os[0] + (int64_t)qh * p.os[1];
+        bool odd = false;
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) {
+            const float v[4] = {acc[r][c].x, acc[r][c].y, acc[r][c].z, acc[r][c].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int d = c * 128 + lane * 4 + e;
+                if (d >= p.c.head_dim) continue;
+                const float x = l[r] == 0.f ? 0.f : v[e] / l[r];
+                odd |= !(fabsf(x) < INFINITY);
+                store_elem(out + d, x);
+            }
+        }
+        if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, h.first_row + tok, h.pos0 + tok, qh);
+    }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -910,7 +948,7 @@ static int launch_tile(const AttnParams& p, const CUtensorMap& key_map, const CU
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     FK_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p, key_map, value_map, unit), "attention (tile) launch");
     FK_LAUNCH_OK("attention (tile) launch");
-    FK_CUDA_OK(launch_pdl(attention_tile_join_kernel<D, T, TC>, dim3((unsigned)pairs, kTileRows / 8), dim3(256), 0, stream, p), "attention (tile) join launch");
+    FK_CUDA_OK(launch_pdl(attention_tile_join_kernel<D, T, TC>, dim3((unsigned)pairs, kTileRows / 32), dim3(256), 0, stream, p), "attention (tile) join launch");
     FK_LAUNCH_OK("attention (tile) join launch");
     return FK_OK;
 }
