@@ -9,8 +9,10 @@ and prints the same timing keys (`elapsed_ms_per_position`, `elapsed_ms_per_laye
 `layer_positions_per_second`), with what this library changes: all layers stay resident in HBM, packed once
 (`ResidentMoELayers`), and `--moe-impl b200` runs the sublayer on the CUDA kernels.
 
-Outside this library's scope and therefore stand-ins here: the sequence mixers (attention, DeltaNet) are the
-identity, and without `--checkpoint` the embedding, head and layer weights are drawn from seeds (the real
+Outside this library's scope and therefore stand-ins here: the sequence mixers of the real layers (gated attention,
+DeltaNet) are the identity by default; `--mixer attention` puts a causal attention sublayer with seeded projections in
+their place, over this library's paged key/value cache (`--cache-dtype fp8` keeps it in 8 bits, `--window` and `--sinks`
+limit what a token sees).  Without `--checkpoint` the embedding, head and layer weights are drawn from seeds (the real
 checkpoint is 72 GB and not bundled).  With `--checkpoint DIR` the MoE tensors of each layer are read from
 safetensors shards through `load_qwen36_moe_weights_from_safetensors`.
 
@@ -28,6 +30,7 @@ from typing import Optional, Sequence
 import torch
 import torch.nn.functional as F
 
+from .kv_cache import PagedKVCache
 from .spec import MoESpec, MoEWeights, synthetic_qwen36_spec
 from .workloads import make_moe_weights
 
@@ -58,11 +61,52 @@ def torch_moe_update(hidden: torch.Tensor, w: MoEWeights, top_k: int, eps: float
     return out
 
 
+class AttentionMixer:
+    """hidden + Wo attention(Wq x, Wk x, Wv x) of one layer with x = RMSNorm(hidden), one sequence, seeded projections `~ N(0, 1/H)`.
+
+    Keys and values live in a paged cache.  `impl` "b200" runs `paged_attention`; "reference" reads the sequence back from the
+    cache and takes the softmax with plain PyTorch ops in fp32 (the comparison arm, as for the MoE sublayer).
+    """
+
+    def __init__(self, hidden_size: int, *, q_heads: int, kv_heads: int, head_dim: int, impl: str, dtype: torch.dtype, seed: int, device: str,
+                 max_positions: int, page_size: int = 16, cache_dtype: Optional[torch.dtype] = None, window: int = 0, sinks: int = 0):
+        g = torch.Generator(device="cpu").manual_seed(seed)
+
+        def weight(rows, cols):
+            return (torch.randn(rows, cols, generator=g) * cols ** -0.5).to(device=device, dtype=dtype)
+        self.wq, self.wk, self.wv = weight(q_heads * head_dim, hidden_size), weight(kv_heads * head_dim, hidden_size), weight(kv_heads * head_dim, hidden_size)
+        self.wo = weight(hidden_size, q_heads * head_dim)
+        self.q_heads, self.kv_heads, self.head_dim, self.impl, self.dtype, self.window, self.sinks = q_heads, kv_heads, head_dim, impl, dtype, window, sinks
+        self.cache = PagedKVCache(-(-max_positions // page_size), kv_heads, head_dim, page_size=page_size, dtype=cache_dtype or dtype, device=device)
+
+    def __call__(self, hidden: torch.Tensor) -> torch.Tensor:
+        x = (hidden * torch.rsqrt((hidden * hidden).mean(-1, keepdim=True) + 1e-6)).to(self.dtype)
+        rows = x.shape[0]
+        q = (x @ self.wq.t()).view(rows, self.q_heads, self.head_dim)
+        self.cache.append((x @ self.wk.t()).view(rows, self.kv_heads, self.head_dim), (x @ self.wv.t()).view(rows, self.kv_heads, self.head_dim), [rows])
+        if self.impl == "b200":
+            out = self.cache.attend(q, window=self.window, sinks=self.sinks)
+        else:
+            k, v = self.cache.read(dtype=torch.float32 if self.cache.key_scale is not None else None)
+            group, length = self.q_heads // self.kv_heads, k.shape[0]
+            k, v = (t.float().repeat_interleave(group, dim=1) for t in (k, v))
+            scores = torch.einsum("rhd,jhd->hrj", q.float(), k) * self.head_dim ** -0.5
+            j, pos = torch.arange(length, device=x.device), torch.arange(length - rows, length, device=x.device).view(rows, 1)
+            hidden_keys = j > pos
+            if self.window:
+                hidden_keys = hidden_keys | ((j <= pos - self.window) & (j >= self.sinks))
+            out = torch.einsum("hrj,jhd->rhd", torch.softmax(scores.masked_fill(hidden_keys, float("-inf")), -1), v).to(self.dtype)
+        return hidden + (out.reshape(rows, -1) @ self.wo.t()).float()
+
+
 class DecodeRunner:
     """Embedding -> L x (mixer stand-in, hidden + MoE(hidden)) -> final norm -> head, one position at a time."""
 
     def __init__(self, layers: Sequence[MoEWeights], spec: MoESpec, *, moe_impl: str = "b200", vocab: int = 1024,
-                 dtype: torch.dtype = torch.bfloat16, seed: int = 0, device: str = "cuda"):
+                 dtype: torch.dtype = torch.bfloat16, seed: int = 0, device: str = "cuda", mixer: str = "identity",
+                 max_positions: int = 1024, cache_dtype: Optional[torch.dtype] = None, window: int = 0, sinks: int = 0):
+        if mixer not in ("identity", "attention"):
+            raise ValueError("mixer must be 'identity' or 'attention'")
         if moe_impl not in ("reference", "b200"):
             raise ValueError("moe_impl must be 'reference' or 'b200'")
         self.spec, self.moe_impl, self.dtype, self.device = spec, moe_impl, dtype, device
@@ -76,13 +120,27 @@ class DecodeRunner:
         if moe_impl == "b200":
             from .stack import ResidentMoELayers          # the CUDA library; raises if it is not built
             self.resident = ResidentMoELayers(self.layers, 1, hidden_dtype=dtype, top_k=spec.num_routed_experts)
+        self.mixers = None
+        if mixer == "attention":
+            # the real spec's attention layers have 16 query and 2 key/value heads of 256; small specs a small head
+            q_heads, kv_heads, head_dim = (16, 2, 256) if H >= 1024 else (4, 2, 8)
+            self.mixers = [AttentionMixer(H, q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, impl=moe_impl, dtype=dtype, seed=seed * 1000 + i, device=device,
+                                          max_positions=max_positions, cache_dtype=cache_dtype, window=window, sinks=sinks) for i in range(len(self.layers))]
         self.position = 0
+
+    def reset(self) -> None:
+        """Back to position 0: the mixers' caches are emptied."""
+        self.position = 0
+        for m in self.mixers or ():
+            m.cache.release(0)
 
     def step(self, token_id: int) -> torch.Tensor:
         """One position through all layers; returns the logits `[vocab]` (fp32)."""
         hidden = self.embedding[token_id].float().unsqueeze(0)
         for i, w in enumerate(self.layers):
-            # the attention / DeltaNet mixer of the layer would run here (out of this library's scope: identity)
+            # the sequence mixer of the layer: identity, or the attention sublayer
+            if self.mixers is not None:
+                hidden = self.mixers[i](hidden)
             if self.moe_impl == "reference":
                 hidden = hidden + torch_moe_update(hidden.to(self.dtype), w, self.spec.num_routed_experts)
             else:
@@ -124,6 +182,10 @@ def main(argv=None) -> None:
     ap.add_argument("--max-new-tokens", type=int, default=1)
     ap.add_argument("--moe-impl", default="b200", choices=["reference", "b200"])
     ap.add_argument("--seed", type=int, default=0)
+    ap.add_argument("--mixer", default="identity", choices=["identity", "attention"], help="sequence mixer of the layers")
+    ap.add_argument("--cache-dtype", default="same", choices=["same", "fp8"], help="key/value cache of the attention mixer")
+    ap.add_argument("--window", type=int, default=0, help="attention mixer: positions that a token sees (0: all)")
+    ap.add_argument("--sinks", type=int, default=0, help="attention mixer: first positions that stay visible outside of the window")
     args = ap.parse_args(argv)
     dtype = getattr(torch, args.dtype)
     spec = MoESpec() if args.spec == "real" else synthetic_qwen36_spec()
@@ -132,9 +194,11 @@ def main(argv=None) -> None:
     if not prompt:
         raise ValueError("prompt must contain at least one token")
     layers = build_layers(spec, n_layers, dtype, args.device, args.checkpoint)
-    runner = DecodeRunner(layers, spec, moe_impl=args.moe_impl, dtype=dtype, seed=args.seed, device=args.device)
+    runner = DecodeRunner(layers, spec, moe_impl=args.moe_impl, dtype=dtype, seed=args.seed, device=args.device, mixer=args.mixer,
+                          max_positions=len(prompt) + args.max_new_tokens + 1, cache_dtype=torch.float8_e4m3fn if args.cache_dtype == "fp8" else None,
+                          window=args.window, sinks=args.sinks)
     runner.step(prompt[0])                 # warm-up position (kernel attributes, tensor maps); not timed
-    runner.position = 0
+    runner.reset()
     if args.device == "cuda":
         torch.cuda.synchronize()
     start = time.perf_counter()
@@ -158,7 +222,10 @@ def main(argv=None) -> None:
     print(f"elapsed_ms_per_position: {elapsed * 1000 / max(positions, 1):.4f}")
     print(f"elapsed_ms_per_layer_position: {elapsed * 1000 / max(layer_positions, 1):.4f}")
     print(f"layer_positions_per_second: {layer_positions / elapsed:.4f}")
-    print("attention_impl: identity (out of scope)")
+    if args.mixer == "identity":
+        print("attention_impl: identity (out of scope)")
+    else:
+        print(f"attention_impl: {args.moe_impl} (paged cache, {args.cache_dtype}; seeded projections)")
     print("deltanet_impl: identity (out of scope)")
     print(f"moe_impl: {args.moe_impl}")
     print("serving_scope: MoE sublayers of the decode loop with resident weights; sequence mixers are stand-ins")
