@@ -49,9 +49,11 @@ struct TileShape {
     static_assert(2 * kMetaRing >= kSlots + 3, "a key tile's description outlives its softmax");
 };
 
+// A wait by parity only tells neighbouring phases apart.  s_full, p_full and o_done are waited for by warps that skip phases or come to
+// them late, so each has one barrier for even and one for odd tiles: when tile t is waited for, t - 2 is known to be over and t + 2 cannot be.
 struct TileBarriers {
     uint64_t full[12], empty[12], landed[12];
-    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done, o_empty;
+    uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], o_empty;
     uint64_t keys_full[kMetaRing];
     uint32_t tmem;
     int abort_flag;
@@ -228,8 +230,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         for (int i = 0; i < kSlots; ++i) mbar_init(&bar.landed[i], 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.q_full[i], 8);
-            mbar_init(&bar.q_empty[i], 1); mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 16); }
-        mbar_init(&bar.o_done, 1);
+            mbar_init(&bar.q_empty[i], 1);
+            mbar_init(&bar.o_done[i], 1); mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 16); }
         mbar_init(&bar.o_empty, 16);
         for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], TMA ? 1 : 4);
         bar.abort_flag = 0;
@@ -580,7 +582,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         const uint32_t a = tmem_s + (t & 1) * kTileKeys, v = v_low + slot * (S::kSlot >> 4);
 #pragma unroll
                         for (int i = 0; i < kTileKeys / 16; ++i) pair_mma_ts(tmem, a + i * 8, v + i * (2048 >> 4), o_idesc, !begins || i > 0);
-                        pair_commit(&bar.o_done);
+                        pair_commit(&bar.o_done[t & 1]);
                         pair_commit(&bar.empty[slot]);
                     }
                     __syncwarp();
@@ -710,7 +712,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 if (!begins) {
                     const float factor = alpha * unit_scale;
                     if (__any_sync(kFull, factor != 1.f)) {              // the same in both warps of a row
-                        mbar_wait_spin(&bar.o_done, (t - 1) & 1, abort_flag);
+                        mbar_wait_spin(&bar.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, abort_flag);
                         tc_fence_after_sync();
 #pragma unroll 1
                         for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 16) {
@@ -757,7 +759,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     sums[half * 128 + r] = l;
                     meet();
                     l = sums[r] + sums[128 + r];                         // in this order in both threads
-                    mbar_wait_spin(&bar.o_done, t & 1, abort_flag);
+                    mbar_wait_spin(&bar.o_done[t & 1], (t >> 1) & 1, abort_flag);
                     tc_fence_after_sync();
                     const int tokens = c.tokens(p), cols = tokens * p.group, first_row = c.first_row(p);
                     const bool whole = ends && began_k == 0;

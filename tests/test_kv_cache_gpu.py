@@ -466,3 +466,51 @@ def test_refusals():
     fk.paged_kv_append(key[:0], key[:0], dk, dv, table, lengths, starts)
     none = (table[:0], lengths[:0], starts[:1])
     assert (att(q, dk, dv, *none) == 0).all() and (fk.paged_kv_gather(dk, dv, *none, 4)[0] == 0).all()
+
+
+@pytest.mark.parametrize("new,lengths,window,sinks", [([2048], [2048], 0, 0), ([700], [9000], 0, 0), ([1500], [6000], 1024, 4), ([1, 900, 1, 1, 333, 2, 64, 1], [4100, 3000, 999, 2500, 3333, 1800, 64, 4000], 0, 0),
+                                                      ([1, 900, 1, 1, 333, 2, 64, 1], [4100, 3000, 999, 2500, 3333, 1800, 64, 4000], 500, 70)])
+@pytest.mark.parametrize("dim,kv_heads,group,dtype,cache,page", [(256, 2, 8, BF, BF, 16), (128, 8, 4, F16, F16, 32), (128, 2, 4, BF, BF, 12), (256, 1, 8, BF, E4, 16), (64, 4, 2, F16, E4, 64), (128, 1, 7, BF, BF, 8)])
+def test_long_chunks(new, lengths, window, sinks, dim, kv_heads, group, dtype, cache, page):
+    """Many key tiles per item and many items per worker: every ring, barrier phase and joined part goes round several times.
+    Against the definition in 64 bits on the GPU, and twice with the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(sum(lengths) + dim)
+    need = [-(-n // page) for n in lengths]
+    pages, starts = sum(need) + 2, [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    order = torch.randperm(pages, generator=g, device="cuda").to(torch.int32)
+    table = torch.full((len(new), max(need)), -1, dtype=torch.int32, device="cuda")
+    at = 0
+    for s, n in enumerate(need):
+        table[s, :n] = order[at:at + n]
+        at += n
+    shape = (pages, kv_heads, page, dim)
+    k, v = (torch.randn(shape, generator=g, device="cuda") * torch.exp2(4 * torch.rand(*shape[:3], 1, generator=g, device="cuda") - 2) for _ in range(2))
+    scales = {}
+    if cache == E4:
+        for name, x in (("key_scale", k), ("value_scale", v)):
+            scales[name] = x.abs().amax(-1) / 448
+        k, v = (x / scales[n].unsqueeze(-1) for n, x in (("key_scale", k), ("value_scale", v)))
+    k, v = k.to(cache), v.to(cache)
+    q = torch.randn(starts[-1], kv_heads * group, dim, generator=g, device="cuda").to(dtype)
+    args = (q, k, v, table, torch.tensor(lengths, dtype=torch.int32, device="cuda"), torch.tensor(starts, dtype=torch.int32, device="cuda"))
+    got = fk.paged_attention(*args, window=window, sinks=sinks, max_query=max(new), **scales)
+    for _ in range(3):
+        assert torch.equal(got, fk.paged_attention(*args, window=window, sinks=sinks, max_query=max(new), **scales))
+    values = []
+    for x, name in ((k, "key_scale"), (v, "value_scale")):
+        x = x.float()
+        values.append(x * scales[name].unsqueeze(-1) if scales else x)
+    for s, (n, length) in enumerate(zip(new, lengths)):
+        kk, vv = (x[table[s, :need[s]].long()].transpose(1, 2).reshape(-1, kv_heads, dim)[:length].double() for x in values)
+        pos, j = torch.arange(length - n, length, device="cuda").view(n, 1), torch.arange(length, device="cuda")
+        seen = (j <= pos) & ((j > pos - window) | (j < sinks)) if window else j <= pos
+        for a in range(kv_heads * group):
+            x, h = q[starts[s]:starts[s + 1], a].double(), a // group
+            w = torch.softmax((x @ kk[:, h].T * dim ** -0.5).masked_fill(~seen, float("-inf")), -1)
+            out, mag = w @ vv[:, h], w @ vv[:, h].abs()
+            size = (x.abs() @ kk[:, h].abs().T * dim ** -0.5).amax(-1)
+            err = (got[starts[s]:starts[s + 1], a].double() - out).abs()
+            tol = O.bound(dtype, out, mag, size, seen.sum(-1).double(), dim)
+            assert (err <= tol).all(), f"sequence {s} head {a}: {(err / tol).max():.2f} times the bound"
