@@ -36,7 +36,7 @@ struct RowSums {
     float acc[FK_MAX_HEAD_DIM / 32];
 };
 
-// One warp, one query row (q(d) is element d times scale * log2 e, q(d >= head_dim) anything finite): groups first, first + step, ..
+// A row that is computed again (row_again): one warp, one query row (q(d) is element d times scale * log2 e, q(d >= head_dim) anything finite): groups first, first + step, ..
 // of 32 of the visible keys.  One lane computes one key's score (no reduction per key); then the value rows are added one at
 // a time, a lane per column.  Keys that are masked never enter any sum, whatever their rows hold.
 template <typename TC, bool WIDE, typename Q>
