@@ -24,7 +24,7 @@ __host__ __device__ inline int any_smem(int dim, int heads) { return (2 * kAnyKe
 // axis).  32 keys and values at a time are brought into shared memory as fp32 by coalesced loads, once for all heads; then a warp per
 // head takes one key per lane for the scores (no reduction per key) and one column per lane for the values.  What bounds it is the
 // shared-memory reads of the products (one per four multiply-adds in the scores, one per multiply-add in the values); a row per warp
-// straight from L2, without the tile, took 55 us where this takes 14 (61 tokens at up to 700, 6 heads of 80 in fp32).
+// straight from L2, without the tile, took 55 us where this takes 24 (61 tokens at up to 700, 6 heads of 80 in fp32).
 // NC: groups of 32 columns, at least head_dim / 32.
 template <typename T, typename TC, bool WIDE, int NC>
 __global__ void __launch_bounds__(32 * kAnyWarps) attention_any_kernel(const __grid_constant__ AttnParams p) {
@@ -301,7 +301,7 @@ int fk_paged_attention(const fk_attention_call* a, void* stream) {
     AttnParams p = attn_params(*a);
     const Path path = path_of(*a, p);
     const size_t need = workspace_need(*a, p, path);
-    if (need > 0 && (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 15))) return FK_ERR_WORKSPACE;
+    if (need > 0 && (!a->workspace || a->workspace_bytes < need || (reinterpret_cast<uintptr_t>(a->workspace) & 31))) return FK_ERR_WORKSPACE;
     cudaStream_t s = (cudaStream_t)stream;
     if (path == Path::few) return attention_few(p, a->dtype, a->starts == nullptr ? 1 : a->max_query, nullptr, s);
     if (path == Path::tile) return attention_tile(p, a->dtype, nullptr, s);

@@ -1,6 +1,8 @@
 // Paged attention: what its kernels share.
 #pragma once
 
+#include <atomic>
+
 #include "kv_cache.cuh"
 
 namespace fk {
@@ -112,6 +114,20 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const Q& q, int se
             }
         }
     }
+}
+
+// A kernel's shared-memory limit, set once per device (a call of the runtime each time costs a twentieth of a decode call's host time).
+// `done` belongs to the kernel.
+template <typename K>
+inline cudaError_t allow_smem(K* kern, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 
 // Kernel for few query rows per key/value head (attention_few.cu).  need != null: only the workspace's size.

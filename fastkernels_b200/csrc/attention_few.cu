@@ -216,7 +216,13 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
         }
         __syncwarp();
     }
-    if (threadIdx.x == 0) *abort_flag = 0;
+    if (threadIdx.x == 0) {
+        *abort_flag = 0;
+        if (TMA) {
+            prefetch_tensormap(&key_map);
+            prefetch_tensormap(&value_map);
+        }
+    }
     pdl_trigger();
     pdl_wait();
 
@@ -751,8 +757,9 @@ static int few(AttnParams p, int max_warps, size_t* need, cudaStream_t stream) {
         return FK_OK;
     }
     CUtensorMap key_map{}, value_map{};
-    auto launch = [&](auto kern) -> int {
-        FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), "attention (few) attr");
+    static std::atomic<uint64_t> allowed[2];
+    auto launch = [&](auto kern, int tma) -> int {
+        FK_CUDA_OK(allow_smem(kern, S::kSmem, allowed[tma]), "attention (few) attr");
         FK_CUDA_OK(launch_pdl(kern, dim3(blocks), dim3(32 * S::kWarps), (size_t)S::kSmem, stream, p, key_map, value_map), "attention (few) launch");
         FK_LAUNCH_OK("attention (few) launch");
         return FK_OK;
@@ -763,9 +770,9 @@ static int few(AttnParams p, int max_warps, size_t* need, cudaStream_t stream) {
         auto scales_ok = [&](const float* s, const int64_t* stride) { return stride[2] == 1 && groups_aligned(s, stride, 2, 4, 16); };
         if (p.c.page_size % kFewKeys == 0 && (!S::kCodes || (scales_ok(p.c.key_scale, p.c.key_scale_stride) && scales_ok(p.c.value_scale, p.c.value_scale_stride))) &&
             group_map(p.c.key, p.c, p.c.key_stride, &key_map) && group_map(p.c.value, p.c, p.c.value_stride, &value_map))
-            st = launch(attention_few_kernel<D, NT, T, TC, true>);
+            st = launch(attention_few_kernel<D, NT, T, TC, true>, 1);
     }
-    if (st < 0) st = launch(attention_few_kernel<D, NT, T, TC, false>);
+    if (st < 0) st = launch(attention_few_kernel<D, NT, T, TC, false>, 0);
     if (st != FK_OK) return st;
     const int cols = (int)min((int64_t)S::kCols, (int64_t)p.tile_tokens * p.group);
     FK_CUDA_OK(launch_pdl(attention_few_join_kernel<D, NT, T, TC>, dim3((unsigned)blocks, cols), dim3(32 * kJoinWarps), 0, stream, p), "attention (few) join launch");

@@ -38,7 +38,9 @@ struct TileShape {
     static constexpr bool kCodes = sizeof(TC) == 1;
     static constexpr int kQuery = 128 * D * 2;                       // bytes of a block's query rows
     static constexpr int kSlot = 64 * D * 2;                         // 64 keys, or 128 values' half rows
-    static constexpr int kQueries = D == 256 ? 1 : 2;                // buffers of query rows: where they fit, the next item's come early
+    // Buffers of query rows.  With one, an item's first scores wait for the last products of the item before (its keys are then loaded
+    // behind the other's last values); with two, items follow each other like the tiles of one
+    static constexpr int kQueries = D == 256 ? 1 : 2;
     static constexpr int kSlots = D == 256 ? (kCodes ? 4 : 5) : (kCodes ? 8 : 9);
     static constexpr int kMeta = kMetaRing * (kCodes ? 2 * kTileKeys * 4 + 32 : 16);
     static constexpr int kExchange = 2 * 2 * 128 * 4;                // between the two threads of a row
@@ -164,6 +166,9 @@ __device__ __forceinline__ uint32_t tile_pack(float lo, float hi, __half) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ void store32(void* p, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 __device__ __forceinline__ uint4 codes8_to_half(uint2 c) {
     uint4 r;
     codes4_to_half(c.x, r.x, r.y);
@@ -236,6 +241,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
         for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], TMA ? 1 : 4);
         bar.abort_flag = 0;
         mbar_init_fence();
+        if (TMA) {
+            prefetch_tensormap(&key_map);
+            prefetch_tensormap(&value_map);
+        }
     }
     if (warp == kMmaWarp) pair_tmem_alloc(&bar.tmem);
     pdl_trigger();
@@ -429,9 +438,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     look_unit();
                     for (int t = 0; t < tiles; ++t) {
                         constexpr int groups = D / 64;
-                        if (first && t > 0) tma_values();
+                        if (S::kQueries == 1 && first && t > 0) tma_values();
                         const int slot = x % kSlots, meta = t % kMetaRing, head = c.head;
-                        const bool edge = edge_tile(p, c), ends = c.k + 1 >= c.span.count, values_now = t > 0 && !first;
+                        const bool edge = edge_tile(p, c), ends = c.k + 1 >= c.span.count, values_now = t > 0 && !(S::kQueries == 1 && first);
                         wait_slot();                 // and with it for the last reader of this description (static_assert above)
                         const uint32_t full = in_first_block(&bar.full[slot]);
                         const unsigned there = __ballot_sync(kFull, page != -1) & (0xffffffffu >> (32 - units));
@@ -464,7 +473,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             if (!TMA) look();
             for (int t = TMA ? tiles : 0; t < tiles; ++t) {
                 if (first) {
-                    if (t > 0) load(true, value_offset);
+                    if (S::kQueries == 1 && t > 0) load(true, value_offset);
                     load_query(segment);
                 }
                 // this tile's rows: their offsets, which of them are there, their scales
@@ -502,7 +511,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     page = -1;
                 }
                 load(false, key_offset);
-                if (t > 0 && !first) load(true, value_offset);
+                if (t > 0 && !(S::kQueries == 1 && first)) load(true, value_offset);
                 value_offset = next_value;
                 first = ends;
                 if (ends) ++segment;
@@ -521,8 +530,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 for (int t = 0; t < tiles; ++t) {
                     const bool ends = c.k + 1 >= c.span.count;
                     if (edge_tile(p, c)) {
-                        // order of the loads: K(0), then [K(t + 1), V(t)] inside an item and [V(t), K(t + 1)] where t ends one
-                        const int slot = (ends || t + 1 == tiles ? 2 * t + 1 : 2 * t + 2) % kSlots, key0 = c.key0(), lo = window_start(p, c.pos0);
+                        // order of the loads: K(0), then [K(t + 1), V(t)], but [V(t), K(t + 1)] where t ends an item and there is one query buffer
+                        const int slot = ((S::kQueries == 1 && ends) || t + 1 == tiles ? 2 * t + 1 : 2 * t + 2) % kSlots, key0 = c.key0(), lo = window_start(p, c.pos0);
                         const uint32_t base = ring + slot * S::kSlot;
                         mbar_wait_spin(&bar.landed[slot], (landed >> slot) & 1, abort_flag);
                         landed ^= 1u << slot;
@@ -592,12 +601,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 for (int t = 0; t < tiles; ++t) {
                     const bool ends = c.k + 1 >= c.span.count;
                     if (first) {
-                        if (t > 0) values(t - 1, last_began);
+                        if (S::kQueries == 1 && t > 0) values(t - 1, last_began);
                         mbar_wait_spin(&bar.q_full[segment % S::kQueries], (segment / S::kQueries) & 1, abort_flag);
                         ++segment;
                     }
                     scores(t, ends || t + 1 == tiles, (segment - 1) % S::kQueries);
-                    if (t > 0 && !first) values(t - 1, last_began);
+                    if (t > 0 && !(S::kQueries == 1 && first)) values(t - 1, last_began);
                     last_began = first;
                     first = ends;
                     if (t + 1 < tiles) {
@@ -770,7 +779,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     const float inv = l == 0.f ? 0.f : scale_out / l;
                     const bool failed = *abort_flag != 0;
                     bool odd = false;
-                    const bool wide = (dim & 7) == 0 && ((p.os[0] | p.os[1]) & 7) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+                    const bool wide = (dim & 15) == 0 && ((p.os[0] | p.os[1]) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
 #pragma unroll 1
                     for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 16) {
                         float o[16];
@@ -783,17 +792,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                                     if (i + e < dim) odd |= !(fabsf(o[e]) < INFINITY);
                                     if (failed) o[e] = NAN;
                                 }
+                                // a row per thread: 32 bytes at a time fill whole sectors
+                                if (wide) {
+                                    uint32_t w[8];
 #pragma unroll
-                                for (int e = 0; e < 16; e += 8)
-                                    if (i + e < dim) {
-                                        const float v[8] = {o[e], o[e + 1], o[e + 2], o[e + 3], o[e + 4], o[e + 5], o[e + 6], o[e + 7]};
-                                        if (wide) store8<true>(out + i + e, 8, v); else store8<false>(out + i + e, dim - i - e, v);
-                                    }
+                                    for (int e = 0; e < 8; ++e) w[e] = tile_pack(o[2 * e], o[2 * e + 1], T{});
+                                    store32(out + i, w);
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < 16; ++e)
+                                        if (i + e < dim) store_elem(out + i + e, o[e]);
+                                }
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 16; e += 4)
-                                    *reinterpret_cast<float4*>(part + 2 * kTileRows + (int64_t)n * D + i + e) =
-                                        failed ? make_float4(NAN, NAN, NAN, NAN) : make_float4(o[e] * scale_out, o[e + 1] * scale_out, o[e + 2] * scale_out, o[e + 3] * scale_out);
+                                for (int e = 0; e < 16; ++e) o[e] = failed ? NAN : o[e] * scale_out;
+                                store32(part + 2 * kTileRows + (int64_t)n * D + i, reinterpret_cast<const uint32_t*>(o));
+                                store32(part + 2 * kTileRows + (int64_t)n * D + i + 8, reinterpret_cast<const uint32_t*>(o + 8));
                             }
                         }
                     }
@@ -933,7 +947,8 @@ template <int D, typename T, typename TC, bool TMA>
 static int launch_tile(const AttnParams& p, const CUtensorMap& key_map, const CUtensorMap& value_map, int unit, cudaStream_t stream) {
     using S = TileShape<D, TC>;
     auto kern = attention_tile_kernel<D, T, TC, TMA>;
-    FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem), "attention (tile) attr");
+    static std::atomic<uint64_t> allowed;
+    FK_CUDA_OK(allow_smem(kern, S::kSmem, allowed), "attention (tile) attr");
     cudaLaunchConfig_t cfg{};
     const int pairs = sm_count() / 2;
     cfg.gridDim = dim3(2 * pairs);

@@ -262,7 +262,7 @@ def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: An
     lib = _lib.load()
     with _On(device):
         if fresh:
-            out = torch.empty((rows, q_heads, dim), device=device, dtype=query.dtype)
+            out = torch.empty_like(query, memory_format=torch.contiguous_format)
         else:
             if _check_rows(out, "out", rows, q_heads, dim, key_cache) != code:
                 raise ValueError("out must have the query's dtype")

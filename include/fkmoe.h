@@ -299,7 +299,7 @@ typedef struct fk_attention_call {
     int32_t zero_rest;                 /* also write zeros to the rows behind the last sequence (otherwise they are left alone) */
     uint32_t flags;                    /* FK_FLAG_FORCE_GENERIC: the shape-agnostic kernel */
     int32_t reserved;
-    void* workspace;                   /* fk_paged_attention_workspace_bytes(); needs no clearing, not shared by calls that overlap */
+    void* workspace;                   /* fk_paged_attention_workspace_bytes(), 32-byte aligned; needs no clearing, not shared by calls that overlap */
     size_t workspace_bytes;
 } fk_attention_call;
 
