@@ -3,21 +3,25 @@
 // A tile is 256 query rows (tokens x heads of the group) of one (sequence, key/value head) on a pair of SMs, 128 rows on each;
 // it walks over its keys 128 at a time:
 //   S[256, 128] = Q K^T          operands in shared memory, each SM holding 64 of the 128 keys
-//   P = 2^(S - m)                one thread per row: no exchange between threads, statistics in registers
+//   P = 2^(S - m)                two threads per row, 64 columns each, that exchange their maxima
 //   O[256, dim] += P V           P from tensor memory, where it replaces S; each SM holds half of the values' columns
 // The pair shares every key and value row, so an SM fetches half of them: at 256 dimensions one SM alone would need 64 bytes
 // of L2 per clock for 128 rows, and the whole chip gets 41 (11.8 TB/s measured); a pair needs 32.  It is also what lets the ring
 // hold 128-key tiles at 256 dimensions: 64 KB of queries + five slots of 32 KB.  Tensor memory: O (dim columns) and two S buffers
 // (128 columns each), so the products of the next tile run while this tile's softmax is taken.
 //
-// Warps of a block: 0..3 softmax (a row per thread, its sums, and the scaling of O), 4..7 producers (rows gathered through the page
-// table with cp.async, written in the 128-byte-swizzled layout; codes are converted to fp16 on the way), 8 issues the products
-// (in the pair's first block).  m is only raised when a row's maximum grows by more than 2^kLazy, which spares nearly all
-// passes over O.  Weights are rounded to the type of the operands (fp16 after a factor 2^7, which with 2^kLazy stays below
-// 2^15); sums are fp32.
+// Warps of a block: 0..7 softmax (and the scaling and storing of O), 8..11 producers (tensor copies out of the pages; where pages or
+// strides do not allow them, and for codes, which become fp16 on the way, rows gathered by the threads), 12 issues the products (in
+// the pair's first block), 13 zeroes value rows that nobody may see.  m is only raised when a row's maximum grows by more than
+// 2^kLazy, which spares nearly all passes over O.  Weights are rounded to the type of the operands (fp16 after a factor 2^7, which with
+// 2^kLazy stays below 2^15); sums are fp32.
 //
 // Key tiles of all tiles are dealt to the pairs in equal contiguous runs as in the few-row kernel; a run's first and last tile
 // may be partial, and attention_tile_join_kernel joins those in key order.
+//
+// What bounds it (256 dimensions, 2048 tokens at 16384): a tile is 2050 clocks of products and 1030 of exponentials; the products of tile
+// t + 1 need the S buffer that tile t - 1's weights leave, so a round is products + barrier + softmax of half a round, some 3100 clocks:
+// 475 us, 1085 TFLOP/s, 0.66 of the measured cuBLAS rate.
 
 #include <cfloat>
 #include <type_traits>

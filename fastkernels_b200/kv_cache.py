@@ -332,6 +332,9 @@ class PagedKVCache:
         new = [1] * self.seqs if new is None else [int(n) for n in new]
         if len(new) != self.seqs or min(new) < 0 or sum(new) != key.shape[0]:
             raise ValueError("new must name each sequence's number of rows, with key's rows as their sum")
+        row = (self.key.shape[1], self.key.shape[3])
+        if key.shape[1:] != row or value.shape != key.shape:
+            raise ValueError(f"key and value must have shape [rows, {row[0]}, {row[1]}]")
         self._grow(new)
         starts = [0]
         for n in new:

@@ -306,7 +306,8 @@ typedef struct fk_attention_call {
 /* Write new tokens into the cache / read the last tokens of each sequence back. */
 int fk_kv_append(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
 int fk_kv_gather(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
-/* out = softmax(scale * query . key) value over the positions that each row sees; a row that sees none gives zeros. */
+/* out = softmax(scale * query . key) value over the positions that each row sees; a row that sees none gives zeros.
+ * Every wait inside the kernels is bounded (about a second); one that runs out makes the rows that depended on it NaN. */
 size_t fk_paged_attention_workspace_bytes(const fk_attention_call* call);
 int fk_paged_attention(const fk_attention_call* call, void* stream);
 
