@@ -112,7 +112,7 @@ struct FewShape {
     // behind the ring, per slot: first key and row mask, scales of its rows, barrier
     static constexpr int kSide = 8 + (kCodes ? 4 * kKeys : 0) + 8;
     static constexpr int kRing = kWarps * kSlots * kSlot;
-    static constexpr int kSmem = kRing + kWarps * kSlots * kSide + kWarps * 2 * (int)sizeof(PartHead) + kWarps * 16 + 16;
+    static constexpr int kSmem = kRing + kWarps * kSlots * kSide + kWarps * 2 * (int)sizeof(PartHead) + kWarps * 16 + 16 + kWarps * 2 * 2 * kCols * 4 + kCols * 4;
     static_assert(kSlots >= 3, "a slot being read and two on their way");
     static_assert(kSmem <= 227 * 1024, "shared memory of a block");
 };
@@ -207,6 +207,8 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     PartHead* warp_heads = reinterpret_cast<PartHead*>(side + S::kWarps * kSlots * S::kSide);
     int64_t* scratch = reinterpret_cast<int64_t*>(warp_heads + S::kWarps * 2);
     int* abort_flag = reinterpret_cast<int*>(scratch + 2 * S::kWarps);
+    int* odd_column = abort_flag + 4;
+    float* stats = reinterpret_cast<float*>(odd_column + S::kCols);         // [2 warps' parts][m, l per column]
     int64_t* upto = reinterpret_cast<int64_t*>(smem);              // over the ring, before its first copy
     const int room = S::kRing / 8;
     if (TMA) {
@@ -625,7 +627,11 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 for (int c = 0; c < 2; ++c) {
                     const int n = nt * 8 + 2 * t + c;
                     if (n >= cols) continue;
-                    if (g == 0) { part[n] = m[nt][c]; part[S::kCols + n] = l[nt][c]; }
+                    if (g == 0) {
+                        float* st = stats + (warp * 2 + which) * 2 * S::kCols;
+                        st[n] = m[nt][c];
+                        st[S::kCols + n] = l[nt][c];
+                    }
 #pragma unroll
                     for (int i = 0; i < kMT; ++i)
 #pragma unroll
@@ -638,40 +644,69 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
         if (at < run1) cur.next_item(p);
     }
 
-    // ---- the parts of the block's warps: one that does not begin its item continues the one before it
+    // ---- the parts of the block's warps: one that does not begin its item continues the one before it.  All threads take four
+    // dimensions of a column each, so that a part costs one round of loads
+    if (threadIdx.x < S::kCols) odd_column[threadIdx.x] = 0;
     __syncthreads();
-    int group = -1, task = 0;
+    int group = -1;
     for (int e = 0; e < 2 * S::kWarps;) {
         if (warp_heads[e].begins < 0) { ++e; continue; }
         ++group;
-        int entries[2] = {e, e};                 // first and last part
-        int count = 1;
+        const int first = e;
+        int last = e, count = 1;
         for (int f = e + 1; f < 2 * S::kWarps; ++f) {
             if (warp_heads[f].begins < 0) continue;
             if (warp_heads[f].begins == 1) break;
-            entries[1] = f;
+            last = f;
             ++count;
         }
-        e = entries[1] + 1;
-        const PartHead h = warp_heads[entries[0]];
-        const bool begins = h.begins == 1, ends = warp_heads[entries[1]].ends == 1;
-        // a first part may be either of its warp's two, all others are the first of theirs
-        auto part = [&](int i) { return warp_parts + (i == 0 ? entries[0] : (entries[0] / 2 + i) * 2) * (int64_t)S::kPart; };
+        e = last + 1;
+        const PartHead h = warp_heads[first];
+        const bool begins = h.begins == 1, ends = warp_heads[last].ends == 1;
+        // the first part may be either of its warp's two, all others are the first of theirs
+        auto entry = [&](int i) { return i == 0 ? first : (first / 2 + i) * 2; };
         const int cols = h.tokens * p.group;
-        for (int n = 0; n < cols; ++n, ++task) {
-            if (task % S::kWarps != warp) continue;
-            Joined<D> j;
-            j.template join<S::kCols>(part, 0, count, 1, n);
-            if (begins && ends) {
-                j.template finish<T, TC>(p, h, n);
-            } else {
-                float* to = block_parts + (group == 0 ? 0 : 1) * S::kPart;
-                if (lane == 0) { to[n] = j.m; to[S::kCols + n] = j.l; }
-#pragma unroll
-                for (int c = 0; c < Joined<D>::kParts; ++c)
-#pragma unroll
-                    for (int x = 0; x < Joined<D>::kVec; ++x) to[2 * S::kCols + n * D + Joined<D>::dim(lane, c, x)] = j.acc[c][x];
+        float* to = block_parts + (group == 0 ? 0 : 1) * S::kPart;
+        for (int i = threadIdx.x; i < cols * (D / 4); i += 32 * S::kWarps) {
+            const int n = i / (D / 4), d = (i - n * (D / 4)) * 4;
+            float m = -INFINITY, l = 0.f;
+            for (int k = 0; k < count; ++k) m = fmaxf(m, stats[entry(k) * 2 * S::kCols + n]);
+            const float base = m == -INFINITY ? 0.f : m;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+            for (int k = 0; k < count; ++k) {
+                const float* st = stats + entry(k) * 2 * S::kCols + n;
+                const float4 v = *reinterpret_cast<const float4*>(warp_parts + entry(k) * (int64_t)S::kPart + 2 * S::kCols + n * D + d);
+                const float weight = exp2_fast(st[0] - base);
+                l = fmaf(weight, st[S::kCols], l);
+                acc.x = fmaf(weight, v.x, acc.x); acc.y = fmaf(weight, v.y, acc.y); acc.z = fmaf(weight, v.z, acc.z); acc.w = fmaf(weight, v.w, acc.w);
             }
+            if (begins && ends) {
+                const int tok = n / p.group;
+                T* out = reinterpret_cast<T*>(p.out) + (int64_t)(h.first_row + tok) * p.os[0] + (int64_t)(h.head * p.group + n - tok * p.group) * p.os[1] + d;
+                const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+                bool odd = false;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float r = l == 0.f ? 0.f : v[x] / l;
+                    odd |= !(fabsf(r) < INFINITY);
+                    store_elem(out + x, r);
+                }
+                if (odd && h.tokens > 1) odd_column[n] = 1;
+            } else {
+                if (d == 0) { to[n] = m; to[S::kCols + n] = l; }
+                *reinterpret_cast<float4*>(to + 2 * S::kCols + n * D + d) = acc;
+            }
+        }
+        if (begins && ends && h.tokens > 1) {
+            __syncthreads();                     // the rows are written, then those that are not finite once more
+            for (int n = warp; n < cols; n += S::kWarps) {
+                const bool odd = odd_column[n] != 0;
+                __syncwarp();
+                if (odd) row_again<T, TC>(p, h.seq, h.first_row + n / p.group, h.pos0 + n / p.group, h.head * p.group + n % p.group);
+                if (lane == 0) odd_column[n] = 0;
+            }
+            __syncthreads();
         }
         if (!(begins && ends) && threadIdx.x == 0) {
             PartHead b = h;
