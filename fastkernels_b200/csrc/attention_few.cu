@@ -84,10 +84,10 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return r;
 }
 
-__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int row, int group, int head, int page, uint64_t* bar) {
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int x, int row, int group, int head, int page, uint64_t* bar, uint64_t policy) {
     asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(group), "r"(head), "r"(page)
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(row), "r"(group), "r"(head), "r"(page), "l"(policy)
         : "memory");
 }
 
@@ -246,6 +246,8 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     __syncthreads();                             // the plan's memory is the ring's from here on
     ahead = cur;
 
+    const uint64_t policy = l2_evict_first_policy();     // a row of the cache is read once per call
+
     // ---- issue side: keys and values of one group after the other into the ring
     int64_t left = run1 - run0;
     int page = -1, in_page = 0;                  // of this lane's row of the next group; tensor copies: of the first of its 16 rows
@@ -276,7 +278,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 const unsigned there = __ballot_sync(kFull, page >= 0);
                 if (lane == 0) mbar_expect_tx(bar, S::kSlot + (kCodes ? 64 * ((there & 1) + (S::kTiles > 1 ? (there >> 16) & 1 : 0)) : 0));
                 if ((lane & 15) == 0 && lane < S::kKeys) {
-                    tma_load_5d(base + lane * 128, values ? &value_map : &key_map, 0, in_page, 0, ahead.head, page < 0 ? p.c.pages : page, bar);
+                    tma_load_5d(base + lane * 128, values ? &value_map : &key_map, 0, in_page, 0, ahead.head, page < 0 ? p.c.pages : page, bar, policy);
                     if (kCodes && page >= 0)
                         bulk_load(scales + issue_slot * S::kKeys + lane,
                                   (values ? p.c.value_scale : p.c.key_scale) + row_offset(values ? p.c.value_scale_stride : p.c.key_scale_stride, page, ahead.head, in_page), 64, bar);
