@@ -235,8 +235,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kSlots; ++i) { mbar_init(&bar.full[i], TMA ? 2 : 8); mbar_init(&bar.empty[i], 1); }
-        for (int i = 0; i < kSlots; ++i) mbar_init(&bar.landed[i], 1);
+        for (int i = 0; i < kSlots; ++i) { mbar_init(&bar.full[i], 2); mbar_init(&bar.empty[i], 1); }
+        for (int i = 0; i < kSlots; ++i) mbar_init(&bar.landed[i], TMA ? 1 : 4);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&bar.q_full[i], 8);
             mbar_init(&bar.q_empty[i], 1);
@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 fence_async_proxy();
                 __syncwarp();
                 for (; arrived < upto; ++arrived)
-                    if (lane == 0) arrive_first_release(&bar.full[arrived % kSlots]);
+                    if (lane == 0) mbar_arrive(&bar.landed[arrived % kSlots]);
             };
             auto load_query = [&](int segment) {     // 32 of the block's 128 rows per warp
                 if (!kCodes && !TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -358,13 +358,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const int r = (i >> 4) * 64 + w * 16 + (i & 15);
                 return base + (chunk >> 3) * (128 * 128) + r * 128 + (((chunk & 7) ^ (r & 7)) << 4);
             };
-            auto load = [&](bool values, int64_t offset) {       // offset: bytes of this lane's row, < 0: no such row
+            // threads' copies of 16-bit rows; offset: bytes of this lane's row, < 0: no such row
+            auto load = [&](bool values, int64_t offset) {
                 const int slot = x % kSlots;
                 if (!mbar_try_wait(&bar.empty[slot], ((x / kSlots) & 1) ^ 1)) {
-                    if (!kCodes) {                               // ahead of the products: announce what is on its way first
-                        asm volatile("cp.async.wait_group 0;" ::: "memory");
-                        announce(x);
-                    }
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");      // ahead of the products: announce what is on its way first
+                    announce(x);
                     mbar_wait_spin(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
                 }
                 const uint32_t base = ring + slot * S::kSlot;
@@ -375,12 +374,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         const int i = i0 + lane / kKeyChunks, chunk = lane % kKeyChunks;
                         const int64_t off = __shfl_sync(kFull, offset, rank * 16 + i);
                         const bool there = off >= 0 && chunk * 8 < dim;
-                        if (kCodes) {
-                            const uint2 v = there ? *reinterpret_cast<const uint2*>(from + off + chunk * 8) : make_uint2(0, 0);
-                            sts16(key_addr(base, i, chunk), codes8_to_half(v));
-                        } else {
-                            tile_copy16(key_addr(base, i, chunk), there ? from + off + chunk * 16 : from, there ? 16 : 0);
-                        }
+                        tile_copy16(key_addr(base, i, chunk), there ? from + off + chunk * 16 : from, there ? 16 : 0);
                     }
                 } else {
 #pragma unroll
@@ -388,24 +382,41 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         const int i = i0 + lane / kValueChunks, chunk = lane % kValueChunks, at = rank * kValueChunks + chunk;
                         const int64_t off = __shfl_sync(kFull, offset, i);
                         const bool there = off >= 0 && at * 8 < dim;
-                        if (kCodes) {
-                            const uint2 v = there ? *reinterpret_cast<const uint2*>(from + off + at * 8) : make_uint2(0, 0);
-                            sts16(value_addr(base, i, chunk), codes8_to_half(v));
-                        } else {
-                            tile_copy16(value_addr(base, i, chunk), there ? from + off + at * 16 : from, there ? 16 : 0);
-                        }
+                        tile_copy16(value_addr(base, i, chunk), there ? from + off + at * 16 : from, there ? 16 : 0);
                     }
                 }
                 ++x;
-                if (kCodes) {
-                    announce(x);
-                } else {
-                    asm volatile("cp.async.commit_group;" ::: "memory");
-                    if (x > kLag) {
-                        asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
-                        announce(x - kLag);
-                    }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                if (x > kLag) {
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kLag) : "memory");
+                    announce(x - kLag);
                 }
+            };
+            // codes: all of a thread's reads of a slot at once, converted and stored when the slot is free
+            constexpr int kRaw = 16 / kKeyAtOnce;                // pieces of eight codes per thread, of keys as of values
+            static_assert(kRaw == 32 / kValueAtOnce, "half of the keys, half of the values' columns");
+            auto fetch = [&](bool values, int64_t offset, uint2 (&raw)[kRaw]) {
+                const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
+#pragma unroll
+                for (int r = 0; r < kRaw; ++r) {
+                    const int i = values ? r * kValueAtOnce + lane / kValueChunks : rank * 16 + r * kKeyAtOnce + lane / kKeyChunks;
+                    const int chunk = values ? rank * kValueChunks + lane % kValueChunks : lane % kKeyChunks;
+                    const int64_t off = __shfl_sync(kFull, offset, i);
+                    raw[r] = off >= 0 && chunk * 8 < dim ? *reinterpret_cast<const uint2*>(from + off + chunk * 8) : make_uint2(0, 0);
+                }
+            };
+            auto put = [&](bool values, int64_t offset) {
+                uint2 raw[kRaw];
+                fetch(values, offset, raw);
+                const int slot = x % kSlots;
+                mbar_wait_spin(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
+                const uint32_t base = ring + slot * S::kSlot;
+#pragma unroll
+                for (int r = 0; r < kRaw; ++r)
+                    sts16(values ? value_addr(base, r * kValueAtOnce + lane / kValueChunks, lane % kValueChunks) : key_addr(base, r * kKeyAtOnce + lane / kKeyChunks, lane % kKeyChunks),
+                          codes8_to_half(raw[r]));
+                ++x;
+                announce(x);
             };
             int segment = 0;
             bool first = true;
@@ -473,57 +484,68 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                     tma_values();
             }
-            int64_t value_offset = -1;
-            if (!TMA) look();
-            for (int t = TMA ? tiles : 0; t < tiles; ++t) {
-                if (first) {
-                    if (S::kQueries == 1 && t > 0) load(true, value_offset);
-                    load_query(segment);
-                }
-                // this tile's rows: their offsets, which of them are there, their scales
-                const int64_t key_offset = page < 0 ? -1 : row_offset(p.c.key_stride, page, c.head, in_page) * (int64_t)sizeof(TC);
-                const int64_t next_value = page < 0 ? -1 : row_offset(p.c.value_stride, page, c.head, in_page) * (int64_t)sizeof(TC);
-                const unsigned rows = __ballot_sync(kFull, page >= 0);
-                const int meta = t % kMetaRing;
-                // a description is written anew only when its last reader has passed: the key slot of this tile, waited for below,
-                // was freed later than that (static_assert above); so wait for the slot first
-                if (!mbar_try_wait(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1)) {
-                    if (!kCodes) {
-                        asm volatile("cp.async.wait_group 0;" ::: "memory");
-                        announce(x);
-                    }
-                    mbar_wait_spin(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
-                }
-                if (lane == 0) key_mask[meta * 4 + w] = rows;
-                if (kCodes) {
-                    const float ks = page < 0 ? 0.f : p.c.key_scale[row_offset(p.c.key_scale_stride, page, c.head, in_page)];
-                    const float vs = page < 0 ? 0.f : p.c.value_scale[row_offset(p.c.value_scale_stride, page, c.head, in_page)];
-                    const int n = (lane >> 4) * 64 + w * 16 + (lane & 15);
-                    key_scale[meta * kTileKeys + n] = ks;
-                    value_scale[meta * kTileKeys + n] = vs;
-                    const float top = warp_max(fabsf(vs));
-                    if (lane == 0) value_top[meta * 4 + w] = top;
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bar.keys_full[meta]);
-                // on to the next tile before the copies: its page numbers arrive meanwhile
-                const bool ends = c.k + 1 >= c.span.count;
-                if (t + 1 < tiles) {
-                    if (ends) c.next_item(p); else ++c.k;
-                    look();
-                } else {
-                    page = -1;
-                }
-                load(false, key_offset);
-                if (t > 0 && !(S::kQueries == 1 && first)) load(true, value_offset);
-                value_offset = next_value;
-                first = ends;
-                if (ends) ++segment;
-            }
             if (!TMA) {
-                load(true, value_offset);
-                asm volatile("cp.async.wait_group 0;" ::: "memory");
-                announce(x);
+                int64_t key_offset = -1, value_offset = -1, next_value = -1;         // of the tile at hand, of the one before, of the tile at hand
+                float ks = 0.f, vs = 0.f;
+                auto place = [&] {                   // of the cursor's tile, looked up before
+                    key_offset = page < 0 ? -1 : row_offset(p.c.key_stride, page, c.head, in_page) * (int64_t)sizeof(TC);
+                    next_value = page < 0 ? -1 : row_offset(p.c.value_stride, page, c.head, in_page) * (int64_t)sizeof(TC);
+                    if constexpr (kCodes) {
+                        ks = page < 0 ? 0.f : p.c.key_scale[row_offset(p.c.key_scale_stride, page, c.head, in_page)];
+                        vs = page < 0 ? 0.f : p.c.value_scale[row_offset(p.c.value_scale_stride, page, c.head, in_page)];
+                    }
+                };
+                auto store_values = [&] {
+                    if constexpr (kCodes) put(true, value_offset); else load(true, value_offset);
+                };
+                look();
+                place();
+                for (int t = 0; t < tiles; ++t) {
+                    if (first) {
+                        if (S::kQueries == 1 && t > 0) store_values();
+                        load_query(segment);
+                    }
+                    // this tile's rows: which of them are there, their scales.  A description is written anew only when its last reader has
+                    // passed: the key slot of this tile was freed later than that (static_assert above); so wait for the slot first
+                    const unsigned rows = __ballot_sync(kFull, page >= 0);
+                    const int meta = t % kMetaRing;
+                    if (!mbar_try_wait(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1)) {
+                        if (!kCodes) {
+                            asm volatile("cp.async.wait_group 0;" ::: "memory");
+                            announce(x);
+                        }
+                        mbar_wait_spin(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
+                    }
+                    if (lane == 0) key_mask[meta * 4 + w] = rows;
+                    if (kCodes) {
+                        const int n = (lane >> 4) * 64 + w * 16 + (lane & 15);
+                        key_scale[meta * kTileKeys + n] = ks;
+                        value_scale[meta * kTileKeys + n] = vs;
+                        const float top = warp_max(fabsf(vs));
+                        if (lane == 0) value_top[meta * 4 + w] = top;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bar.keys_full[meta]);
+                    // on to the next tile before the copies: its page numbers arrive meanwhile
+                    const bool ends = c.k + 1 >= c.span.count;
+                    const int64_t value_now = next_value;
+                    const bool more = t + 1 < tiles;
+                    if (more) {
+                        if (ends) c.next_item(p); else ++c.k;
+                        look();
+                    }
+                    if constexpr (kCodes) put(false, key_offset); else load(false, key_offset);
+                    if (t > 0 && !(S::kQueries == 1 && first)) store_values();
+                    value_offset = value_now;
+                    if (more) place();
+                    first = ends;
+                    if (ends) ++segment;
+                }
+                store_values();
+                if (!kCodes) {
+                    asm volatile("cp.async.wait_group 0;" ::: "memory");
+                    announce(x);
+                }
             }
         } else if (warp == kEdgeWarp) {
             // ------------------------------------------------------------------------------------------------- edges
@@ -552,6 +574,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     if (t + 1 < tiles) {
                         if (ends) c.next_item(p); else ++c.k;
                     }
+                }
+            } else {
+                // rows written by the producers' threads: announced to the pair from here, because a release at cluster scope waits for all
+                // of its thread's memory accesses, and this warp has none
+                for (int x = 0; x < 2 * tiles; ++x) {
+                    mbar_wait_spin(&bar.landed[x % kSlots], (x / kSlots) & 1, abort_flag);
+                    if (lane == 0) arrive_first_release(&bar.full[x % kSlots]);
+                    __syncwarp();
                 }
             }
         } else if (warp == kMmaWarp) {

@@ -21,7 +21,7 @@ int dtype_bytes(int dtype) { return dtype == FK_F32 ? 4 : dtype == FK_E4M3 ? 1 :
 int check_cache(const fk_kv_cache& c) {
     if (c.pages < 1 || c.kv_heads < 1 || c.page_size < 1 || c.head_dim < 1 || c.head_dim > FK_MAX_HEAD_DIM) return FK_ERR_ARG;
     if (c.seqs < 0 || c.max_pages < 0 || c.table_stride < 0) return FK_ERR_ARG;
-    if ((int64_t)c.max_pages * c.page_size > INT32_MAX) return FK_ERR_ARG;
+    if ((int64_t)c.max_pages * c.page_size > INT32_MAX - 1024) return FK_ERR_ARG;       // positions past a tile's end are still ints
     if (c.dtype < FK_F32 || c.dtype > FK_E4M3) return FK_ERR_UNSUPPORTED;
     if (!c.key || !c.value) return FK_ERR_ARG;
     if (c.seqs > 0 && (!c.lengths || (c.max_pages > 0 && !c.page_table))) return FK_ERR_ARG;

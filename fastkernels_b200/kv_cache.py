@@ -104,8 +104,8 @@ def _pack_cache(into: Any, key_cache, value_cache, page_table, lengths, query_st
     seqs, max_pages = table_shape = page_table.shape
     _check_index(page_table, "page_table", table_shape, device)
     _check_index(lengths, "lengths", (seqs,), device)
-    if max_pages * page_size >= 1 << 31:
-        raise ValueError("page_table must hold less than 2^31 positions per sequence")
+    if max_pages * page_size >= (1 << 31) - 1024:
+        raise ValueError("page_table must hold less than 2^31 - 1024 positions per sequence")
     if query_starts is not None:
         _check_index(query_starts, "query_starts", (seqs + 1,), device)
     if dtype == _E4M3:
@@ -179,7 +179,7 @@ def paged_kv_append(key: Any, value: Any, key_cache: Any, value_cache: Any, page
 
     A float8_e4m3fn cache keeps `value = code * scale` with one fp32 scale per token and head in `key_scale` / `value_scale`
     `[pages, kv_heads, page_size]`: scale = max(|x|, 2^-100) / 448, the code is the nearest one (ties to even) to
-    x * 448 / max.  A row with an infinity or a NaN reads back as NaN.  Rows behind the last sequence are ignored.
+    x * 448 / max.  A row with an infinity or a NaN reads back as NaN.  Rows behind the last sequence are ignored.  `key` and `value` must not be views of the cache.
     """
     c, r = KvCache(), KvRows()
     heads, dim, _ = _pack_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
