@@ -103,7 +103,6 @@ struct FewShape {
     static constexpr int kTiles = kPitch <= 128 ? 2 : 1, kKeys = 16 * kTiles;
     static constexpr uint32_t kAllRows = 0xffffffffu >> (32 - kKeys);
     static constexpr int kSlot = kKeys * kPitch;
-    static constexpr int kGroups = kPitch >= 128 ? kPitch / 128 : 1;   // a slot is [groups of 128 bytes][keys]
     static constexpr int kWarps = kCodes && NT == 1 && D <= 128 ? 12 : 8;      // as many as the registers hold
     static constexpr int kFit = 192 * 1024 / kWarps / kSlot;           // slots per warp in 192 KB
     static constexpr int kSlots = kFit > 8 ? 8 : kFit;

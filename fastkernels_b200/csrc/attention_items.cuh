@@ -109,12 +109,6 @@ __device__ __forceinline__ int64_t seq_tiles(const AttnParams& p, const SeqRows&
     return sum;
 }
 
-__device__ __forceinline__ int64_t warp_sum64(int64_t v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-    return v;
-}
-
 // The order's extent and, in shared memory, where each sequence ends in it: upto[s] key tiles up to and with sequence s, for as many
 // sequences as `room` holds (others are counted again by locate).  Every thread of the block calls it; `scratch` holds two words
 // per warp.

@@ -136,13 +136,6 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
           "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-          "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
-          "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr) : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
                  "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
@@ -180,10 +173,8 @@ __device__ __forceinline__ uint4 codes8_to_half(uint2 c) {
     return r;
 }
 
-// Key of column / value row n of a tile, relative to its first.  Where threads copy the rows, producer warp w looks up keys
-// 32 w .. 32 w + 31 and puts 16 of them into each block's half of the columns.
-template <bool TMA>
-__device__ __forceinline__ constexpr int key_of_column(int n) { return TMA ? n : ((n & 63) >> 4) * 32 + (n >> 6) * 16 + (n & 15); }
+// Keys of a tile by column (and by value row): with tensor copies, column n is key n.  Where threads copy the rows, producer warp w looks
+// up keys 32 w .. 32 w + 31 and puts 16 of them into each block's half of the columns: column n is key 32 (n % 64 / 16) + 16 (n / 64) + n % 16.
 
 // Copies of a box of [unit rows][64 columns] out of one page into this block's shared memory, announced at the pair's first block's
 // barrier (address in the cluster's window).

@@ -13,8 +13,6 @@ struct RowPlace {
     int pos;       // position in the sequence; may lie outside of it if starts and lengths do not fit together
 };
 
-__device__ __forceinline__ int seq_first(const int* starts, int s) { return starts ? starts[s] : s; }
-
 __device__ __forceinline__ RowPlace place_of_row(const int* __restrict__ starts, const int* __restrict__ lengths, int seqs, int rows, int row) {
     RowPlace r{-1, 0};
     if (starts == nullptr) {

@@ -514,3 +514,33 @@ def test_long_chunks(new, lengths, window, sinks, dim, kv_heads, group, dtype, c
             err = (got[starts[s]:starts[s + 1], a].double() - out).abs()
             tol = O.bound(dtype, out, mag, size, seen.sum(-1).double(), dim)
             assert (err <= tol).all(), f"sequence {s} head {a}: {(err / tol).max():.2f} times the bound"
+
+
+@pytest.mark.parametrize("page", [2, 8, 16, 24, 48, 64, 80, 128, 256])
+@pytest.mark.parametrize("dtype,cache,dim", [(BF, BF, 256), (F16, E4, 128), (F16, F16, 64)])
+@pytest.mark.parametrize("new", [[1, 1, 1], [70, 1, 300]])
+def test_attention_page_sizes(page, dtype, cache, dim, new):
+    """Pages smaller and larger than a tile of keys, with and without tensor copies, ending inside of tiles."""
+    b = Batch(page, new, [517, 129, 300], kv_heads=2, heads=8, dim=dim, page=page, dtype=dtype, cache=cache)
+    b.check(b.attend(max_query=max(new)))
+    b.check(b.attend(max_query=max(new), window=100, sinks=3), window=100, sinks=3)
+
+
+def test_calls_on_two_streams_at_once():
+    """Decode and chunk calls of both cache types issued on two streams without waiting give what they give alone."""
+    batches = [Batch(s, new, [900, 400, 700], kv_heads=2, heads=16, dim=256, cache=cache) for s, (new, cache) in
+               enumerate([([1, 1, 1], BF), ([200, 1, 64], BF), ([1, 1, 1], E4), ([200, 1, 64], E4)])]
+    args = [(b.q.cuda(), *b.dev()) for b in batches]
+
+    def call(i):
+        return fk.paged_attention(*args[i], max_query=max(batches[i].new), **batches[i].scales)
+    alone = [call(i) for i in range(4)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for turn in range(10):
+        for i in range(4):
+            with torch.cuda.stream(streams[(i + turn) % 2]):
+                got.append((i, call(i)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(alone[i], x) for i, x in got)
