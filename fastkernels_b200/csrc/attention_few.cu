@@ -242,6 +242,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 
     ItemCursor<S::kKeys> cur, ahead;
     if (run0 < run1) locate(p, run0, upto, room, cur);
+    if (TMA) fence_async_proxy();                // every thread's accesses to the plan, before copies of the other proxy write there
     __syncthreads();                             // the plan's memory is the ring's from here on
     ahead = cur;
 
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     auto next_slot = [&](bool issue_values) {
         if (TMA) mbar_wait_spin(&landed[slot], phase, abort_flag);
         else asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
-        if (TMA && zeroed) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        if (TMA && zeroed) fence_async_proxy();
         zeroed = false;
         __syncwarp();
         issue(issue_values);

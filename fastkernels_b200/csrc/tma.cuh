@@ -84,6 +84,10 @@ __device__ __forceinline__ void mbar_wait_spin(uint64_t* bar, uint32_t parity, v
     }
 }
 
+// Orders this thread's ordinary accesses to shared memory with those of bulk and tensor copies and of tensor-core operands
+// (the async proxy), on both sides of a barrier that follows.
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
 // Contiguous global -> shared copy of `bytes` (multiple of 16, both addresses 16-byte aligned);
 // completion is signalled on `bar` as transaction bytes.
 __device__ __forceinline__ void bulk_load(void* dst_smem, const void* src_gmem, uint32_t bytes, uint64_t* bar) {

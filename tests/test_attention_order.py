@@ -1,0 +1,22 @@
+"""CPU: orderings that the attention kernels' correctness rests on and that no run on a GPU can show to be missing, checked in
+their source."""
+
+import re
+from pathlib import Path
+
+import pytest
+
+CSRC = Path(__file__).resolve().parents[1] / "fastkernels_b200" / "csrc"
+
+
+def code(name):
+    """A kernel file without its comments."""
+    return re.sub(r"//[^\n]*", "", (CSRC / name).read_text())
+
+
+@pytest.mark.parametrize("name", ["attention_few.cu", "attention_tile.cu"])
+def test_the_plan_is_fenced_from_the_copies_that_take_its_memory(name):
+    """The plan is written and read in the ring's memory by ordinary accesses; tensor copies, which belong to the async proxy, write there
+    next.  A barrier alone does not order the two proxies: every thread has to fence before it."""
+    after = code(name).split("locate(p, run0, upto, room", 1)[1]
+    assert "fence_async_proxy();" in after.split("__syncthreads();", 1)[0]
