@@ -282,6 +282,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 for (; arrived < upto; ++arrived)
                     if (lane == 0) mbar_arrive(&bar.landed[arrived % kSlots]);
             };
+            // Whether the next load's slot is free, the same for all lanes: one that sees the phase change before another must not leave the
+            // warp alone in what follows, which announces loads for all of it
+            auto slot_free = [&] { return __all_sync(kFull, mbar_try_wait(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1)) != 0; };
             auto load_query = [&](int segment) {     // 32 of the block's 128 rows per warp
                 if (!kCodes && !TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
                 if (!TMA) announce(x);               // the products that read the old rows wait for these loads
@@ -351,7 +354,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             // threads' copies of 16-bit rows; offset: bytes of this lane's row, < 0: no such row
             auto load = [&](bool values, int64_t offset) {
                 const int slot = x % kSlots;
-                if (!mbar_try_wait(&bar.empty[slot], ((x / kSlots) & 1) ^ 1)) {
+                if (!slot_free()) {
                     asm volatile("cp.async.wait_group 0;" ::: "memory");      // ahead of the products: announce what is on its way first
                     announce(x);
                     mbar_wait_spin(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
@@ -499,7 +502,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     // passed: the key slot of this tile was freed later than that (static_assert above); so wait for the slot first
                     const unsigned rows = __ballot_sync(kFull, page >= 0);
                     const int meta = t % kMetaRing;
-                    if (!mbar_try_wait(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1)) {
+                    if (!slot_free()) {
                         if (!kCodes) {
                             asm volatile("cp.async.wait_group 0;" ::: "memory");
                             announce(x);

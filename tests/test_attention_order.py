@@ -20,3 +20,11 @@ def test_the_plan_is_fenced_from_the_copies_that_take_its_memory(name):
     next.  A barrier alone does not order the two proxies: every thread has to fence before it."""
     after = code(name).split("locate(p, run0, upto, room", 1)[1]
     assert "fence_async_proxy();" in after.split("__syncthreads();", 1)[0]
+
+
+@pytest.mark.parametrize("name", ["attention_few.cu", "attention_tile.cu"])
+def test_a_warp_decides_together_whether_a_barrier_has_passed(name):
+    """A barrier's phase may change between the looks of two lanes.  What depends on a look and is done by the whole warp (announcing the
+    loads of all lanes) needs one answer for all of them."""
+    looks = [m.start() for m in re.finditer(r"mbar_(?:try|test)_wait\(", code(name))]
+    assert all(code(name)[:at].rstrip().endswith("__all_sync(kFull,") for at in looks)
