@@ -5,10 +5,12 @@
 // sums and statistics in fp32.  Pieces (m, l, acc) of one row over disjoint keys join as
 // m = max m_i, l = sum 2^(m_i - m) l_i, acc = sum 2^(m_i - m) acc_i.
 
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
 #include "attention.cuh"
+#include "kernels.cuh"
 
 namespace fk {
 
@@ -252,6 +254,7 @@ static AttnParams attn_params(const fk_attention_call& a) {
     p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
     if (fabsf(p.scale_log2) < FLT_MIN) p.scale_log2 = FLT_MIN;
     p.part = reinterpret_cast<float*>(a.workspace);
+    p.wait_cycles = (uint32_t)std::min(wait_limit_cycles(), 1ll << 31);       // clocks are compared in 32 bits
     return p;
 }
 

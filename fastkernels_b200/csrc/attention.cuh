@@ -19,6 +19,7 @@ struct AttnParams {
     int splits;                // pieces of the key axis (shape-agnostic kernel)
     float* part;               // partial results
     int tile_tokens;           // tokens of an item of the kernels that work on tiles of tokens
+    uint32_t wait_cycles;      // limit of every wait for a barrier
 };
 
 // What a token at position p sees: [0, min(sinks, lo)) and [lo, p], lo = first position of its window.

@@ -180,7 +180,7 @@ struct Joined {
 #pragma unroll
             for (int e = 0; e < kVec; ++e) {
                 const float v = l == 0.f ? 0.f : acc[c][e] / l;
-                odd |= !(fabsf(v) < INFINITY);
+                odd |= l == l && !(fabsf(v) < INFINITY);
                 store_elem(out + dim(lane, c, e), v);
             }
         if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, row, h.pos0 + tok, qh);
@@ -317,8 +317,9 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     bool zeroed = false;                         // threads wrote to the slot that is read
     // the oldest slot has landed for the whole warp, and the one before it is free
     auto next_slot = [&](bool issue_values) {
-        if (TMA) mbar_wait_spin(&landed[slot], phase, abort_flag);
-        else asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
+        if (TMA) {
+            if (left >= 0 && !warp_wait(&landed[slot], phase, abort_flag, p.wait_cycles)) left = -1;       // nothing more is issued or waited for
+        } else asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
         if (TMA && zeroed) fence_async_proxy();
         zeroed = false;
         __syncwarp();
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 4);
                 l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 8);
                 l[nt][c] += __shfl_xor_sync(kFull, l[nt][c], 16);
-                if (TMA && *reinterpret_cast<volatile int*>(abort_flag)) l[nt][c] = NAN;       // a copy that never came: no number is right
+                if (TMA && left < 0) l[nt][c] = NAN;       // a copy that never came: no number is right
             }
         if (begins && ends) {
             bool odd = false;
@@ -613,7 +614,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const float v = l[nt][c] == 0.f ? 0.f : acc[nt][i][c + 2 * h] * inv;
-                            odd |= !(fabsf(v) < INFINITY);
+                            odd |= l[nt][c] == l[nt][c] && !(fabsf(v) < INFINITY);
                             store_elem(out + dim_of(i, h), v);
                         }
                 }
@@ -646,6 +647,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
         if (at < run1) cur.next_item(p);
     }
 
+    if (TMA && *reinterpret_cast<volatile int*>(abort_flag)) linger();       // copies still on their way to this block
     // ---- the parts of the block's warps: one that does not begin its item continues the one before it.  All threads take four
     // dimensions of a column each, so that a part costs one round of loads
     if (threadIdx.x < S::kCols) odd_column[threadIdx.x] = 0;
@@ -691,7 +693,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     const float r = l == 0.f ? 0.f : v[x] / l;
-                    odd |= !(fabsf(r) < INFINITY);
+                    odd |= l == l && !(fabsf(r) < INFINITY);
                     store_elem(out + x, r);
                 }
                 if (odd && h.tokens > 1) odd_column[n] = 1;

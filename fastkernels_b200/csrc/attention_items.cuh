@@ -215,7 +215,8 @@ __device__ __forceinline__ void zero_blind_rows(const AttnParams& p) {
 }
 
 // A row whose result is not finite, alone and exactly: in a tile of several tokens a key that one of them must not see may have
-// entered the row's product as 0 * infinity.  A whole warp.
+// entered the row's product as 0 * infinity.  It cannot have entered the sum of the weights: where that is no number the result is final.
+// A whole warp.
 template <typename T, typename TC>
 __device__ __noinline__ void row_again(const AttnParams& p, int seq, int row, int pos, int qh) {
     const int lane = threadIdx.x & 31, D = p.c.head_dim;

@@ -192,6 +192,12 @@ __device__ __forceinline__ void arrive_expect(uint32_t cluster_bar, uint32_t byt
     asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cluster_bar), "r"(bytes) : "memory");
 }
 
+// Sets the flag at the same address of the pair's other block.
+__device__ __forceinline__ void tell_other_block(int* flag) {
+    asm volatile("{\n\t.reg .b32 a, r;\n\tmov.u32 r, %%cluster_ctarank;\n\txor.b32 r, r, 1;\n\tmapa.shared::cluster.u32 a, %0, r;\n\tst.shared::cluster.u32 [a], 1;\n\t}"
+                 ::"r"(smem_u32(flag)) : "memory");
+}
+
 // Whether the cursor's key tile has keys that no row of the item sees.
 __device__ __forceinline__ bool edge_tile(const AttnParams& p, const ItemCursor<kTileKeys>& c) {
     const int key0 = c.key0();
@@ -247,6 +253,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     tc_fence_after_sync();
     const uint32_t tmem = bar.tmem, tmem_s = tmem + (D == 256 ? 256 : 128);
     volatile int* abort_flag = &bar.abort_flag;
+    // Both blocks of the pair give up together: a warp whose wait fails issues nothing more, so whatever the other block then waits for
+    // stays away, and what it has been given by then is right
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+        if (warp_wait(b, parity, abort_flag, p.wait_cycles)) return true;
+        tell_other_block(&bar.abort_flag);
+        return false;
+    };
     pdl_wait();
 
     int64_t* upto = reinterpret_cast<int64_t*>(smem);              // over the queries and the ring, before their first copy
@@ -274,6 +287,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 if (c.some_row_sees(p, j)) page = page_of(p.c, c.seq, j, in_page);
             };
             int x = 0;                               // loads so far
+            bool alive = true;                       // no wait has failed
             int arrived = 0;                         // of them announced
             constexpr int kLag = 2;                  // loads in flight behind the newest
             auto announce = [&](int upto) {          // loads below `upto` have landed for this thread
@@ -285,6 +299,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             // Whether the next load's slot is free, the same for all lanes: one that sees the phase change before another must not leave the
             // warp alone in what follows, which announces loads for all of it
             auto slot_free = [&] { return __all_sync(kFull, mbar_try_wait(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1)) != 0; };
+            auto wait_slot = [&] { return wait(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1); };
             auto load_query = [&](int segment) {     // 32 of the block's 128 rows per warp
                 if (!kCodes && !TMA) asm volatile("cp.async.wait_group 0;" ::: "memory");
                 if (!TMA) announce(x);               // the products that read the old rows wait for these loads
@@ -298,8 +313,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     if (n >= cols || chunk * 8 >= dim) return nullptr;
                     return reinterpret_cast<const T*>(p.query) + (int64_t)(first_row + tok) * p.qs[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.qs[1] + chunk * 8;
                 };
+                auto free_buffer = [&] { return wait(&bar.q_empty[buffer], ((segment / S::kQueries) & 1) ^ 1); };
                 if (!kCodes) {
-                    mbar_wait_spin(&bar.q_empty[buffer], ((segment / S::kQueries) & 1) ^ 1, abort_flag);
+                    if (!(alive = free_buffer())) return;
 #pragma unroll 4
                     for (int i = 0; i < kSteps; ++i) {
                         const int r = w * 32 + i * kAtOnce + lane / kChunks;
@@ -315,7 +331,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             const T* q = source(w * 32 + (i0 + b) * kAtOnce + lane / kChunks);
                             raw[b] = q ? *reinterpret_cast<const uint4*>(q) : make_uint4(0, 0, 0, 0);
                         }
-                        if (i0 == 0) mbar_wait_spin(&bar.q_empty[buffer], ((segment / S::kQueries) & 1) ^ 1, abort_flag);
+                        if (i0 == 0 && !(alive = free_buffer())) return;
 #pragma unroll
                         for (int b = 0; b < kBatch; ++b) {
                             const int r = w * 32 + (i0 + b) * kAtOnce + lane / kChunks;
@@ -357,7 +373,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 if (!slot_free()) {
                     asm volatile("cp.async.wait_group 0;" ::: "memory");      // ahead of the products: announce what is on its way first
                     announce(x);
-                    mbar_wait_spin(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
+                    if (!(alive = wait_slot())) return;
                 }
                 const uint32_t base = ring + slot * S::kSlot;
                 const char* from = reinterpret_cast<const char*>(values ? p.c.value : p.c.key);
@@ -402,7 +418,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 uint2 raw[kRaw];
                 fetch(values, offset, raw);
                 const int slot = x % kSlots;
-                mbar_wait_spin(&bar.empty[slot], ((x / kSlots) & 1) ^ 1, abort_flag);
+                if (!(alive = wait_slot())) return;
                 const uint32_t base = ring + slot * S::kSlot;
 #pragma unroll
                 for (int r = 0; r < kRaw; ++r)
@@ -425,11 +441,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         const int j = c.key0() + lane * unit;
                         if (lane < units && j < c.span.end && (p.window == 0 || j + unit > window_start(p, c.pos0) || j < p.sinks)) page = page_of(p.c, c.seq, j, row);
                     };
-                    auto wait_slot = [&] { mbar_wait_spin(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag); };
                     auto tma_values = [&] {
                         constexpr int groups = D / 128;
                         const int slot = x % kSlots;
-                        wait_slot();
+                        if (!(alive = wait_slot())) return;
                         uint32_t to = in_first_block(&bar.full[slot]);
                         if (edge_v) to = smem_u32(&bar.landed[slot]);
                         if (lane == 0 && w == 0) {
@@ -447,9 +462,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     for (int t = 0; t < tiles; ++t) {
                         constexpr int groups = D / 64;
                         if (S::kQueries == 1 && first && t > 0) tma_values();
+                        if (!alive) break;
                         const int slot = x % kSlots, meta = t % kMetaRing, head = c.head;
                         const bool edge = edge_tile(p, c), ends = c.k + 1 >= c.span.count, values_now = t > 0 && !(S::kQueries == 1 && first);
-                        wait_slot();                 // and with it for the last reader of this description (static_assert above)
+                        if (!(alive = wait_slot())) break;       // and with it for the last reader of this description (static_assert above)
                         const uint32_t full = in_first_block(&bar.full[slot]);
                         const unsigned there = __ballot_sync(kFull, page != -1) & (0xffffffffu >> (32 - units));
                         if (lane == 0 && w == 0) {
@@ -464,6 +480,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             pair_tma_load(ring + slot * S::kSlot + g * (64 * 128) + u * unit * 128, &key_map, g * 64, rw, head, pg < 0 ? p.c.pages : pg, full);
                         ++x;
                         if (first) load_query(segment);
+                        if (!alive) break;
                         // on to the next tile: its page numbers arrive while the previous tile's values are issued
                         const int page_now = page, row_now = row;
                         if (t + 1 < tiles) {
@@ -471,11 +488,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             look_unit();
                         }
                         if (values_now) tma_values();
+                        if (!alive) break;
                         page_v = page_now; row_v = row_now; head_v = head; edge_v = edge;
                         first = ends;
                         if (ends) ++segment;
                     }
-                    tma_values();
+                    if (alive) tma_values();
             }
             if (!TMA) {
                 int64_t key_offset = -1, value_offset = -1, next_value = -1;         // of the tile at hand, of the one before, of the tile at hand
@@ -496,8 +514,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 for (int t = 0; t < tiles; ++t) {
                     if (first) {
                         if (S::kQueries == 1 && t > 0) store_values();
-                        load_query(segment);
+                        if (alive) load_query(segment);
                     }
+                    if (!alive) break;
                     // this tile's rows: which of them are there, their scales.  A description is written anew only when its last reader has
                     // passed: the key slot of this tile was freed later than that (static_assert above); so wait for the slot first
                     const unsigned rows = __ballot_sync(kFull, page >= 0);
@@ -507,7 +526,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             asm volatile("cp.async.wait_group 0;" ::: "memory");
                             announce(x);
                         }
-                        mbar_wait_spin(&bar.empty[x % kSlots], ((x / kSlots) & 1) ^ 1, abort_flag);
+                        if (!(alive = wait_slot())) break;
                     }
                     if (lane == 0) key_mask[meta * 4 + w] = rows;
                     if (kCodes) {
@@ -528,17 +547,24 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         look();
                     }
                     if constexpr (kCodes) put(false, key_offset); else load(false, key_offset);
-                    if (t > 0 && !(S::kQueries == 1 && first)) store_values();
+                    if (alive && t > 0 && !(S::kQueries == 1 && first)) store_values();
+                    if (!alive) break;
                     value_offset = value_now;
                     if (more) place();
                     first = ends;
                     if (ends) ++segment;
                 }
-                store_values();
+                if (alive) store_values();
                 if (!kCodes) {
                     asm volatile("cp.async.wait_group 0;" ::: "memory");
                     announce(x);
                 }
+            }
+            // The products' last arrivals at this block's barriers, which nobody else waits for: the block must still be there
+            if (w == 0 && alive) {
+                for (int i = max(0, x - kSlots); i < x && alive; ++i) alive = wait(&bar.empty[i % kSlots], (i / kSlots) & 1);
+                const int queries = first ? segment : segment + 1;
+                for (int i = max(0, queries - S::kQueries); i < queries && alive; ++i) alive = wait(&bar.q_empty[i % S::kQueries], (i / S::kQueries) & 1);
             }
         } else if (warp == kEdgeWarp) {
             // ------------------------------------------------------------------------------------------------- edges
@@ -552,7 +578,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         // order of the loads: K(0), then [K(t + 1), V(t)], but [V(t), K(t + 1)] where t ends an item and there is one query buffer
                         const int slot = ((S::kQueries == 1 && ends) || t + 1 == tiles ? 2 * t + 1 : 2 * t + 2) % kSlots, key0 = c.key0(), lo = window_start(p, c.pos0);
                         const uint32_t base = ring + slot * S::kSlot;
-                        mbar_wait_spin(&bar.landed[slot], (landed >> slot) & 1, abort_flag);
+                        if (!wait(&bar.landed[slot], (landed >> slot) & 1)) break;
                         landed ^= 1u << slot;
                         for (int r = lane; r < kTileKeys; r += 32) {
                             const int j = key0 + r;
@@ -572,7 +598,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 // rows written by the producers' threads: announced to the pair from here, because a release at cluster scope waits for all
                 // of its thread's memory accesses, and this warp has none
                 for (int x = 0; x < 2 * tiles; ++x) {
-                    mbar_wait_spin(&bar.landed[x % kSlots], (x / kSlots) & 1, abort_flag);
+                    if (!wait(&bar.landed[x % kSlots], (x / kSlots) & 1)) break;
                     if (lane == 0) arrive_first_release(&bar.full[x % kSlots]);
                     __syncwarp();
                 }
@@ -592,7 +618,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     if (++slot == kSlots) { slot = 0; phase ^= 1; }
                 };
                 auto scores = [&](int t, bool ends, int buffer) {
-                    mbar_wait_spin(&bar.full[slot], phase, abort_flag);
+                    if (!wait(&bar.full[slot], phase)) return false;
                     tc_fence_after_sync();
                     if (leader) {
                         const uint32_t d = tmem_s + (t & 1) * kTileKeys, k = k_low + slot * (S::kSlot >> 4), q = q_low + buffer * (S::kQuery >> 4);
@@ -605,14 +631,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                     __syncwarp();
                     next();
+                    return true;
                 };
                 auto values = [&](int t, bool begins) {
-                    mbar_wait_spin(&bar.full[slot], phase, abort_flag);
+                    if (!wait(&bar.full[slot], phase)) return false;
                     if (begins) {
-                        if (o_segment > 0) mbar_wait_spin(&bar.o_empty, (o_segment - 1) & 1, abort_flag);
+                        if (o_segment > 0 && !wait(&bar.o_empty, (o_segment - 1) & 1)) return false;
                         ++o_segment;
                     }
-                    mbar_wait_spin(&bar.p_full[t & 1], (t >> 1) & 1, abort_flag);
+                    if (!wait(&bar.p_full[t & 1], (t >> 1) & 1)) return false;
                     tc_fence_after_sync();
                     if (leader) {
                         const uint32_t a = tmem_s + (t & 1) * kTileKeys, v = v_low + slot * (S::kSlot >> 4);
@@ -623,24 +650,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                     __syncwarp();
                     next();
+                    return true;
                 };
-                bool first = true, last_began = false;
+                bool first = true, last_began = false, alive = true;
                 for (int t = 0; t < tiles; ++t) {
                     const bool ends = c.k + 1 >= c.span.count;
                     if (first) {
-                        if (S::kQueries == 1 && t > 0) values(t - 1, last_began);
-                        mbar_wait_spin(&bar.q_full[segment % S::kQueries], (segment / S::kQueries) & 1, abort_flag);
+                        if (S::kQueries == 1 && t > 0) alive = values(t - 1, last_began);
+                        alive = alive && wait(&bar.q_full[segment % S::kQueries], (segment / S::kQueries) & 1);
                         ++segment;
                     }
-                    scores(t, ends || t + 1 == tiles, (segment - 1) % S::kQueries);
-                    if (t > 0 && !(S::kQueries == 1 && first)) values(t - 1, last_began);
+                    alive = alive && scores(t, ends || t + 1 == tiles, (segment - 1) % S::kQueries);
+                    if (t > 0 && !(S::kQueries == 1 && first)) alive = alive && values(t - 1, last_began);
+                    if (!alive) break;
                     last_began = first;
                     first = ends;
                     if (t + 1 < tiles) {
                         if (ends) c.next_item(p); else ++c.k;
                     }
                 }
-                values(tiles - 1, last_began);
+                if (alive) values(tiles - 1, last_began);
             }
         } else {
             // ------------------------------------------------------------------------------------------------- softmax
@@ -651,6 +680,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             const uint32_t o_addr = tmem + lanes;
             float m = -INFINITY, l = 0.f, top = 0.f, qscale = fabsf(p.scale_log2);
             bool begins = true;                                          // of this run's part of the item
+            // When a wait fails the walk goes on without waiting or announcing (the two warps of a row still meet), and every sum from
+            // here on is no number: the factor of the scores says so, which takes no register
+            auto dead = [&] { return qscale != qscale; };
+            auto wait_or_die = [&](uint64_t* b, uint32_t parity) {
+                if (!wait(b, parity)) qscale = NAN;
+            };
             int segment = 0;
             int64_t at = run0;                                           // tile of the order
             int began_k = c.k;
@@ -661,7 +696,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 const int pos = c.pos0 + tok, meta = t % kMetaRing;
                 const int key0 = c.key0();
                 const bool inside = key0 + kTileKeys - 1 <= c.pos0 && (p.window == 0 || key0 >= window_start(p, c.pos1) || key0 + kTileKeys <= p.sinks);
-                mbar_wait_spin(&bar.keys_full[meta], (t / kMetaRing) & 1, abort_flag);
+                wait_or_die(&bar.keys_full[meta], (t / kMetaRing) & 1);
                 uint32_t there[2] = {0xffffffffu, 0xffffffffu};          // one bit per key: its page is not missing
                 bool complete;
                 if (TMA) {
@@ -677,7 +712,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     there[0] = ((v.x >> (16 * half)) & 0xffffu) | ((v.y >> (16 * half)) << 16);
                     there[1] = ((v.z >> (16 * half)) & 0xffffu) | ((v.w >> (16 * half)) << 16);
                 }
-                mbar_wait_spin(&bar.s_full[t & 1], (t >> 1) & 1, abort_flag);
+                wait_or_die(&bar.s_full[t & 1], (t >> 1) & 1);
                 tc_fence_after_sync();
                 const uint32_t s_addr = tmem_s + lanes + (t & 1) * kTileKeys;
                 float s[64];
@@ -688,7 +723,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     m = -INFINITY;
                     l = 0.f;
                     top = 0.f;
-                    if (kCodes) qscale = query_scale[(segment & 3) * 128 + r];
+                    if (kCodes && !dead()) qscale = query_scale[(segment & 3) * 128 + r];
                     began_k = c.k;
                 }
                 if (kCodes) {
@@ -748,7 +783,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 if (!begins) {
                     const float factor = alpha * unit_scale;
                     if (__any_sync(kFull, factor != 1.f)) {              // the same in both warps of a row
-                        mbar_wait_spin(&bar.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, abort_flag);
+                        wait_or_die(&bar.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
                         tc_fence_after_sync();
 #pragma unroll 1
                         for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 16) {
@@ -786,7 +821,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 tmem_wait_st();
                 tc_fence_before_sync();
                 __syncwarp();
-                if (lane == 0) arrive_first(&bar.p_full[t & 1]);
+                if (lane == 0 && !dead()) arrive_first(&bar.p_full[t & 1]);
                 // ---- the end of the item, or of the run
                 const bool ends = c.k + 1 >= c.span.count;
                 if (ends || t + 1 == tiles) {
@@ -795,16 +830,17 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     sums[half * 128 + r] = l;
                     meet();
                     l = sums[r] + sums[128 + r];                         // in this order in both threads
-                    mbar_wait_spin(&bar.o_done[t & 1], (t >> 1) & 1, abort_flag);
+                    if (t > 0) wait_or_die(&bar.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1);      // long over; at the run's end nobody else sees that it arrived
+                    wait_or_die(&bar.o_done[t & 1], (t >> 1) & 1);
                     tc_fence_after_sync();
                     const int tokens = c.tokens(p), cols = tokens * p.group, first_row = c.first_row(p);
                     const bool whole = ends && began_k == 0;
-                    const float scale_out = kCodes ? (top > 0.f ? top : 1.f) : 1.f;
+                    if (dead()) l = NAN;
+                    const float scale_out = dead() ? NAN : kCodes ? (top > 0.f ? top : 1.f) : 1.f;
                     const int which = at - (c.k - began_k) == run0 ? 0 : 1;
                     float* part = parts + which * (int64_t)S::kPart;
                     T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first_row + tok) * p.os[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.os[1];
                     const float inv = l == 0.f ? 0.f : scale_out / l;
-                    const bool failed = *abort_flag != 0;
                     bool odd = false;
                     const bool wide = (dim & 15) == 0 && ((p.os[0] | p.os[1]) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0;
 #pragma unroll 1
@@ -817,7 +853,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                                 for (int e = 0; e < 16; ++e) {
                                     o[e] = l == 0.f ? 0.f : o[e] * inv;
                                     if (i + e < dim) odd |= !(fabsf(o[e]) < INFINITY);
-                                    if (failed) o[e] = NAN;
                                 }
                                 // a row per thread: 32 bytes at a time fill whole sectors
                                 if (wide) {
@@ -832,7 +867,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                                 }
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) o[e] = failed ? NAN : o[e] * scale_out;
+                                for (int e = 0; e < 16; ++e) o[e] *= scale_out;
                                 store32(part + 2 * kTileRows + (int64_t)n * D + i, reinterpret_cast<const uint32_t*>(o));
                                 store32(part + 2 * kTileRows + (int64_t)n * D + i + 8, reinterpret_cast<const uint32_t*>(o + 8));
                             }
@@ -840,13 +875,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     }
                     tc_fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) arrive_first(&bar.o_empty);
+                    if (lane == 0 && !dead()) arrive_first(&bar.o_empty);
                     if (whole) {
                         // rows of a tile with several tokens whose result is not finite: once more, when both halves are written
                         float* flags = exchange + (t & 1) * 256;
-                        flags[half * 128 + r] = odd ? 1.f : 0.f;
+                        flags[half * 128 + r] = odd && l == l ? 1.f : 0.f;
                         meet();
-                        unsigned again = half == 0 && tokens > 1 && !failed ? __ballot_sync(kFull, flags[r] + flags[128 + r] != 0.f) : 0u;
+                        unsigned again = half == 0 && tokens > 1 ? __ballot_sync(kFull, flags[r] + flags[128 + r] != 0.f) : 0u;
                         while (again) {
                             const int i = __ffs(again) - 1;
                             again &= again - 1;
@@ -868,6 +903,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             }
         }
     }
+    if (*abort_flag) linger();                       // copies and products still on their way to either block
     __syncwarp();
     tc_fence_before_sync();
     cluster_sync();                                  // nothing more arrives at either block's barriers
@@ -943,7 +979,7 @@ __global__ void __launch_bounds__(256, 4) attention_tile_join_kernel(const __gri
                 const int d = c * 128 + lane * 4 + e;
                 if (d >= p.c.head_dim) continue;
                 const float x = l[r] == 0.f ? 0.f : v[e] / l[r];
-                odd |= !(fabsf(x) < INFINITY);
+                odd |= l[r] == l[r] && !(fabsf(x) < INFINITY);
                 store_elem(out + d, x);
             }
         }

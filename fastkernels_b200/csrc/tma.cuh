@@ -71,17 +71,26 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     return true;
 }
 
-// The same without the back-off, for warps whose next step is what everything waits for.
-__device__ __forceinline__ void mbar_wait_spin(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-    if (mbar_try_wait(bar, parity)) return;
-    const long long limit = *abort_flag ? kWaitCyclesAfterAbort : kWaitCycles;
-    const long long t0 = clock64();
-    while (!mbar_try_wait(bar, parity)) {
-        if (clock64() - t0 > limit) {
+// A whole warp waits, without the back-off: for warps whose next step is what everything waits for.  The answer is the same in all lanes;
+// false when the limit (clocks, below 2^32) ran out, here or in another warp of the block (*abort_flag).  A warp that gets it issues
+// nothing more.  Few registers on purpose: it is inlined where 64 scores are live.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    const uint32_t t0 = (uint32_t)clock();
+    do {
+        if (__any_sync(0xffffffffu, *abort_flag != 0 || (uint32_t)clock() - t0 >= limit)) {
             *abort_flag = 1;
-            return;
+            return false;
         }
-    }
+    } while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)));
+    return true;
+}
+
+// Before a block that gave up leaves: longer than any copy or product that it has in flight can take.
+constexpr long long kLingerCycles = 1 << 20;
+__device__ __forceinline__ void linger() {
+    const long long t0 = clock64();
+    while (clock64() - t0 < kLingerCycles) {}
 }
 
 // Orders this thread's ordinary accesses to shared memory with those of bulk and tensor copies and of tensor-core operands

@@ -125,7 +125,8 @@ int fk_moe_experts_timed(const fk_moe_call* call, void* stream, float* stage_ms,
 /* Limit of every device-side wait on another block or another rank, in SM clock cycles (default: about one
  * second; 0 restores the default).  A wait that runs out never traps and never spins on: the kernel raises an
  * error word, finishes with undefined output, and the next fk_moe_status / fk_ep_status call reports it.
- * Process-wide; applies to calls enqueued afterwards.  No counterpart in the reference, which has no
+ * Process-wide; applies to calls enqueued afterwards.  Paged attention, which has no workspace of its own to keep a word in, uses it for
+ * all of its waits and marks rows as NaN instead.  No counterpart in the reference, which has no
  * device-side waits (each of its stages is a separate launch, e.g.
  * src/fastkernels/kernels/triton/qwen36_expert.py:1249-1308). */
 int fk_set_wait_limit_cycles(long long cycles);
@@ -307,7 +308,7 @@ typedef struct fk_attention_call {
 int fk_kv_append(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
 int fk_kv_gather(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
 /* out = softmax(scale * query . key) value over the positions that each row sees; a row that sees none gives zeros.
- * Every wait inside the kernels is bounded (about a second); one that runs out makes the rows that depended on it NaN. */
+ * Every wait inside the kernels is bounded (fk_set_wait_limit_cycles); one that runs out makes the rows that depended on it NaN. */
 size_t fk_paged_attention_workspace_bytes(const fk_attention_call* call);
 int fk_paged_attention(const fk_attention_call* call, void* stream);
 

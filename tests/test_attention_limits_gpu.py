@@ -1,0 +1,31 @@
+"""GPU: a wait of the attention kernels that runs out.  Nothing here traps, faults or spins without a limit: the wait limit is set to
+(almost) nothing, the kernels give up their waits at once and end by themselves, what depended on a wait is NaN, and the next call is
+right again."""
+
+import pytest
+import torch
+
+from fastkernels_b200 import _lib
+from tests.test_kv_cache_gpu import BF, E4, F16, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [200, 1, 64], [900]])
+@pytest.mark.parametrize("dim,dtype,cache,page", [(256, BF, BF, 16), (128, F16, F16, 12), (256, BF, E4, 16), (128, F16, E4, 32)])
+def test_rows_of_a_wait_that_ran_out_are_nan_and_no_other_number_is_wrong(new, dim, dtype, cache, page):
+    lib = _lib.load()
+    b = Batch(dim + page, new, [900, 400, 700][:len(new)], kv_heads=2, heads=16, dim=dim, page=page, dtype=dtype, cache=cache)
+    want = b.attend(max_query=max(new))
+    torch.cuda.synchronize()
+    try:
+        assert lib.fk_set_wait_limit_cycles(1) == 0
+        got = b.attend(max_query=max(new))
+        torch.cuda.synchronize()
+    finally:
+        assert lib.fk_set_wait_limit_cycles(0) == 0
+    lost = torch.isnan(got)
+    assert torch.equal(torch.where(lost, want, got), want)
+    if max(new) > 1:                                 # a decode warp's copies may land while its queries are loaded: then it has nothing to wait for
+        assert lost.any()
+    assert torch.equal(b.attend(max_query=max(new)), want)

@@ -28,3 +28,16 @@ def test_a_warp_decides_together_whether_a_barrier_has_passed(name):
     loads of all lanes) needs one answer for all of them."""
     looks = [m.start() for m in re.finditer(r"mbar_(?:try|test)_wait\(", code(name))]
     assert all(code(name)[:at].rstrip().endswith("__all_sync(kFull,") for at in looks)
+
+
+def test_every_wait_of_a_pair_reaches_both_blocks_and_stops_what_follows():
+    """Blocks of a pair depend on each other: when a wait of one gives up, the other must learn of it, nothing more may be issued or announced,
+    and neither block may leave while something is on its way to it."""
+    text = code("attention_tile.cu")
+    assert text.count("warp_wait(") == 1 and "mbar_wait" not in text                          # one place, which sets the flag of the other block
+    assert "tell_other_block(&bar.abort_flag);" in text.split("warp_wait(", 1)[1].split("return false;", 1)[0]
+    assert "%%cluster_ctarank" in text and "st.shared::cluster" in text.split("void tell_other_block", 1)[1].split("}\n", 1)[0]
+    waits = re.findall(r"([^\n;{}]*)\bwait\(&?b", text)
+    assert waits and all(re.search(r"(=|!|&&|return) *\(?$", w) for w in waits)               # no answer is thrown away
+    assert all("!dead()" in line for line in re.findall(r"[^\n]*arrive_first\(&bar[^\n]*", text))
+    assert text.rindex("linger();") < text.rindex("cluster_sync();") < text.rindex("pair_tmem_dealloc(tmem)")
