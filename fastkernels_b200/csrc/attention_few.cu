@@ -183,7 +183,10 @@ struct Joined {
                 odd |= l == l && !(fabsf(v) < INFINITY);
                 store_elem(out + dim(lane, c, e), v);
             }
-        if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, row, h.pos0 + tok, qh);
+        if (h.tokens > 1 && __any_sync(kFull, odd)) {
+            __syncwarp();
+            row_again<T, TC>(p, h.seq, h.first_row, h.pos0, h.tokens, tok, qh);
+        }
     }
 };
 
@@ -618,9 +621,10 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                             store_elem(out + dim_of(i, h), v);
                         }
                 }
-            if (tokens > 1 && __any_sync(kFull, odd))
-                for (int n = 0; n < cols; ++n)
-                    row_again<T, TC>(p, cur.seq, first_row + n / p.group, cur.pos0 + n / p.group, cur.head * p.group + n % p.group);
+            if (tokens > 1 && __any_sync(kFull, odd)) {
+                __syncwarp();
+                for (int n = 0; n < cols; ++n) row_again<T, TC>(p, cur.seq, first_row, cur.pos0, tokens, n / p.group, cur.head * p.group + n % p.group);
+            }
         } else {
             const int which = at == run0 ? 0 : 1;
             float* part = parts + which * S::kPart;
@@ -707,7 +711,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
             for (int n = warp; n < cols; n += S::kWarps) {
                 const bool odd = odd_column[n] != 0;
                 __syncwarp();
-                if (odd) row_again<T, TC>(p, h.seq, h.first_row + n / p.group, h.pos0 + n / p.group, h.head * p.group + n % p.group);
+                if (odd) row_again<T, TC>(p, h.seq, h.first_row, h.pos0, h.tokens, n / p.group, h.head * p.group + n % p.group);
                 if (lane == 0) odd_column[n] = 0;
             }
             __syncthreads();

@@ -214,16 +214,60 @@ __device__ __forceinline__ void zero_blind_rows(const AttnParams& p) {
     }
 }
 
-// A row whose result is not finite, alone and exactly: in a tile of several tokens a key that one of them must not see may have
-// entered the row's product as 0 * infinity.  It cannot have entered the sum of the weights: where that is no number the result is final.
-// A whole warp.
-template <typename T, typename TC>
-__device__ __noinline__ void row_again(const AttnParams& p, int seq, int row, int pos, int qh) {
+// Columns of the values at positions [from, to) of a sequence that are not finite (NAN_ONLY: not a number), one bit per group of 32 columns,
+// for this lane's column of each.  A whole warp: a lane looks a position up, then the rows are read one after the other.
+template <typename TC, bool NAN_ONLY>
+__device__ __forceinline__ unsigned odd_columns(const AttnParams& p, int seq, int head, int from, int to) {
     const int lane = threadIdx.x & 31, D = p.c.head_dim;
+    const TC* values = reinterpret_cast<const TC*>(p.c.value);
+    unsigned odd = 0;
+    for (int64_t j0 = max(from, 0); j0 < to; j0 += 32) {
+        int in_page = 0, page = -1;
+        if (j0 + lane < to) page = page_of(p.c, seq, (int)(j0 + lane), in_page);
+        const int64_t off = page < 0 ? -1 : row_offset(p.c.value_stride, page, head, in_page);
+        float scale = 1.f;
+        if (sizeof(TC) == 1 && page >= 0) scale = p.c.value_scale[row_offset(p.c.value_scale_stride, page, head, in_page)];
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) {
+            const int64_t row = __shfl_sync(kFull, off, i);
+            const float one = __shfl_sync(kFull, scale, i);
+            if (row < 0) continue;
+#pragma unroll
+            for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
+                if (c * 32 + lane < D) {
+                    const float v = load_elem(values + row + c * 32 + lane) * one;
+                    if (NAN_ONLY ? v != v : !(fabsf(v) < INFINITY)) odd |= 1u << c;
+                }
+        }
+    }
+    return odd;
+}
+
+// A row of an item of several tokens, once more by itself and exactly if its result owes a number that is not finite to a key that it does
+// not see: such a key's value may have entered the row's product as 0 * infinity.  Only keys that some tokens of the item see and others
+// do not can: those of the item's own tokens, and those that the window leaves behind.  They are looked at first, so that numbers that
+// are not finite and that the row does see cost no second pass over its keys; nor do columns in which it sees a NaN among them anyway.  A whole warp;
+// the item's tokens are at positions pos0 .. pos0 + tokens - 1, the row is the tok-th of them.
+template <typename T, typename TC>
+__device__ __noinline__ void row_again(const AttnParams& p, int seq, int first_row, int pos0, int tokens, int tok, int qh) {
+    const int lane = threadIdx.x & 31, D = p.c.head_dim, row = first_row + tok, pos = pos0 + tok, pos1 = pos0 + tokens - 1, head = qh / p.group;
+    T* out = reinterpret_cast<T*>(p.out) + row * p.os[0] + qh * p.os[1];
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
+        if (c * 32 + lane < D) odd |= !(fabsf(to_float(out[c * 32 + lane])) < INFINITY);
+    if (!__any_sync(kFull, odd)) return;
+    const int all = p.c.max_pages * p.c.page_size, lo = window_start(p, pos);
+    unsigned hidden = odd_columns<TC, false>(p, seq, head, pos + 1, min(pos1 + 1, all));
+    if (p.window > 0) hidden |= odd_columns<TC, false>(p, seq, head, max(window_start(p, pos0), p.sinks), min(lo, all));
+    if (!__any_sync(kFull, hidden != 0)) return;
+    hidden &= ~odd_columns<TC, true>(p, seq, head, max(pos0, lo), min(pos + 1, all));
+    if (p.window > 0) hidden &= ~odd_columns<TC, true>(p, seq, head, lo, min(min(window_start(p, pos1), pos + 1), all));
+    if (!__any_sync(kFull, hidden != 0)) return;
     const T* query = reinterpret_cast<const T*>(p.query) + row * p.qs[0] + qh * p.qs[1];
     RowSums r;
-    warp_row<TC, false>(p, [&](int d) { return d < D ? load_elem(query + d) * p.scale_log2 : 0.f; }, seq, qh / p.group, pos, 0, 1, r);
-    T* out = reinterpret_cast<T*>(p.out) + row * p.os[0] + qh * p.os[1];
+    // 16 bytes (8 of codes) at a time: the kernels of tiles only take calls whose rows allow it
+    warp_row<TC, true>(p, [&](int d) { return d < D ? load_elem(query + d) * p.scale_log2 : 0.f; }, seq, head, pos, 0, 1, r);
 #pragma unroll
     for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
         if (c * 32 + lane < D) store_elem(out + c * 32 + lane, r.l == 0.f ? 0.f : r.acc[c] / r.l);

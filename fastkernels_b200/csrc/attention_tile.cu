@@ -62,7 +62,7 @@ struct TileBarriers {
     uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], o_empty;
     uint64_t keys_full[kMetaRing];
     uint32_t tmem;
-    int abort_flag;
+    int abort_flag, odd;
 };
 static_assert(sizeof(TileBarriers) <= 640, "fits behind the ring");
 
@@ -204,6 +204,11 @@ __device__ __forceinline__ bool edge_tile(const AttnParams& p, const ItemCursor<
     return !(key0 + kTileKeys <= c.span.end && (p.window == 0 || key0 >= window_start(p, c.pos0) || key0 + kTileKeys <= p.sinks));
 }
 
+// Workspace: two parts' heads per pair, one mark per block (it wrote a whole item's row of several tokens that is not finite), the parts.
+__host__ __device__ inline size_t tile_head_bytes(int pairs) { return (size_t)pairs * 2 * sizeof(PartHead) + ((size_t)pairs * 2 * sizeof(int) + 31) / 32 * 32; }
+__device__ __forceinline__ int* tile_marks(const AttnParams& p, int pairs) { return reinterpret_cast<int*>(reinterpret_cast<PartHead*>(p.part) + 2 * pairs); }
+__device__ __forceinline__ float* tile_parts(const AttnParams& p, int pairs) { return p.part + tile_head_bytes(pairs) / sizeof(float); }
+
 // D: dimensions of the tiles, a multiple of 128 not below head_dim (the rest is zero).  T: type of queries and results, TC: of the
 // cache.  TMA: rows come by tensor copies of `unit` rows (a divisor of the page size), else by the producers' threads.
 template <int D, typename T, typename TC, bool TMA>
@@ -239,7 +244,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             mbar_init(&bar.o_done[i], 1); mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 16); }
         mbar_init(&bar.o_empty, 16);
         for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], TMA ? 1 : 4);
-        bar.abort_flag = 0;
+        bar.abort_flag = bar.odd = 0;
         mbar_init_fence();
         if (TMA) {
             prefetch_tensormap(&key_map);
@@ -268,7 +273,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     const int64_t run0 = runs.begin(pair), run1 = runs.begin(pair + 1);
     const int tiles = (int)(run1 - run0);
     PartHead* heads = reinterpret_cast<PartHead*>(p.part) + 2 * (int64_t)pair;
-    float* parts = p.part + runs.workers * 2 * (sizeof(PartHead) / 4) + 2 * (int64_t)pair * S::kPart;
+    float* parts = tile_parts(p, pairs) + 2 * (int64_t)pair * S::kPart;
     if (threadIdx.x == 0 && rank == 0) heads[0].begins = heads[0].ends = heads[1].begins = heads[1].ends = -1;
 
     ItemCursor<kTileKeys> c;
@@ -877,17 +882,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     __syncwarp();
                     if (lane == 0 && !dead()) arrive_first(&bar.o_empty);
                     if (whole) {
-                        // rows of a tile with several tokens whose result is not finite: once more, when both halves are written
-                        float* flags = exchange + (t & 1) * 256;
-                        flags[half * 128 + r] = odd && l == l ? 1.f : 0.f;
-                        meet();
-                        unsigned again = half == 0 && tokens > 1 ? __ballot_sync(kFull, flags[r] + flags[128 + r] != 0.f) : 0u;
-                        while (again) {
-                            const int i = __ffs(again) - 1;
-                            again &= again - 1;
-                            const int row = rank * 128 + quarter * 32 + i, rt = row / p.group;
-                            row_again<T, TC>(p, c.seq, first_row + rt, c.pos0 + rt, c.head * p.group + row - rt * p.group);
-                        }
+                        // the join kernel sees to rows whose result is not finite: nothing here waits for that
+                        if (odd && l == l && tokens > 1) bar.odd = 1;
                     } else {
                         if (n < cols && half == 0) { part[n] = m; part[kTileRows + n] = l; }
                         if (rank == 0 && threadIdx.x == 0)
@@ -907,9 +903,30 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     __syncwarp();
     tc_fence_before_sync();
     cluster_sync();                                  // nothing more arrives at either block's barriers
+    if (threadIdx.x == 0) tile_marks(p, pairs)[blockIdx.x] = bar.odd;
     if (warp == kMmaWarp) {
         tc_fence_after_sync();
         pair_tmem_dealloc(tmem);
+    }
+}
+
+// Rows of the whole items of this block's pair that are not finite (row_again): the pair's run is walked once more, its rows dealt to the warps
+// of the blocks of the same pair.
+template <typename T, typename TC>
+__device__ __noinline__ void odd_rows_of_run(const AttnParams& p) {
+    __shared__ int64_t scratch[2 * 8];
+    const Runs runs{plan_tiles<kTileKeys>(p, scratch, nullptr, 0), (int64_t)gridDim.x, 1};
+    const int64_t run1 = runs.begin(blockIdx.x + 1);
+    int64_t at = runs.begin(blockIdx.x);
+    ItemCursor<kTileKeys> c;
+    locate(p, at, nullptr, 0, c);
+    while (at < run1) {
+        const int steps = (int)min((int64_t)(c.span.count - c.k), run1 - at), tokens = c.tokens(p);
+        if (c.k == 0 && steps == c.span.count && tokens > 1)
+            for (int n = blockIdx.y * 8 + (threadIdx.x >> 5); n < tokens * p.group; n += gridDim.y * 8)
+                row_again<T, TC>(p, c.seq, c.first_row(p), c.pos0, tokens, n / p.group, c.head * p.group + n % p.group);
+        at += steps;
+        if (at < run1) c.next_item(p);
     }
 }
 
@@ -921,9 +938,10 @@ __global__ void __launch_bounds__(256, 4) attention_tile_join_kernel(const __gri
     pdl_trigger();
     pdl_wait();
     if (blockIdx.y == 0) zero_blind_rows<T>(p);
-    const int64_t pairs = gridDim.x;
+    const int pairs = gridDim.x;
+    if (tile_marks(p, pairs)[2 * blockIdx.x] | tile_marks(p, pairs)[2 * blockIdx.x + 1]) odd_rows_of_run<T, TC>(p);
     const PartHead* heads = reinterpret_cast<const PartHead*>(p.part);
-    const float* parts = p.part + pairs * 2 * (sizeof(PartHead) / 4);
+    const float* parts = tile_parts(p, pairs);
     const int w0 = blockIdx.x, lane = threadIdx.x & 31, n0 = blockIdx.y * 8 * kRows + (threadIdx.x >> 5) * kRows;
     int which = -1;
 #pragma unroll
@@ -983,7 +1001,10 @@ __global__ void __launch_bounds__(256, 4) attention_tile_join_kernel(const __gri
                 store_elem(out + d, x);
             }
         }
-        if (h.tokens > 1 && __any_sync(kFull, odd)) row_again<T, TC>(p, h.seq, h.first_row + tok, h.pos0 + tok, qh);
+        if (h.tokens > 1 && __any_sync(kFull, odd)) {
+            __syncwarp();
+            row_again<T, TC>(p, h.seq, h.first_row, h.pos0, h.tokens, tok, qh);
+        }
     }
 }
 
@@ -1037,7 +1058,8 @@ template <int D, typename T, typename TC>
 static int tile(AttnParams p, size_t* need, cudaStream_t stream) {
     p.tile_tokens = kTileRows / p.group;
     if (need) {
-        *need = (size_t)(sm_count() / 2) * 2 * (sizeof(PartHead) + TileShape<D, TC>::kPart * sizeof(float));
+        const int pairs = sm_count() / 2;
+        *need = tile_head_bytes(pairs) + (size_t)pairs * 2 * TileShape<D, TC>::kPart * sizeof(float);
         return FK_OK;
     }
     CUtensorMap key_map{}, value_map{};
