@@ -14,7 +14,8 @@
 //
 // 8-bit caches: the codes go to fp16 exactly; a query row is scaled by a power of two into fp16's range (exact for what is
 // within 2^-14 of its largest element, to 2^-25 of it below), scores are multiplied by their key's scale, and the weights by
-// their value's scale over the largest one met so far.  Weights are rounded to the type of the products' operands, fp16 ones
+// their value's scale and a power of two per query row, which follows the largest such product that the row has met: no scale takes bits
+// from the weights of rows that do not see it, or in which it has no weight.  Weights are rounded to the type of the products' operands, fp16 ones
 // after a factor of 2^14 so that small ones keep their bits; sums stay in fp32.
 
 #include <type_traits>
@@ -381,13 +382,20 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 qscale[nt][0] = qscale[nt][1] = p.scale_log2;
             }
         }
-        float acc[NT][kMT][4], m[NT][2], l[NT][2], top = 0.f, inv_top = 1.f;
+        float acc[NT][kMT][4], m[NT][2], l[NT][2];
+        // codes, per column: the largest weight x value scale met so far, and the power of two that such products are multiplied by before they
+        // are rounded; it only moves where one exceeds 2^15 or the maximum of the scores has risen
+        float most_out[NT][2], up_out[NT][2];
+        auto power_for = [](float product) { return __int_as_float(min(max(253 - (__float_as_int(product) >> 23), 15), 239) << 23); };     // -> [1/2, 1)
+        auto inverse = [](float power) { return __int_as_float(0x7f000000 - __float_as_int(power)); };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int i = 0; i < kMT; ++i) acc[nt][i][0] = acc[nt][i][1] = acc[nt][i][2] = acc[nt][i][3] = 0.f;
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.f;
+            most_out[nt][0] = most_out[nt][1] = 0.f;
+            up_out[nt][0] = up_out[nt][1] = 0x1p112f;
         }
         const int sure_lo = window_start(p, cur.pos1);        // keys that every token of the item sees: sure_lo .. pos0
 
@@ -476,8 +484,17 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                         const float a = mn[nt][c] > m[nt][c] ? exp2_fast(m[nt][c] - mn[nt][c]) : 1.f;
                         m[nt][c] = mn[nt][c];
                         l[nt][c] *= a;
+                        float factor = a;
+                        if (kCodes) {
+                            most_out[nt][c] *= a;
+                            if (most_out[nt][c] > 0.f) {
+                                const float power = power_for(most_out[nt][c]);
+                                factor = a * (power * inverse(up_out[nt][c]));
+                                up_out[nt][c] = power;
+                            }
+                        }
 #pragma unroll
-                        for (int i = 0; i < kMT; ++i) { acc[nt][i][c] *= a; acc[nt][i][c + 2] *= a; }
+                        for (int i = 0; i < kMT; ++i) { acc[nt][i][c] *= factor; acc[nt][i][c + 2] *= factor; }
                     }
             }
 #pragma unroll
@@ -505,7 +522,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 zeroed = true;
             }
             if (kCodes) {
-                float v[S::kTiles][2], most = 0.f;
+                float v[S::kTiles][2];
 #pragma unroll
                 for (int kt = 0; kt < S::kTiles; ++kt) {
                     v[kt][0] = scales[vs * S::kKeys + row_lo + 16 * kt];
@@ -514,28 +531,41 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                         if (!(((uint32_t)what.y >> (row_lo + 16 * kt)) & 1)) v[kt][0] = 0.f;
                         if (!(((uint32_t)what.y >> (row_hi + 16 * kt)) & 1)) v[kt][1] = 0.f;
                     }
-                    most = fmaxf(most, fmaxf(fabsf(v[kt][0]), fabsf(v[kt][1])));
                 }
-                most = fmaxf(most, __shfl_xor_sync(kFull, most, 4));
-                most = fmaxf(most, __shfl_xor_sync(kFull, most, 8));
-                most = fmaxf(most, __shfl_xor_sync(kFull, most, 16));
-                if (most > top) {                 // the same in all lanes
-                    const float a = top / most;
-                    top = most;
-                    inv_top = 1.f / top;
+                bool over = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int kt = 0; kt < S::kTiles; ++kt)
+                            over |= fmaxf(fabsf(s[kt][nt][c] * up_out[nt][c] * v[kt][0]), fabsf(s[kt][nt][c + 2] * up_out[nt][c] * v[kt][1])) > 0x1p15f;
+                if (__any_sync(kFull, over)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                        for (int i = 0; i < kMT; ++i)
+                        for (int c = 0; c < 2; ++c) {
+                            float x = most_out[nt][c];
 #pragma unroll
-                            for (int c = 0; c < 4; ++c) acc[nt][i][c] *= a;
+                            for (int kt = 0; kt < S::kTiles; ++kt)
+                                x = fmaxf(x, fmaxf(fabsf(s[kt][nt][c] * 0x1p-14f * v[kt][0]), fabsf(s[kt][nt][c + 2] * 0x1p-14f * v[kt][1])));
+                            x = fmaxf(x, __shfl_xor_sync(kFull, x, 4));
+                            x = fmaxf(x, __shfl_xor_sync(kFull, x, 8));
+                            x = fmaxf(x, __shfl_xor_sync(kFull, x, 16));
+                            if (x == 0.f) continue;
+                            most_out[nt][c] = x;
+                            const float power = power_for(x), factor = power * inverse(up_out[nt][c]);
+                            up_out[nt][c] = power;
+#pragma unroll
+                            for (int i = 0; i < kMT; ++i) { acc[nt][i][c] *= factor; acc[nt][i][c + 2] *= factor; }
+                        }
                 }
 #pragma unroll
-                for (int kt = 0; kt < S::kTiles; ++kt) {
-                    const float v0 = v[kt][0] * inv_top, v1 = v[kt][1] * inv_top;
+                for (int kt = 0; kt < S::kTiles; ++kt)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) { s[kt][nt][0] *= v0; s[kt][nt][1] *= v0; s[kt][nt][2] *= v1; s[kt][nt][3] *= v1; }
-                }
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[kt][nt][i] = s[kt][nt][i] * up_out[nt][i & 1] * v[kt][i >> 1];
             }
 #pragma unroll
             for (int kt = 0; kt < S::kTiles; ++kt) {
@@ -591,7 +621,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 
         // ---- the item's result, or this run's part of it.  acc[.][i][c + 2 h] is column 2t + c at dimension dim_of(i, h)
         auto dim_of = [&](int i, int h) { return kCodes ? (D >= 128 ? ((i >> 3) * 8 + g) * 16 + (i & 7) * 2 + h : g * 8 + i * 2 + h) : i * 16 + g + 8 * h; };
-        const float unit = kCodes ? top : 1.f;
+        auto unit = [&](int nt, int c) { return kCodes ? inverse(up_out[nt][c]) : 1.f; };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -611,7 +641,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                     if (n >= cols) continue;
                     const int tok = n / p.group;
                     T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first_row + tok) * p.os[0] + (int64_t)(cur.head * p.group + n - tok * p.group) * p.os[1];
-                    const float inv = l[nt][c] == 0.f ? 0.f : unit / l[nt][c];
+                    const float inv = l[nt][c] == 0.f ? 0.f : unit(nt, c) / l[nt][c];
 #pragma unroll
                     for (int i = 0; i < kMT; ++i)
 #pragma unroll
@@ -642,7 +672,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
 #pragma unroll
                     for (int i = 0; i < kMT; ++i)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) part[2 * S::kCols + n * D + dim_of(i, h)] = acc[nt][i][c + 2 * h] * unit;
+                        for (int h = 0; h < 2; ++h) part[2 * S::kCols + n * D + dim_of(i, h)] = acc[nt][i][c + 2 * h] * unit(nt, c);
                 }
             if (lane == 0)
                 heads[which] = PartHead{first_row, tokens, cur.head, cur.seq, cur.pos0, begins, ends, runs.worker_of(at - cur.k + cur.span.count - 1) / S::kWarps};

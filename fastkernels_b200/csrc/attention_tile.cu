@@ -14,7 +14,9 @@
 // strides do not allow them, and for codes, which become fp16 on the way, rows gathered by the threads), 12 issues the products (in
 // the pair's first block), 13 zeroes value rows that nobody may see.  m is only raised when a row's maximum grows by more than
 // 2^kLazy, which spares nearly all passes over O.  Weights are rounded to the type of the operands (fp16 after a factor 2^7, which with
-// 2^kLazy stays below 2^15); sums are fp32.
+// 2^kLazy stays below 2^15); sums are fp32.  Codes: a weight is multiplied by its value's scale before it is rounded, and by a power of two of
+// the row's own, which follows the largest such product among the keys that the row sees: a scale far larger or smaller than the others,
+// masked or of no weight, takes no bits from the rest.
 //
 // Key tiles of all tiles are dealt to the pairs in equal contiguous runs as in the few-row kernel; a run's first and last tile
 // may be partial, and attention_tile_join_kernel joins those in key order.
@@ -46,8 +48,8 @@ struct TileShape {
     // behind the other's last values); with two, items follow each other like the tiles of one
     static constexpr int kQueries = D == 256 ? 1 : 2;
     static constexpr int kSlots = D == 256 ? (kCodes ? 4 : 5) : (kCodes ? 8 : 9);
-    static constexpr int kMeta = kMetaRing * (kCodes ? 2 * kTileKeys * 4 + 32 : 16);
-    static constexpr int kExchange = 2 * 2 * 128 * 4;                // between the two threads of a row
+    static constexpr int kMeta = kMetaRing * (kCodes ? 3 * kTileKeys * 4 + 16 : 16);
+    static constexpr int kExchange = (kCodes ? 2 : 1) * 2 * 2 * 128 * 4;      // between the two threads of a row
     static constexpr int kSmem = kQueries * kQuery + kSlots * kSlot + 640 + kMeta + kExchange + 4 * 128 * (kCodes ? 4 : 0);
 
     static constexpr int kPart = (D + 2) * kTileRows;                // floats of a partial result: m, l per row, [row][D]
@@ -228,9 +230,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     uint32_t* key_mask = reinterpret_cast<uint32_t*>(tail + 640);                       // [kMetaRing][4]
     float* key_scale = reinterpret_cast<float*>(tail + 640 + kMetaRing * 16);           // codes: [kMetaRing][128], by column
     float* value_scale = key_scale + kMetaRing * kTileKeys;                             // codes: [kMetaRing][128], by value row
-    float* value_top = value_scale + kMetaRing * kTileKeys;                             // codes: [kMetaRing][4]
-    float* exchange = reinterpret_cast<float*>(tail + 640 + S::kMeta);                  // [2][2][128]
-    float* query_scale = exchange + 2 * 2 * 128;                                        // codes: [4][128], by row of the block
+    float* value_log = value_scale + kMetaRing * kTileKeys;                             // codes: the same, |value scale| < 2^this
+    float* exchange = reinterpret_cast<float*>(tail + 640 + S::kMeta);                  // [2][2][128], codes: twice
+    float* query_scale = exchange + S::kExchange / 4;                                   // codes: [4][128], by row of the block
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = (int)cluster_rank();
     const int pair = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1);
@@ -538,8 +540,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         const int n = (lane >> 4) * 64 + w * 16 + (lane & 15);
                         key_scale[meta * kTileKeys + n] = ks;
                         value_scale[meta * kTileKeys + n] = vs;
-                        const float top = warp_max(fabsf(vs));
-                        if (lane == 0) value_top[meta * 4 + w] = top;
+                        value_log[meta * kTileKeys + n] = vs == 0.f ? -INFINITY : (float)((int)((__float_as_uint(vs) >> 23) & 255) - 126);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bar.keys_full[meta]);
@@ -683,7 +684,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             const int r = quarter * 32 + lane, n = rank * 128 + r;       // row of the block, of the pair
             const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
             const uint32_t o_addr = tmem + lanes;
-            float m = -INFINITY, l = 0.f, top = 0.f, qscale = fabsf(p.scale_log2);
+            float m = -INFINITY, l = 0.f, qscale = fabsf(p.scale_log2);
+            // codes: the largest log2 of weight x value scale met so far, and the power of two (less m) that such products are held by
+            float m_out = -INFINITY, k_out = 0.f;
+            auto pow2 = [](float k) { return __int_as_float((127 + (int)k) << 23); };
             bool begins = true;                                          // of this run's part of the item
             // When a wait fails the walk goes on without waiting or announcing (the two warps of a row still meet), and every sum from
             // here on is no number: the factor of the scores says so, which takes no register
@@ -727,7 +731,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 if (begins) {
                     m = -INFINITY;
                     l = 0.f;
-                    top = 0.f;
+                    m_out = -INFINITY;
+                    k_out = 0.f;
                     if (kCodes && !dead()) qscale = query_scale[(segment & 3) * 128 + r];
                     began_k = c.k;
                 }
@@ -770,23 +775,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 float most = fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
                 float* ex = exchange + (t & 1) * 256;
                 ex[half * 128 + r] = most;
+                float most_out = -INFINITY;
+                if (kCodes) {
+                    const float4* vl = reinterpret_cast<const float4*>(value_log + meta * kTileKeys + half * 64);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float4 f = vl[i];
+                        most_out = fmaxf(most_out, fmaxf(fmaxf(fmaf(s[4 * i], qscale, f.x), fmaf(s[4 * i + 1], qscale, f.y)),
+                                                         fmaxf(fmaf(s[4 * i + 2], qscale, f.z), fmaf(s[4 * i + 3], qscale, f.w))));
+                    }
+                    ex[512 + half * 128 + r] = most_out;
+                }
                 meet();                                                  // also: both have read their scores
                 most = qscale * fmaxf(most, ex[(half ^ 1) * 128 + r]);
                 float alpha = 1.f;
                 const float m_new = most > m + kLazy ? most : m;
-                if (m_new > m) alpha = m == -INFINITY ? 0.f : tile_exp2(m - m_new);
+                const bool raised = m_new > m;
+                const float fell = m - m_new;                            // log2 of what the older weights are worth now
+                if (raised) alpha = m == -INFINITY ? 0.f : tile_exp2(fell);
                 m = m_new;
-                float unit_scale = 1.f;
+                float factor = alpha;
                 if (kCodes) {
-                    const float4 vt = *reinterpret_cast<const float4*>(value_top + meta * 4);
-                    const float tile_top = fmaxf(fmaxf(vt.x, vt.y), fmaxf(vt.z, vt.w));
-                    if (tile_top > 2.f * top) {                          // the same in all rows
-                        unit_scale = top > 0.f ? top / tile_top : 0.f;
-                        top = tile_top;
+                    m_out = fmaxf(m_out, fmaxf(most_out, ex[512 + (half ^ 1) * 128 + r]));
+                    // kept within 2^kLazy of the largest product; p 2^-k_out below stays finite
+                    if (m_out > -INFINITY && (raised || m_out - m > k_out + kLazy)) {
+                        const float k = fminf(fmaxf(ceilf(m_out - m), -112.f), 112.f);
+                        if (alpha != 0.f) factor = tile_exp2((raised ? fell : 0.f) + k_out - k);
+                        k_out = k;
                     }
                 }
                 if (!begins) {
-                    const float factor = alpha * unit_scale;
                     if (__any_sync(kFull, factor != 1.f)) {              // the same in both warps of a row
                         wait_or_die(&bar.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1);
                         tc_fence_after_sync();
@@ -804,7 +822,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 // ---- weights
                 const float base = m == -INFINITY ? 0.f : m - kShift;
                 float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                const float inv_top = kCodes ? (top > 0.f ? 1.f / top : 1.f) : 1.f;
+                const float down_out = kCodes ? pow2(-k_out) : 1.f;
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
                     uint32_t w[16];
@@ -815,8 +833,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         sum[i & 3] += a + b;
                         if (kCodes) {
                             const float2 vs = *reinterpret_cast<const float2*>(value_scale + meta * kTileKeys + half * 64 + e);
-                            a *= vs.x * inv_top;
-                            b *= vs.y * inv_top;
+                            a = (a * down_out) * vs.x;                   // in this order: a weight of zero stays zero beside any scale
+                            b = (b * down_out) * vs.y;
                         }
                         w[i] = tile_pack(a, b, OT{});
                     }
@@ -841,7 +859,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                     const int tokens = c.tokens(p), cols = tokens * p.group, first_row = c.first_row(p);
                     const bool whole = ends && began_k == 0;
                     if (dead()) l = NAN;
-                    const float scale_out = dead() ? NAN : kCodes ? (top > 0.f ? top : 1.f) : 1.f;
+                    const float scale_out = dead() ? NAN : kCodes ? pow2(k_out) : 1.f;
                     const int which = at - (c.k - began_k) == run0 ? 0 : 1;
                     float* part = parts + which * (int64_t)S::kPart;
                     T* out = reinterpret_cast<T*>(p.out) + (int64_t)(first_row + tok) * p.os[0] + (int64_t)(c.head * p.group + n - tok * p.group) * p.os[1];

@@ -1,0 +1,81 @@
+"""GPU: 8-bit caches whose values differ in magnitude by far more than 16 bits hold.  A key that a row does not see, or that has no
+weight in it, takes nothing from the others, however large its value is."""
+
+import pytest
+import torch
+
+from tests import paged_oracle as O
+from tests.test_kv_cache_gpu import BF, E4, Batch
+
+pytestmark = pytest.mark.gpu
+
+# decode with and without tensor copies, a few tokens per sequence, tiles
+FORMS = [(256, 2, 8, [1, 1, 1]), (128, 8, 4, [1, 1, 1]), (64, 2, 4, [1, 1, 1]), (128, 2, 4, [2, 4, 3]), (64, 2, 4, [2, 4, 3]), (128, 2, 4, [40, 1, 90]), (256, 2, 8, [40, 1, 90])]
+
+
+def batch(dim, kv_heads, group, new, seed=1):
+    return Batch(seed, new, [300, 70, 200], kv_heads=kv_heads, heads=kv_heads * group, dim=dim, dtype=BF, cache=E4)
+
+
+def spot(b, seq, pos):
+    return O.place(b.table, b.page, b.k.shape[0], seq, pos)
+
+
+def set_key(b, pg, rw, first):
+    """A key of one element: its score is what the queries' first element makes of it."""
+    b.k[pg, :, rw] = 0.0
+    b.k[pg, :, rw, 0] = 448.0 if first >= 0 else -448.0
+    b.k_scale[pg, :, rw] = abs(first) / 448.0
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,new", FORMS)
+@pytest.mark.parametrize("exponent", [24, 31, 40, 100])
+def test_a_large_value_of_a_later_token(dim, kv_heads, group, new, exponent):
+    b = batch(dim, kv_heads, group, new)
+    for s, length in enumerate([300, 70, 200]):
+        pg, rw = spot(b, s, length - 1)
+        b.v_scale[pg, :, rw] *= 2.0 ** exponent
+    b.check(b.attend(max_query=max(new)))
+    b.check(b.attend(max_query=max(new), window=30, sinks=1), window=30, sinks=1)
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,new", FORMS)
+@pytest.mark.parametrize("exponent", [31, 40, 60])
+def test_a_large_value_of_no_weight(dim, kv_heads, group, new, exponent):
+    """Scores some 60 powers of two below the others', in an early, a middle and a late key."""
+    b = batch(dim, kv_heads, group, new)
+    b.q[:, :, 0] = 16.0
+    for s, length in enumerate([300, 70, 200]):
+        for pos in (1, length // 2, length - max(new) - 1 if length > max(new) else 2):
+            pg, rw = spot(b, s, max(pos, 1))
+            set_key(b, pg, rw, -30.0 * (dim / 128) ** 0.5)
+            b.v_scale[pg, :, rw] *= 2.0 ** exponent
+    b.check(b.attend(max_query=max(new)))
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,new", FORMS)
+def test_a_large_value_that_loses_its_weight(dim, kv_heads, group, new):
+    """The first key leads, with a large value; later ones outscore it by some 60 powers of two."""
+    b = batch(dim, kv_heads, group, new)
+    b.q[:, :, 0] = 16.0
+    for s, length in enumerate([300, 70, 200]):
+        pg, rw = spot(b, s, 0)
+        b.v_scale[pg, :, rw] *= 2.0 ** 40
+        for pos in range(length // 3, length, 7):
+            pg, rw = spot(b, s, pos)
+            set_key(b, pg, rw, 30.0 * (dim / 128) ** 0.5)
+    b.check(b.attend(max_query=max(new)))
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,new", FORMS)
+@pytest.mark.parametrize("large", [0, 60])
+def test_values_of_zero_and_values_of_all_magnitudes(dim, kv_heads, group, new, large):
+    b = batch(dim, kv_heads, group, new)
+    g = torch.Generator().manual_seed(3)
+    for s, length in enumerate([300, 70, 200]):
+        for pos in list(range(0, length // 2)) + [length - 2]:
+            pg, rw = spot(b, s, pos)
+            b.v[pg, :, rw] = 0.0
+            b.v_scale[pg, :, rw] = O.LEAST / 448.0
+    b.v_scale *= torch.exp2(large * (torch.rand(b.v_scale.shape, generator=g) - 0.5))
+    b.check(b.attend(max_query=max(new)))
