@@ -33,6 +33,10 @@ __device__ __forceinline__ void store_elem(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_elem(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_elem(__half* p, float v) { *p = __float2half_rn(v); }
 
+// Exponent by which a query row of largest magnitude `most` is brought to fp16.  Not below -126: 2^-it has to be a number, and a row of
+// subnormal elements needs no more.
+__device__ __forceinline__ int row_exponent(float most) { return most > 0.f && most < INFINITY ? max(ilogbf(most), -126) : 0; }
+
 // The sums of one row over some keys, held by a warp: lane l has the elements l, l + 32, ... of acc.
 struct RowSums {
     float m, l;

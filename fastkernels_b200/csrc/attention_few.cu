@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                     }
                 most = fmaxf(most, __shfl_xor_sync(kFull, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(kFull, most, 2));
-                const int e = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
+                const int e = row_exponent(most);
                 const float down = ldexpf(1.f, -e);
 #pragma unroll
                 for (int kk = 0; kk < kMT; ++kk)

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
 #pragma unroll
                             for (int o = kChunks / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(kFull, most, o));
-                            const int e2 = most > 0.f && most < INFINITY ? ilogbf(most) : 0;
+                            const int e2 = row_exponent(most);
                             const float down = ldexpf(1.f, -e2);
                             uint4 out;
                             uint32_t* o = reinterpret_cast<uint32_t*>(&out);

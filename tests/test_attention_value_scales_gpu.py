@@ -79,3 +79,14 @@ def test_values_of_zero_and_values_of_all_magnitudes(dim, kv_heads, group, new, 
             b.v_scale[pg, :, rw] = O.LEAST / 448.0
     b.v_scale *= torch.exp2(large * (torch.rand(b.v_scale.shape, generator=g) - 0.5))
     b.check(b.attend(max_query=max(new)))
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,new", FORMS)
+@pytest.mark.parametrize("exponent", [-126, -127, -128, -130, -133, -100, 100])
+def test_queries_of_any_magnitude(dim, kv_heads, group, new, exponent):
+    """Subnormal bf16 queries among them: their scores are all but zero, the result is nearly the mean of the values."""
+    b = batch(dim, kv_heads, group, new, seed=2)
+    heads = b.q.shape[1]
+    b.q[:, : heads // 2] = (b.q[:, : heads // 2].sign() * 2.0 ** exponent).to(BF)
+    scale = 1e-30 if exponent > 0 else None
+    b.check(b.attend(max_query=max(new), scale=scale), scale=scale)
