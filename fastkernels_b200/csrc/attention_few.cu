@@ -656,6 +656,8 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                 for (int n = 0; n < cols; ++n) row_again<T, TC>(p, cur.seq, first_row, cur.pos0, tokens, n / p.group, cur.head * p.group + n % p.group);
             }
         } else {
+            // parts are kept without the weights' factor: beside it, sums of large values would end as infinities before the division
+            constexpr float kUnshift = std::is_same<OT, __half>::value ? 0x1p-14f : 1.f;
             const int which = at == run0 ? 0 : 1;
             float* part = parts + which * S::kPart;
 #pragma unroll
@@ -667,12 +669,12 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
                     if (g == 0) {
                         float* st = stats + (warp * 2 + which) * 2 * S::kCols;
                         st[n] = m[nt][c];
-                        st[S::kCols + n] = l[nt][c];
+                        st[S::kCols + n] = l[nt][c] * kUnshift;
                     }
 #pragma unroll
                     for (int i = 0; i < kMT; ++i)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) part[2 * S::kCols + n * D + dim_of(i, h)] = acc[nt][i][c + 2 * h] * unit(nt, c);
+                        for (int h = 0; h < 2; ++h) part[2 * S::kCols + n * D + dim_of(i, h)] = acc[nt][i][c + 2 * h] * (unit(nt, c) * kUnshift);
                 }
             if (lane == 0)
                 heads[which] = PartHead{first_row, tokens, cur.head, cur.seq, cur.pos0, begins, ends, runs.worker_of(at - cur.k + cur.span.count - 1) / S::kWarps};

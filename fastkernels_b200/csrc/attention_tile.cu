@@ -221,7 +221,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     constexpr bool kCodes = S::kCodes;
     using OT = typename std::conditional<kCodes, __half, TC>::type;
     constexpr bool kHalf = std::is_same<OT, __half>::value;
-    constexpr float kShift = kHalf ? 7.f : 0.f, kLazy = 8.f - (kCodes ? 1.f : 0.f);
+    constexpr float kShift = kHalf ? 7.f : 0.f, kUnshift = kHalf ? 0x1p-7f : 1.f;       // parts are kept without the weights' factor: large values
+    constexpr float kLazy = 8.f - (kCodes ? 1.f : 0.f);
     constexpr int kSlots = S::kSlots;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t q_smem = smem_u32(smem), ring = q_smem + S::kQueries * S::kQuery;
@@ -890,7 +891,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                                 }
                             } else {
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) o[e] *= scale_out;
+                                for (int e = 0; e < 16; ++e) o[e] *= scale_out * kUnshift;
                                 store32(part + 2 * kTileRows + (int64_t)n * D + i, reinterpret_cast<const uint32_t*>(o));
                                 store32(part + 2 * kTileRows + (int64_t)n * D + i + 8, reinterpret_cast<const uint32_t*>(o + 8));
                             }
@@ -903,7 +904,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                         // the join kernel sees to rows whose result is not finite: nothing here waits for that
                         if (odd && l == l && tokens > 1) bar.odd = 1;
                     } else {
-                        if (n < cols && half == 0) { part[n] = m; part[kTileRows + n] = l; }
+                        if (n < cols && half == 0) { part[n] = m; part[kTileRows + n] = l * kUnshift; }
                         if (rank == 0 && threadIdx.x == 0)
                             heads[which] = PartHead{first_row, tokens, c.head, c.seq, c.pos0, began_k == 0, ends, runs.worker_of(at - c.k + c.span.count - 1)};
                     }

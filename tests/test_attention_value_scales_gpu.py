@@ -90,3 +90,11 @@ def test_queries_of_any_magnitude(dim, kv_heads, group, new, exponent):
     b.q[:, : heads // 2] = (b.q[:, : heads // 2].sign() * 2.0 ** exponent).to(BF)
     scale = 1e-30 if exponent > 0 else None
     b.check(b.attend(max_query=max(new), scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,new", FORMS)
+def test_large_values_stay_finite(dim, kv_heads, group, new):
+    """Values up to 2^115: sums over 300 keys stay below 2^124, in whole items and in parts, as long as no factor is left in them."""
+    b = batch(dim, kv_heads, group, new, seed=4)
+    b.v_scale *= 2.0 ** 115 / (448.0 * b.v_scale.max())
+    b.check(b.attend(max_query=max(new)))
