@@ -296,6 +296,8 @@ class PagedKVCache:
             raise ValueError(f"the cache must be float32, bfloat16, float16 or float8_e4m3fn, got {dtype}")
         if min(pages, kv_heads, seqs, page_size) < 1 or not 1 <= head_dim <= _lib.MAX_HEAD_DIM:
             raise ValueError(f"pages, kv_heads, seqs and page_size must be positive, head_dim between 1 and {_lib.MAX_HEAD_DIM}")
+        if pages * page_size >= (1 << 31) - 1024 or kv_heads > 1024:          # every append would be refused
+            raise ValueError("the cache must hold less than 2^31 - 1024 positions, with at most 1024 heads")
         shape = (pages, kv_heads, page_size, head_dim)
         self.key, self.value = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if dtype == torch.float8_e4m3fn
                                 else torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
@@ -332,9 +334,12 @@ class PagedKVCache:
         new = [1] * self.seqs if new is None else [int(n) for n in new]
         if len(new) != self.seqs or min(new) < 0 or sum(new) != key.shape[0]:
             raise ValueError("new must name each sequence's number of rows, with key's rows as their sum")
-        row = (self.key.shape[1], self.key.shape[3])
-        if key.shape[1:] != row or value.shape != key.shape:
-            raise ValueError(f"key and value must have shape [rows, {row[0]}, {row[1]}]")
+        # all refusals before the sequences grow: a refused call leaves the cache as it was
+        if not self.key.is_cuda:
+            raise ValueError("the cache must be on a CUDA device")
+        code = _check_rows(key, "key", key.shape[0], self.key.shape[1], self.key.shape[3], self.key)
+        if code != _check_rows(value, "value", key.shape[0], self.key.shape[1], self.key.shape[3], self.key):
+            raise ValueError("key and value must have the same dtype")
         self._grow(new)
         starts = [0]
         for n in new:

@@ -112,3 +112,17 @@ def test_oracle_e4m3_is_the_nearest_code():
     dist = (x.unsqueeze(1) - codes).abs()
     assert torch.equal((got - x).abs(), dist.min(1).values)
     assert torch.equal(got, x.float().to(torch.float8_e4m3fn).double())       # ties to even as the type's own conversion takes them
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+def test_a_refused_append_leaves_the_cache_as_it_was(dtype):
+    c = fk.PagedKVCache(4, 2, 64, device="cpu", dtype=dtype)
+    rows = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    for key, value, new in ((rows.float(), rows, [3]), (rows, rows.half(), [3]), (rows.int(), rows.int(), [3]), (rows, rows[:2], [3]), (rows[:, :1], rows[:, :1], [3]),
+                            (rows, rows, [2]), (rows, rows, [-3]), (rows, rows, [3, 0]), (rows.transpose(1, 2).contiguous().transpose(1, 2), rows, [3]), (rows, rows, [3])):
+        with pytest.raises(ValueError):
+            c.append(key, value, new)
+        assert c.host_lengths == [0] and c.lengths.tolist() == [0] and (c.page_table == -1).all() and len(c._free) == 4 and c._starts is None
+    for shape in ((2 ** 20, 1, 1, 2 ** 11), (4, 1025, 1, 16)):                 # caches that no append would take
+        with pytest.raises(ValueError, match="positions"):
+            fk.PagedKVCache(*shape[:3], page_size=shape[3], device="cpu", dtype=dtype)
