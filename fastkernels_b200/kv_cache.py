@@ -24,6 +24,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import struct
+from collections import deque
 from typing import Any, Optional
 
 import torch
@@ -282,12 +283,17 @@ def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: An
     return out
 
 
+_PAGES_AT_ONCE = 4096          # entries of the page table in one copy
+
+
 class PagedKVCache:
     """One layer's paged cache for a fixed number of sequences, with the pages handed out as the sequences grow.
 
     `append` writes each sequence's new tokens and grows it, `attend` runs their attention, `read` returns whole
     sequences, `release` gives a sequence's pages back.  The lengths live on the host as well, so that growing a sequence
-    needs no synchronisation; the page table and the lengths on the device are updated by copies on the current stream.
+    needs no synchronisation; the page table and the lengths on the device are updated by asynchronous copies out of pinned
+    memory on the current stream, in place.  What grows on the host cannot be captured in a graph (a replay would write to the
+    same positions again): `append`, `read` and `release` are refused there, `attend` and the three functions are not.
     """
 
     def __init__(self, pages: int, kv_heads: int, head_dim: int, *, seqs: int = 1, page_size: int = 16,
@@ -309,28 +315,69 @@ class PagedKVCache:
         self._owned: list[list[int]] = [[] for _ in range(seqs)]
         self._free = list(range(pages - 1, -1, -1))
         self.page_table = torch.full((seqs, pages), -1, dtype=torch.int32, device=self.key.device)
-        self.lengths = torch.zeros(seqs, dtype=torch.int32, device=self.key.device)
+        # lengths and starts next to each other: one copy brings both
+        self._state = torch.zeros(2 * seqs + 1, dtype=torch.int32, device=self.key.device)
+        self.lengths = self._state[:seqs]
         self._starts: Any = None
         self._new = [0] * seqs
+        # some 32 appends of 64 pages, and never less than one of the largest copies
+        self._ring = torch.zeros(max(32 * (96 + seqs + 1), 2 * _PAGES_AT_ONCE), dtype=torch.int64, pin_memory=self.key.is_cuda)
+        self._ring_at, self._copies = 0, deque()
 
     def _scales(self) -> dict:
         return {"key_scale": self.key_scale, "value_scale": self.value_scale}
+
+    def _to_device(self, values, dtype: torch.dtype, into: Any = None):
+        """`values` on the device by a copy on the current stream that the host does not wait for.  They are put down in a ring of
+        pinned words made once (pinning more while the device works would wait for it); only if the host is a whole ring ahead it waits for
+        the oldest copy."""
+        size = (len(values) * dtype.itemsize + 7) // 8
+        if self._ring_at + size > self._ring.numel():            # back to the front, behind what the lap before left at the end
+            while self._copies and self._copies[0][0] >= self._ring_at:
+                self._copies.popleft()[1].synchronize()
+            self._ring_at = 0
+        first, last = self._ring_at, self._ring_at + size
+        while self._copies and first <= self._copies[0][0] < last:
+            self._copies.popleft()[1].synchronize()
+        pinned = self._ring[first:last].view(dtype)[:len(values)]
+        pinned.copy_(torch.tensor(values, dtype=dtype))
+        self._ring_at = last
+        out = torch.empty(len(values), dtype=dtype, device=self.key.device) if into is None else into
+        out.copy_(pinned, non_blocking=True)
+        over = torch.cuda.Event()
+        over.record()
+        self._copies.append((first, over))
+        return out
+
+    def _not_captured(self, what: str) -> None:
+        if self.key.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(f"{what} changes or reads lengths on the host and cannot be captured in a graph")
 
     def _grow(self, new) -> None:
         need = [-(-(n + m) // self.page_size) - len(own) for n, m, own in zip(self.host_lengths, new, self._owned)]
         if sum(max(0, n) for n in need) > len(self._free):
             raise ValueError("the cache has no pages left for these tokens")
+        at, pages, width = [], [], self.page_table.shape[1]
         for s, n in enumerate(need):
             if n > 0:
                 got = [self._free.pop() for _ in range(n)]
-                at = len(self._owned[s])
+                first = s * width + len(self._owned[s])
+                at += range(first, first + n)
+                pages += got
                 self._owned[s] += got
-                self.page_table[s, at:at + n] = torch.tensor(got, dtype=torch.int32, device=self.key.device)
+        for i in range(0, len(pages), _PAGES_AT_ONCE):
+            part = slice(i, i + _PAGES_AT_ONCE)
+            self.page_table.view(-1).index_copy_(0, self._to_device(at[part], torch.int64), self._to_device(pages[part], torch.int32))
         self.host_lengths = [n + m for n, m in zip(self.host_lengths, new)]
-        self.lengths.copy_(torch.tensor(self.host_lengths, dtype=torch.int32))
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        self._to_device(self.host_lengths + starts, torch.int32, self._state)
+        self._new, self._starts = new, self._state[self.seqs:]
 
     def append(self, key: Any, value: Any, new=None) -> None:
         """`key`, `value` `[rows, kv_heads, head_dim]`: `new[s]` rows for each sequence in turn (default: one each)."""
+        self._not_captured("append")
         new = [1] * self.seqs if new is None else [int(n) for n in new]
         if len(new) != self.seqs or min(new) < 0 or sum(new) != key.shape[0]:
             raise ValueError("new must name each sequence's number of rows, with key's rows as their sum")
@@ -340,11 +387,8 @@ class PagedKVCache:
         code = _check_rows(key, "key", key.shape[0], self.key.shape[1], self.key.shape[3], self.key)
         if code != _check_rows(value, "value", key.shape[0], self.key.shape[1], self.key.shape[3], self.key):
             raise ValueError("key and value must have the same dtype")
-        self._grow(new)
-        starts = [0]
-        for n in new:
-            starts.append(starts[-1] + n)
-        self._new, self._starts = new, torch.tensor(starts, dtype=torch.int32, device=self.key.device)
+        with _On(self.key.device):
+            self._grow(new)
         paged_kv_append(key, value, self.key, self.value, self.page_table, self.lengths, self._starts, **self._scales())
 
     def attend(self, query: Any, *, scale: Optional[float] = None, window: int = 0, sinks: int = 0):
@@ -356,14 +400,17 @@ class PagedKVCache:
 
     def read(self, dtype: Optional[torch.dtype] = None):
         """Every sequence whole: `(key, value)` `[sum of lengths, kv_heads, head_dim]`, one sequence after the other."""
+        self._not_captured("read")
         starts = [0]
         for n in self.host_lengths:
             starts.append(starts[-1] + n)
-        return paged_kv_gather(self.key, self.value, self.page_table, self.lengths, torch.tensor(starts, dtype=torch.int32, device=self.key.device),
-                               starts[-1], dtype=dtype, **self._scales())
+        with _On(self.key.device):
+            at = self._to_device(starts, torch.int32)
+        return paged_kv_gather(self.key, self.value, self.page_table, self.lengths, at, starts[-1], dtype=dtype, **self._scales())
 
     def release(self, seq: int) -> None:
         """Empty one sequence and give its pages back."""
+        self._not_captured("release")
         self._free += reversed(self._owned[seq])
         self._owned[seq] = []
         self.host_lengths[seq] = 0
