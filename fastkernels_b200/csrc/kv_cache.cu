@@ -10,7 +10,8 @@
 // exactly there.  q = x r with r = 1 / max, then q + (x - q max) r (one step of Newton's iteration with the exact residual of a
 // fused multiply-add; P. Markstein, IBM J. Res. Dev. 34, 1990): where x / max is a number of few bits the step lands on it, since
 // what it adds is off by 2^-24 of the residual only.  A divide per element costs three times as many instructions and bounds the
-// kernel instead of HBM.
+// kernel instead of HBM.  Elements of 24 bits leave quotients that round to such a middle without lying on it (a few in ten million): theirs
+// are rounded to odd, the residual telling the side, so that the second rounding, to the code, sees where they were.
 
 #include "kv_cache.cuh"
 
@@ -163,6 +164,20 @@ __device__ __forceinline__ RowAt row_at(const KvParams& p, int row) {
     return a;
 }
 
+// x * 448 / most to 24 bits, rounded to odd where they do not hold it: the rounding to a code that follows sees on which side of a middle
+// the quotient lies.
+__device__ __forceinline__ void nearest_quotients(float most, float (&v)[kPiece]) {
+    const float lift = most < 0x1p-40f ? 0x1p60f : 1.f;            // residuals stay above the least fp32 number
+    const float b = most * lift * 0x1p-9f, inv = 1.0f / b;
+#pragma unroll
+    for (int i = 0; i < kPiece; ++i) {
+        const float y = v[i] * lift, x = y * 0.875f, rest = fmaf(y, 0.875f, -x), q0 = x * inv;
+        const float q = fmaf(fmaf(-q0, b, x) + rest, inv, q0), r = fmaf(-q, b, x) + rest;
+        const uint32_t bits = __float_as_uint(q);
+        v[i] = r == 0.f || q == 0.f ? q : __uint_as_float(((r < 0.f) != (q < 0.f) ? bits - 1 : bits) | 1u);
+    }
+}
+
 template <typename T, typename TC, Access A>
 __global__ void __launch_bounds__(kRowThreads) kv_append_kernel(const __grid_constant__ KvParams p) {
     __shared__ int2 place[kMostTokens];
@@ -203,11 +218,23 @@ __global__ void __launch_bounds__(kRowThreads) kv_append_kernel(const __grid_con
                 most = max_nan(most, 0x1p-100f);
                 // 448 = 0.875 * 2^9: the factors are split so that nothing overflows
                 const float b = most * 0x1p-9f, inv = 1.0f / b;
+                uint32_t middle = 0xffffffffu;           // fp32 rows: steps from two below a middle between codes to the quotient next to it
+                float least = INFINITY;
 #pragma unroll
                 for (int i = 0; i < kPiece; ++i) {
                     const float x = v[i] * 0.875f, q = x * inv;
                     v[i] = fmaf(fmaf(-q, b, x), inv, q);
+                    if constexpr (sizeof(T) == 4) {
+                        middle = min(middle, (__float_as_uint(v[i]) - 0x7fffeu) & 0xfffffu);
+                        least = fminf(least, fabsf(v[i]));
+                    }
                 }
+                // off by two steps of 2^-23 at most.  Below 2^-6 the middles lie closer together
+                if constexpr (sizeof(T) == 4)
+                    if (middle < 5 || !(least >= 0x1p-6f) || most < 0x1p-40f) {
+                        raw[a].values(v);
+                        nearest_quotients(most, v);
+                    }
                 if (to_page.x < 0) continue;
                 if (d0 == 0) {
                     const int64_t* ts = at.value ? p.c.value_scale_stride : p.c.key_scale_stride;
