@@ -199,6 +199,8 @@ __global__ void __launch_bounds__(32 * kAnyWarps) attention_any_join_kernel(cons
         if (c * 32 + lane < D) store_elem(out + c * 32 + lane, l == 0.f ? 0.f : acc[c] / l);
 }
 
+constexpr double kLog2E = 1.4426950408889634;
+
 static int check_attention(const fk_attention_call* a) {
     if (a == nullptr) return FK_ERR_ARG;
     const int st = check_cache(a->cache);
@@ -208,7 +210,7 @@ static int check_attention(const fk_attention_call* a) {
     if (a->rows < 0 || a->q_heads < 1 || a->q_heads % a->cache.kv_heads != 0) return FK_ERR_ARG;
     if ((int64_t)a->rows * a->q_heads > INT32_MAX || a->window < 0 || a->sinks < 0 || a->max_query < 0) return FK_ERR_ARG;
     if (a->rows > 0 && (!a->query || !a->out)) return FK_ERR_ARG;
-    if (!(a->scale == a->scale) || a->scale - a->scale != 0.f) return FK_ERR_ARG;      // NaN or infinite
+    if (!(fabs((double)a->scale) * kLog2E <= FLT_MAX)) return FK_ERR_ARG;      // NaN, infinite, or infinite as a power of two
     return FK_OK;
 }
 
@@ -251,7 +253,7 @@ static AttnParams attn_params(const fk_attention_call& a) {
     for (int i = 0; i < 2; ++i) { p.qs[i] = a.query_stride[i]; p.os[i] = a.out_stride[i]; }
     p.rows = a.rows; p.q_heads = a.q_heads; p.group = a.q_heads / a.cache.kv_heads;
     p.window = a.window; p.sinks = a.window > 0 ? a.sinks : 0; p.zero_rest = a.zero_rest;
-    p.scale_log2 = (float)((double)a.scale * 1.4426950408889634);
+    p.scale_log2 = (float)((double)a.scale * kLog2E);
     if (fabsf(p.scale_log2) < FLT_MIN) p.scale_log2 = FLT_MIN;
     p.part = reinterpret_cast<float*>(a.workspace);
     p.wait_cycles = (uint32_t)std::min(wait_limit_cycles(), 1ll << 31);       // clocks are compared in 32 bits

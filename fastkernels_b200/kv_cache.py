@@ -43,6 +43,7 @@ _ROW_FIELDS = "2Q4i4qQ"
 _CALL_FIELDS = "2Q4i4qQf3iIi2Q"
 _PACK_CACHE, _PACK_ROWS, _PACK_CALL = (struct.Struct("=" + f) for f in (_CACHE_FIELDS, _ROW_FIELDS, _CALL_FIELDS))
 _CACHE_BYTES = C.sizeof(KvCache)
+_FP32_MAX = torch.finfo(torch.float32).max
 assert (_PACK_CACHE.size, _PACK_ROWS.size, _PACK_CALL.size) == (_CACHE_BYTES, C.sizeof(KvRows), C.sizeof(AttentionCall) - _CACHE_BYTES)
 
 
@@ -257,8 +258,8 @@ def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: An
         raise ValueError("window and sinks must be below 2^31")
     if scale is None:
         scale = dim ** -0.5
-    elif not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    elif not abs(scale) * math.log2(math.e) <= _FP32_MAX:
+        raise ValueError("scale must be finite, in fp32 and times log2(e)")
     device, fresh = query.device, out is None
     lib = _lib.load()
     with _On(device):

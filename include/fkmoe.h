@@ -294,7 +294,7 @@ typedef struct fk_attention_call {
     int32_t max_query;                 /* most rows of one sequence, or 0 if not known: it chooses between kernels, no result depends on it */
     int64_t query_stride[2], out_stride[2];              /* row, head; in elements */
     const int32_t* starts;
-    float scale;                       /* of the scores */
+    float scale;                       /* of the scores; scale * log2(e) must be finite */
     int32_t window;                    /* > 0: a token sees the last `window` positions up to its own, and the first `sinks`; 0: all up to its own */
     int32_t sinks;
     int32_t zero_rest;                 /* also write zeros to the rows behind the last sequence (otherwise they are left alone) */

@@ -126,3 +126,10 @@ def test_a_refused_append_leaves_the_cache_as_it_was(dtype):
     for shape in ((2 ** 20, 1, 1, 2 ** 11), (4, 1025, 1, 16)):                 # caches that no append would take
         with pytest.raises(ValueError, match="positions"):
             fk.PagedKVCache(*shape[:3], page_size=shape[3], device="cpu", dtype=dtype)
+
+
+@pytest.mark.parametrize("scale,status", [(2.4e38, ARG), (-2.4e38, ARG), (3.4e38, ARG), (2.35e38, WORKSPACE), (-2.35e38, WORKSPACE)])
+def test_scales_at_the_end_of_fp32(scale, status):
+    """Scores are held as powers of two: the scale times log2(e) has to be a number."""
+    a = AttentionCall(cache=cache(max_pages=1000, table_stride=1000), query=4096, out=4096, dtype=_lib.FK_BF16, rows=3, q_heads=4, scale=scale)
+    assert _lib.load().fk_paged_attention(C.byref(a), None) == status

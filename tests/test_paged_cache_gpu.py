@@ -98,3 +98,13 @@ def test_an_append_after_a_refused_one():
     fresh = fk.PagedKVCache(20, 2, 128, seqs=2)
     fresh.append(k, v, [2, 3])
     assert torch.equal(c.attend(q), fresh.attend(q)) and torch.equal(c.read()[0], k)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 2.4e38, float("inf"), float("nan")])
+def test_scales_that_fp32_does_not_hold_are_refused(scale):
+    c = fk.PagedKVCache(4, 2, 128)
+    k, q = rows(1, gen(5)), rows(1, gen(5), 4)
+    c.append(k, k)
+    with pytest.raises(ValueError, match="finite"):
+        c.attend(q, scale=scale)
+    assert torch.equal(c.attend(q), c.attend(q, scale=128 ** -0.5))
