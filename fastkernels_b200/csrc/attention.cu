@@ -222,7 +222,7 @@ static int64_t any_blocks(const fk_attention_call& a) {
 // Pieces of the key axis: enough blocks for the whole chip (8 per SM) where there are few rows, none shorter than 64 keys.
 static int any_splits(const fk_attention_call& a) {
     const int64_t blocks = any_blocks(a), longest = (int64_t)a.cache.max_pages * a.cache.page_size;
-    int64_t want = (148 * 8 + blocks - 1) / blocks;
+    int64_t want = ((int64_t)sm_count() * 8 + blocks - 1) / blocks;
     if (want > (longest + 63) / 64) want = (longest + 63) / 64;
     if (want > 64) want = 64;
     return want < 1 ? 1 : (int)want;
@@ -230,11 +230,13 @@ static int any_splits(const fk_attention_call& a) {
 
 template <typename T, typename TC>
 static int launch_any(const AttnParams& p, int64_t blocks, bool wide, cudaStream_t stream) {
-    auto pick = [&](auto few, auto some, auto all) { return p.c.head_dim <= 64 ? few : p.c.head_dim <= 128 ? some : all; };
+    const int columns = p.c.head_dim <= 64 ? 0 : p.c.head_dim <= 128 ? 1 : 2;
+    auto pick = [&](auto few, auto some, auto all) { return columns == 0 ? few : columns == 1 ? some : all; };
     auto kern = wide ? pick(attention_any_kernel<T, TC, true, 2>, attention_any_kernel<T, TC, true, 4>, attention_any_kernel<T, TC, true, 8>)
                      : pick(attention_any_kernel<T, TC, false, 2>, attention_any_kernel<T, TC, false, 4>, attention_any_kernel<T, TC, false, 8>);
     const int heads = p.group < kAnyWarps * kAnyHeads ? p.group : kAnyWarps * kAnyHeads, smem = any_smem(p.c.head_dim, heads);
-    FK_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, any_smem(FK_MAX_HEAD_DIM, kAnyWarps * kAnyHeads)), "attention attr");
+    static std::atomic<uint64_t> allowed[2][3];
+    FK_CUDA_OK(allow_smem(kern, any_smem(FK_MAX_HEAD_DIM, kAnyWarps * kAnyHeads), allowed[wide][columns]), "attention attr");
     FK_CUDA_OK(launch_pdl(kern, dim3((unsigned)(blocks * p.splits)), dim3(32 * kAnyWarps), (size_t)smem, stream, p), "attention launch");
     FK_LAUNCH_OK("attention launch");
     if (p.splits > 1) {

@@ -13,6 +13,7 @@
 // kernel instead of HBM.  Elements of 24 bits leave quotients that round to such a middle without lying on it (a few in ten million): theirs
 // are rounded to odd, the residual telling the side, so that the second rounding, to the code, sees where they were.
 
+#include "kernels.cuh"
 #include "kv_cache.cuh"
 
 namespace fk {
@@ -345,7 +346,7 @@ static int kv_rows(const fk_kv_cache* cache, const fk_kv_rows* rows, void* strea
     while ((kPiece << p.group_log2) < cache->head_dim) ++p.group_log2;
     // Tokens per block: as many as leave four blocks for every SM and a turn of the loop for a block
     const int64_t token_items = (int64_t)(2 * cache->kv_heads) << p.group_log2;
-    while (p.block_tokens < kMostTokens && p.block_tokens * token_items < kRowThreads * kAhead && rows->rows / (2 * p.block_tokens) >= 4 * 148) p.block_tokens *= 2;
+    while (p.block_tokens < kMostTokens && p.block_tokens * token_items < kRowThreads * kAhead && rows->rows / (2 * p.block_tokens) >= 4 * sm_count()) p.block_tokens *= 2;
     cudaStream_t s = (cudaStream_t)stream;
     if (cache->dtype == FK_E4M3) {
         if (rows->dtype == FK_BF16) return launch_rows<APPEND, __nv_bfloat16, __nv_fp8_e4m3>(p, s);
