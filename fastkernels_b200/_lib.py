@@ -54,7 +54,7 @@ class EpComm(C.Structure):          # struct fk_ep_comm
                 ("base", C.c_void_p * EP_MAX_RANKS), ("bytes", C.c_size_t)]
 
 
-MAX_HEAD_DIM = 256
+MAX_HEAD_DIM, MAX_KV_HEADS = 256, 1024
 
 
 class KvCache(C.Structure):         # struct fk_kv_cache

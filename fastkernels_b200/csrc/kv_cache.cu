@@ -340,7 +340,7 @@ static int kv_rows(const fk_kv_cache* cache, const fk_kv_rows* rows, void* strea
     if (st != FK_OK) return st;
     st = check_rows(*cache, *rows);
     if (st != FK_OK) return st;
-    if (cache->kv_heads > 1024) return FK_ERR_UNSUPPORTED;      // row numbers of a block stay below 2^16
+    if (cache->kv_heads > FK_MAX_KV_HEADS) return FK_ERR_UNSUPPORTED;      // row numbers of a block stay below 2^16
     if (rows->rows == 0 || (cache->seqs == 0 && (APPEND || !rows->zero_rest))) return FK_OK;
     KvParams p{*cache, *rows, 0, 1, (uint32_t)((1ull << 32) / (2 * cache->kv_heads) + 1)};
     while ((kPiece << p.group_log2) < cache->head_dim) ++p.group_log2;

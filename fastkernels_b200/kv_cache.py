@@ -16,7 +16,7 @@ int32 `[seqs + 1]`: rows `query_starts[s] .. query_starts[s+1]-1` of a call are 
 (`None`: one token per sequence).  All of it is read on the device; nothing synchronises, so calls can be captured in a
 CUDA graph and replayed with other lengths.  Page numbers outside the cache (-1 for a page that was given back, say)
 are safe: such tokens are skipped, read as zeros, or not visible.  A position must not be mapped to a page that another
-position of the same call writes.  No gradients.
+position of the same call writes.  Writing and reading back take caches of at most 1024 heads.  No gradients.
 """
 
 from __future__ import annotations
@@ -144,6 +144,11 @@ def _check_rows(t: Any, what: str, rows: int, heads: int, dim: int, key_cache) -
     return code
 
 
+def _check_heads(heads: int) -> None:
+    if heads > _lib.MAX_KV_HEADS:
+        raise ValueError(f"the cache must have at most {_lib.MAX_KV_HEADS} heads to be written or read back")
+
+
 def _span(t: Any) -> tuple[int, int]:
     """First and one-past-last byte that a tensor can touch."""
     if t.numel() == 0:
@@ -185,6 +190,7 @@ def paged_kv_append(key: Any, value: Any, key_cache: Any, value_cache: Any, page
     """
     c, r = KvCache(), KvRows()
     heads, dim, _ = _pack_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    _check_heads(heads)
     rows = key.shape[0]
     code = _check_rows(key, "key", rows, heads, dim, key_cache)
     if code != _check_rows(value, "value", rows, heads, dim, key_cache):
@@ -205,6 +211,7 @@ def paged_kv_gather(key_cache: Any, value_cache: Any, page_table: Any, lengths: 
     """
     c, r = KvCache(), KvRows()
     heads, dim, _ = _pack_cache(c, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)
+    _check_heads(heads)
     if rows < 0:
         raise ValueError("rows must not be negative")
     if dtype is None:
@@ -303,8 +310,8 @@ class PagedKVCache:
             raise ValueError(f"the cache must be float32, bfloat16, float16 or float8_e4m3fn, got {dtype}")
         if min(pages, kv_heads, seqs, page_size) < 1 or not 1 <= head_dim <= _lib.MAX_HEAD_DIM:
             raise ValueError(f"pages, kv_heads, seqs and page_size must be positive, head_dim between 1 and {_lib.MAX_HEAD_DIM}")
-        if pages * page_size >= (1 << 31) - 1024 or kv_heads > 1024:          # every append would be refused
-            raise ValueError("the cache must hold less than 2^31 - 1024 positions, with at most 1024 heads")
+        if pages * page_size >= (1 << 31) - 1024 or kv_heads > _lib.MAX_KV_HEADS:          # every append would be refused
+            raise ValueError(f"the cache must hold less than 2^31 - 1024 positions, with at most {_lib.MAX_KV_HEADS} heads")
         shape = (pages, kv_heads, page_size, head_dim)
         self.key, self.value = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) if dtype == torch.float8_e4m3fn
                                 else torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))

@@ -257,6 +257,7 @@ int fk_moe_layer_residual(const fk_moe_call* c, const float* resid_in, const flo
  * back as NaN.
  * --------------------------------------------------------------------------------------------- */
 #define FK_MAX_HEAD_DIM 256
+#define FK_MAX_KV_HEADS 1024           /* fk_kv_append, fk_kv_gather; FK_ERR_UNSUPPORTED above */
 
 typedef struct fk_kv_cache {
     int32_t pages, kv_heads, page_size, head_dim;

@@ -108,3 +108,18 @@ def test_scales_that_fp32_does_not_hold_are_refused(scale):
     with pytest.raises(ValueError, match="finite"):
         c.attend(q, scale=scale)
     assert torch.equal(c.attend(q), c.attend(q, scale=128 ** -0.5))
+
+
+def test_more_heads_than_a_block_counts_are_refused():
+    cache = [torch.zeros(2, 1025, 1, 8, device="cuda", dtype=BF) for _ in range(2)]
+    where = (torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda"))
+    row = torch.zeros(1, 1025, 8, device="cuda", dtype=BF)
+    with pytest.raises(ValueError, match="at most 1024 heads"):
+        fk.paged_kv_append(row, row, *cache, *where)
+    with pytest.raises(ValueError, match="at most 1024 heads"):
+        fk.paged_kv_gather(*cache, *where, None, 1)
+    assert (fk.paged_attention(row, *cache, *where) == 0).all()          # the attention takes them
+    fit = [t[:, :1024].contiguous() for t in cache]
+    ones = torch.ones(1, 1024, 8, device="cuda", dtype=BF)
+    fk.paged_kv_append(ones, ones, *fit, *where)
+    assert all((t == 1).all() for t in fk.paged_kv_gather(*fit, *where, None, 1)) and (fit[0][1] == 0).all()
