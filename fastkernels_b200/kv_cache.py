@@ -149,6 +149,13 @@ def _check_heads(heads: int) -> None:
         raise ValueError(f"the cache must have at most {_lib.MAX_KV_HEADS} heads to be written or read back")
 
 
+def _check_written(a: Any, b: Any, what: str) -> None:
+    """Refuses tensors to be written whose elements share memory (expanded ones): several threads would write to one place."""
+    for t in (a, b):
+        if 0 in t.stride() and any(stride == 0 and n > 1 for n, stride in zip(t.shape, t.stride())):
+            raise ValueError(f"{what} must not be expanded: every element needs a place of its own")
+
+
 def _span(t: Any) -> tuple[int, int]:
     """First and one-past-last byte that a tensor can touch."""
     if t.numel() == 0:
@@ -195,6 +202,7 @@ def paged_kv_append(key: Any, value: Any, key_cache: Any, value_cache: Any, page
     code = _check_rows(key, "key", rows, heads, dim, key_cache)
     if code != _check_rows(value, "value", rows, heads, dim, key_cache):
         raise ValueError("key and value must have the same dtype")
+    _check_written(key_cache, value_cache, "key_cache and value_cache")
     _pack_rows(r, key, value, code, query_starts, False)
     device = key_cache.device
     with _On(device):
@@ -227,6 +235,7 @@ def paged_kv_gather(key_cache: Any, value_cache: Any, page_table: Any, lengths: 
         _check_rows(value, "value" if out is None else "out[1]", rows, heads, dim, key_cache)
         if key.dtype != dtype or value.dtype != dtype:
             raise ValueError(f"out must have dtype {dtype}")
+        _check_written(key, value, "out")
         if out is not None and (_overlap(key, value) or any(_overlap(a, b) for a in out for b in (key_cache, value_cache))):
             raise ValueError("out must not overlap the cache, nor its two tensors each other")
         _pack_rows(r, key, value, code, query_starts, out is None)
@@ -275,6 +284,7 @@ def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: An
         else:
             if _check_rows(out, "out", rows, q_heads, dim, key_cache) != code:
                 raise ValueError("out must have the query's dtype")
+            _check_written(out, out, "out")
             if any(_overlap(out, t) for t in (query, key_cache, value_cache)):
                 raise ValueError("out must not overlap the query or the cache")
         q0, q1, _ = query.stride()

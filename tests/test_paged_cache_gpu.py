@@ -123,3 +123,26 @@ def test_more_heads_than_a_block_counts_are_refused():
     ones = torch.ones(1, 1024, 8, device="cuda", dtype=BF)
     fk.paged_kv_append(ones, ones, *fit, *where)
     assert all((t == 1).all() for t in fk.paged_kv_gather(*fit, *where, None, 1)) and (fit[0][1] == 0).all()
+
+
+def test_expanded_tensors_are_read_and_not_written():
+    """Rows, queries and caches that repeat one element's memory are fine to read; as outputs they are refused."""
+    g = gen(6)
+    cache = [torch.zeros(3, 2, 16, 128, device="cuda", dtype=BF) for _ in range(2)]
+    where = (torch.tensor([[2, 0]], dtype=torch.int32, device="cuda"), torch.tensor([4], dtype=torch.int32, device="cuda"), torch.tensor([0, 4], dtype=torch.int32, device="cuda"))
+    one = rows(1, g)
+    fk.paged_kv_append(one.expand(4, 2, 128), one.expand(4, 2, 128), *cache, *where)
+    got = fk.paged_kv_gather(*cache, *where, 4)
+    assert torch.equal(got[0], one.expand(4, 2, 128)) and torch.equal(got[1], got[0])
+    q = rows(1, g, 4)
+    out = fk.paged_attention(q.expand(4, 4, 128), *cache, *where)
+    want = one.repeat_interleave(2, dim=1).expand(4, 4, 128)
+    assert ((out - want).abs() <= 2.0 ** -7 * want.abs()).all()          # equal values: one rounding of the weights, one of the result
+    wide = [t[:, :1].expand(3, 2, 16, 128) for t in cache]
+    fk.paged_attention(q.expand(4, 4, 128), *wide, *where)
+    empty = torch.zeros(1, 4, 128, device="cuda", dtype=BF)
+    for call in (lambda: fk.paged_kv_append(one.expand(4, 2, 128), one.expand(4, 2, 128), *wide, *where),
+                 lambda: fk.paged_kv_gather(*cache, *where, 4, out=(empty[:, :2].expand(4, 2, 128), got[1])),
+                 lambda: fk.paged_attention(q.expand(4, 4, 128), *cache, *where, out=empty.expand(4, 4, 128))):
+        with pytest.raises(ValueError, match="expanded"):
+            call()
