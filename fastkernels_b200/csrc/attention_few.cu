@@ -322,7 +322,10 @@ __global__ void __launch_bounds__(32 * FewShape<D, NT, TC>::kWarps, 1) attention
     // the oldest slot has landed for the whole warp, and the one before it is free
     auto next_slot = [&](bool issue_values) {
         if (TMA) {
-            if (left >= 0 && !warp_wait(&landed[slot], phase, abort_flag, p.wait_cycles)) left = -1;       // nothing more is issued or waited for
+            if (left >= 0 && !warp_wait(&landed[slot], phase, abort_flag, p.wait_cycles)) {
+                left = -1;                       // nothing more is issued or waited for
+                *abort_flag = 1;
+            }
         } else asm volatile("cp.async.wait_group %0;" ::"n"(kSlots - 2) : "memory");
         if (TMA && zeroed) fence_async_proxy();
         zeroed = false;

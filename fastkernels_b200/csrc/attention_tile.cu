@@ -64,7 +64,7 @@ struct TileBarriers {
     uint64_t q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], o_empty;
     uint64_t keys_full[kMetaRing];
     uint32_t tmem;
-    int abort_flag, odd;
+    int abort_flag, odd, walked;
 };
 static_assert(sizeof(TileBarriers) <= 640, "fits behind the ring");
 
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             mbar_init(&bar.o_done[i], 1); mbar_init(&bar.s_full[i], 1); mbar_init(&bar.p_full[i], 16); }
         mbar_init(&bar.o_empty, 16);
         for (int i = 0; i < kMetaRing; ++i) mbar_init(&bar.keys_full[i], TMA ? 1 : 4);
-        bar.abort_flag = bar.odd = 0;
+        bar.abort_flag = bar.odd = bar.walked = 0;
         mbar_init_fence();
         if (TMA) {
             prefetch_tensormap(&key_map);
@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
     // stays away, and what it has been given by then is right
     auto wait = [&](uint64_t* b, uint32_t parity) {
         if (warp_wait(b, parity, abort_flag, p.wait_cycles)) return true;
+        bar.abort_flag = 1;
         tell_other_block(&bar.abort_flag);
         return false;
     };
@@ -480,6 +481,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                             key_mask[meta * 4] = there;          // one bit per unit: not missing
                             mbar_arrive(&bar.keys_full[meta]);
                             arrive_expect(full, S::kSlot);
+                            *reinterpret_cast<volatile int*>(&bar.walked) = t;
                         }
                         __syncwarp();
                         const int u = lane / groups, g = lane % groups;
@@ -579,13 +581,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
             // its own: here those rows are zeroed, which can hold anything (0 * infinity is no zero), and the slot is announced.
             if (TMA) {
                 uint32_t landed = 0;                     // per slot: parity of its next such copy
+                // From one such tile to the next may be an item's whole time: the limit counts from the producers' last tile
+                auto wait_long = [&](uint64_t* b, uint32_t parity) {
+                    while (true) {
+                        const int walked = __shfl_sync(kFull, *reinterpret_cast<volatile int*>(&bar.walked), 0);
+                        if (warp_wait(b, parity, abort_flag, p.wait_cycles)) return true;
+                        if (__any_sync(kFull, *abort_flag != 0 || *reinterpret_cast<volatile int*>(&bar.walked) == walked)) return wait(b, parity);
+                    }
+                };
                 for (int t = 0; t < tiles; ++t) {
                     const bool ends = c.k + 1 >= c.span.count;
                     if (edge_tile(p, c)) {
                         // order of the loads: K(0), then [K(t + 1), V(t)], but [V(t), K(t + 1)] where t ends an item and there is one query buffer
                         const int slot = ((S::kQueries == 1 && ends) || t + 1 == tiles ? 2 * t + 1 : 2 * t + 2) % kSlots, key0 = c.key0(), lo = window_start(p, c.pos0);
                         const uint32_t base = ring + slot * S::kSlot;
-                        if (!wait(&bar.landed[slot], (landed >> slot) & 1)) break;
+                        if (!wait_long(&bar.landed[slot], (landed >> slot) & 1)) break;
                         landed ^= 1u << slot;
                         for (int r = lane; r < kTileKeys; r += 32) {
                             const int j = key0 + r;

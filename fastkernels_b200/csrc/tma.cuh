@@ -72,16 +72,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
 }
 
 // A whole warp waits, without the back-off: for warps whose next step is what everything waits for.  The answer is the same in all lanes;
-// false when the limit (clocks, below 2^32) ran out, here or in another warp of the block (*abort_flag).  A warp that gets it issues
-// nothing more.  Few registers on purpose: it is inlined where 64 scores are live.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, uint32_t limit) {
+// false when the limit (clocks, below 2^32) ran out, or another warp of the block gave up (*abort_flag, which the caller sets).  A warp that
+// gives up issues nothing more.  Few registers on purpose: it is inlined where 64 scores are live.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, const volatile int* abort_flag, uint32_t limit) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     const uint32_t t0 = (uint32_t)clock();
     do {
-        if (__any_sync(0xffffffffu, *abort_flag != 0 || (uint32_t)clock() - t0 >= limit)) {
-            *abort_flag = 1;
-            return false;
-        }
+        if (__any_sync(0xffffffffu, *abort_flag != 0 || (uint32_t)clock() - t0 >= limit)) return false;
     } while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)));
     return true;
 }

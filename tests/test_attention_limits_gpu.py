@@ -5,6 +5,7 @@ right again."""
 import pytest
 import torch
 
+import fastkernels_b200 as fk
 from fastkernels_b200 import _lib
 from tests.test_kv_cache_gpu import BF, E4, F16, Batch
 
@@ -29,3 +30,29 @@ def test_rows_of_a_wait_that_ran_out_are_nan_and_no_other_number_is_wrong(new, d
     if max(new) > 1:                                 # a decode warp's copies may land while its queries are loaded: then it has nothing to wait for
         assert lost.any()
     assert torch.equal(b.attend(max_query=max(new)), want)
+
+
+@pytest.mark.parametrize("dim,dtype,cache,page", [(256, BF, BF, 16), (128, F16, F16, 12), (256, BF, E4, 16), (64, BF, BF, 64)])
+def test_a_limit_below_the_time_of_a_call_stops_nothing_that_moves(dim, dtype, cache, page):
+    """100000 clocks, some 50 us, where an item alone takes hundreds: waits that last from one edge of the mask to the next count from
+    what moved last."""
+    lib = _lib.load()
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    pages = -(-40000 // page)
+    k, v = (torch.randn(pages, 1, page, dim, generator=g, device="cuda").to(cache) for _ in range(2))
+    scales = {} if cache != E4 else {name: torch.ones(pages, 1, page, device="cuda") for name in ("key_scale", "value_scale")}
+    q = torch.randn(1500, 8, dim, generator=g, device="cuda").to(dtype)
+    where = (torch.randperm(pages, generator=g, device="cuda").to(torch.int32).view(1, -1), torch.tensor([40000], dtype=torch.int32, device="cuda"),
+             torch.tensor([0, 1500], dtype=torch.int32, device="cuda"))
+
+    def call():
+        return fk.paged_attention(q, k, v, *where, max_query=1500, **scales)
+    want = call()
+    torch.cuda.synchronize()
+    try:
+        assert lib.fk_set_wait_limit_cycles(100000) == 0
+        got = [call() for _ in range(5)]
+        torch.cuda.synchronize()
+    finally:
+        assert lib.fk_set_wait_limit_cycles(0) == 0
+    assert torch.isfinite(want).all() and all(torch.equal(x, want) for x in got)

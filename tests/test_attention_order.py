@@ -34,10 +34,12 @@ def test_every_wait_of_a_pair_reaches_both_blocks_and_stops_what_follows():
     """Blocks of a pair depend on each other: when a wait of one gives up, the other must learn of it, nothing more may be issued or announced,
     and neither block may leave while something is on its way to it."""
     text = code("attention_tile.cu")
-    assert text.count("warp_wait(") == 1 and "mbar_wait" not in text                          # one place, which sets the flag of the other block
-    assert "tell_other_block(&bar.abort_flag);" in text.split("warp_wait(", 1)[1].split("return false;", 1)[0]
+    assert text.count("warp_wait(") == 2 and "mbar_wait" not in text                          # the place that tells the other block, and one that ends there
+    given_up = text.split("warp_wait(", 1)[1].split("return false;", 1)[0]
+    assert "bar.abort_flag = 1;" in given_up and "tell_other_block(&bar.abort_flag);" in given_up
+    assert "return wait(b, parity);" in text.split("warp_wait(", 2)[2].split("};", 1)[0]
     assert "%%cluster_ctarank" in text and "st.shared::cluster" in text.split("void tell_other_block", 1)[1].split("}\n", 1)[0]
-    waits = re.findall(r"([^\n;{}]*)\bwait\(&?b", text)
+    waits = re.findall(r"([^\n;{}]*)\bwait(?:_long)?\(&?b", text)
     assert waits and all(re.search(r"(=|!|&&|return) *\(?$", w) for w in waits)               # no answer is thrown away
     assert all("!dead()" in line for line in re.findall(r"[^\n]*arrive_first\(&bar[^\n]*", text))
     assert text.rindex("linger();") < text.rindex("cluster_sync();") < text.rindex("pair_tmem_dealloc(tmem)")
