@@ -220,19 +220,19 @@ __global__ void __launch_bounds__(kRowThreads) kv_append_kernel(const __grid_con
                 // 448 = 0.875 * 2^9: the factors are split so that nothing overflows
                 const float b = most * 0x1p-9f, inv = 1.0f / b;
                 uint32_t middle = 0xffffffffu;           // fp32 rows: steps from two below a middle between codes to the quotient next to it
-                float least = INFINITY;
+                uint32_t least = 0xffffffffu;            // twice the bits of the least magnitude but zero, less 1
 #pragma unroll
                 for (int i = 0; i < kPiece; ++i) {
                     const float x = v[i] * 0.875f, q = x * inv;
                     v[i] = fmaf(fmaf(-q, b, x), inv, q);
                     if constexpr (sizeof(T) == 4) {
                         middle = min(middle, (__float_as_uint(v[i]) - 0x7fffeu) & 0xfffffu);
-                        least = fminf(least, fabsf(v[i]));
+                        least = min(least, (__float_as_uint(v[i]) << 1) - 1u);
                     }
                 }
                 // off by two steps of 2^-23 at most.  Below 2^-6 the middles lie closer together
                 if constexpr (sizeof(T) == 4)
-                    if (middle < 5 || !(least >= 0x1p-6f) || most < 0x1p-40f) {
+                    if (middle < 5 || least < 0x78ffffffu || most < 0x1p-40f) {
                         raw[a].values(v);
                         nearest_quotients(most, v);
                     }
