@@ -2,6 +2,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include "kv_cache.cuh"
 
@@ -37,17 +38,30 @@ __device__ __forceinline__ void store_elem(__half* p, float v) { *p = __float2ha
 // subnormal elements needs no more.
 __device__ __forceinline__ int row_exponent(float most) { return most > 0.f && most < INFINITY ? max(ilogbf(most), -126) : 0; }
 
-// The sums of one row over some keys, held by a warp: lane l has the elements l, l + 32, ... of acc.
-struct RowSums {
-    float m, l;
-    float acc[FK_MAX_HEAD_DIM / 32];
+// Eight elements of a key or value row as they lie in memory: 16 bytes, 8 of codes.
+template <typename TC>
+struct Raw8 {
+    static_assert(sizeof(TC) <= 2, "rows of 16-bit elements or codes");
+    typename std::conditional<sizeof(TC) == 2, uint4, uint2>::type w;
+    __device__ __forceinline__ void load(const TC* p, bool there) {
+        w = {};
+        if (there) w = *reinterpret_cast<const decltype(w)*>(p);
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const { load8<true>(reinterpret_cast<const TC*>(&w), 8, v); }
 };
 
-// A row that is computed again (row_again): one warp, one query row (q(d) is element d times scale * log2 e, q(d >= head_dim) anything finite): groups first, first + step, ..
-// of 32 of the visible keys.  One lane computes one key's score (no reduction per key); then the value rows are added one at
-// a time, a lane per column.  Keys that are masked never enter any sum, whatever their rows hold.
-template <typename TC, bool WIDE, typename Q>
-__device__ __forceinline__ void warp_row(const AttnParams& p, const Q& q, int seq, int head, int pos, int first, int step, RowSums& r) {
+// The sums of one row over its keys, held by a warp: lane l has the elements 8 l .. 8 l + 7 of acc.
+struct RowSums {
+    float m, l;
+    float acc[8];
+};
+
+// A row that is computed again (row_again): one warp, one query row (lane l has the elements 8 l .. 8 l + 7 times scale * log2 e, zeros behind
+// head_dim), 32 of the visible keys at a time.  One lane computes one key's score (no reduction per key; the query's elements go round by
+// shuffles), then the value rows are added one at a time, eight columns per lane; four loads are in flight, which is what 64 registers
+// hold.  Keys that are masked never enter any sum, whatever their rows hold.
+template <typename TC>
+__device__ __forceinline__ void warp_row(const AttnParams& p, const float (&q)[8], int seq, int head, int pos, RowSums& r) {
     const int lane = threadIdx.x & 31, D = p.c.head_dim;
     const int end = min(pos + 1, p.c.max_pages * p.c.page_size);       // positions that the table does not hold are not visible
     const int lo = window_start(p, pos), n_sinks = max(0, min(p.sinks, min(lo, end)));
@@ -55,41 +69,36 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const Q& q, int se
     r.m = -INFINITY;
     r.l = 0.f;
 #pragma unroll
-    for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] = 0.f;
+    for (int e = 0; e < 8; ++e) r.acc[e] = 0.f;
     const TC* keys = reinterpret_cast<const TC*>(p.c.key) + head * p.c.key_stride[1];
     const TC* values = reinterpret_cast<const TC*>(p.c.value) + head * p.c.value_stride[1];
-    // where the key of this lane in the group at k0 is; looked up one group ahead of its use
-    int next_page = -1, next_row = 0;
-    auto look = [&](int64_t k0) {
-        next_page = -1;
-        const int64_t k = k0 + lane;
-        if (k < count) next_page = page_of(p.c, seq, (int)(k < n_sinks ? k : lo + k - n_sinks), next_row);
-    };
-    look((int64_t)first * 32);
-    for (int64_t k0 = (int64_t)first * 32; k0 < count; k0 += (int64_t)step * 32) {
-        const int page = next_page, in_page = next_row;
-        look(k0 + (int64_t)step * 32);
-        float s = -INFINITY, vscale = 1.f;
-        int64_t voff = 0;
-        if (page >= 0) {
-            const TC* row = keys + page * p.c.key_stride[0] + in_page * p.c.key_stride[2];
-            voff = page * p.c.value_stride[0] + in_page * p.c.value_stride[2];
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-            for (int d = 0; d < D; d += 8) {
-                float v[8];
-                load8<WIDE>(row + d, D - d, v);
+    for (int64_t k0 = 0; k0 < count; k0 += 32) {
+        int page = -1, in_page = 0;
+        if (k0 + lane < count) page = page_of(p.c, seq, (int)(k0 + lane < n_sinks ? k0 + lane : lo + k0 + lane - n_sinks), in_page);
+        if (!__any_sync(kFull, page >= 0)) continue;
+        const TC* row = keys + (page < 0 ? 0 : page * p.c.key_stride[0] + in_page * p.c.key_stride[2]);
+        const int64_t voff = page < 0 ? 0 : page * p.c.value_stride[0] + in_page * p.c.value_stride[2];
+        float s = 0.f;
+        for (int d0 = 0; d0 < D; d0 += 32) {
+            Raw8<TC> raw[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sum[i & 3] = fmaf(q(d + i), v[i], sum[i & 3]);
+            for (int i = 0; i < 4; ++i) raw[i].load(row + d0 + 8 * i, page >= 0 && d0 + 8 * i < D);
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float v[8];
+                raw[i].values(v);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum[e & 3] = fmaf(__shfl_sync(kFull, q[e], d0 / 8 + i), v[e], sum[e & 3]);
             }
-            s = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            if (sizeof(TC) == 1) {
-                s *= p.c.key_scale[row_offset(p.c.key_scale_stride, page, head, in_page)];
-                vscale = p.c.value_scale[row_offset(p.c.value_scale_stride, page, head, in_page)];
-            }
+            s += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
-        const unsigned seen = __ballot_sync(kFull, page >= 0);
-        if (seen == 0) continue;
+        float vscale = 1.f;
+        if (sizeof(TC) == 1 && page >= 0) {
+            s *= p.c.key_scale[row_offset(p.c.key_scale_stride, page, head, in_page)];
+            vscale = p.c.value_scale[row_offset(p.c.value_scale_stride, page, head, in_page)];
+        }
+        if (page < 0) s = -INFINITY;
         const float m = fmaxf(r.m, warp_max(s));
         const float base = m == -INFINITY ? 0.f : m;        // nothing but scores of -infinity so far
         const float alpha = exp2f(r.m - base);
@@ -97,25 +106,20 @@ __device__ __forceinline__ void warp_row(const AttnParams& p, const Q& q, int se
         r.m = m;
         r.l = r.l * alpha + warp_sum(w);
 #pragma unroll
-        for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] *= alpha;
+        for (int e = 0; e < 8; ++e) r.acc[e] *= alpha;
         const float weight = page >= 0 && w != 0.f ? w * vscale : 0.f;
         const unsigned adds = __ballot_sync(kFull, page >= 0 && w != 0.f);
-        constexpr int kRows = 4;                            // value rows in flight
-#pragma unroll 2
-        for (int i0 = 0; i0 < 32; i0 += kRows) {
-            float v[kRows][FK_MAX_HEAD_DIM / 32];
+        for (int i0 = 0; i0 < 32; i0 += 4) {
+            Raw8<TC> raw[4];
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const int64_t off = __shfl_sync(kFull, voff, i0 + i);
+            for (int i = 0; i < 4; ++i) raw[i].load(values + __shfl_sync(kFull, voff, i0 + i) + 8 * lane, ((adds >> (i0 + i)) & 1u) && 8 * lane < D);
 #pragma unroll
-                for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
-                    v[i][c] = ((adds >> (i0 + i)) & 1u) && c * 32 + lane < D ? load_elem(values + off + c * 32 + lane) : 0.f;
-            }
+            for (int i = 0; i < 4; ++i) {
+                const float one = __shfl_sync(kFull, weight, i0 + i);
+                float v[8];
+                raw[i].values(v);
 #pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const float wi = __shfl_sync(kFull, weight, i0 + i);
-#pragma unroll
-                for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c) r.acc[c] = fmaf(wi, v[i][c], r.acc[c]);
+                for (int e = 0; e < 8; ++e) r.acc[e] = fmaf(one, v[e], r.acc[e]);
             }
         }
     }

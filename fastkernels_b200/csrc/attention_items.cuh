@@ -265,12 +265,14 @@ __device__ __noinline__ void row_again(const AttnParams& p, int seq, int first_r
     if (p.window > 0) hidden &= ~odd_columns<TC, true>(p, seq, head, lo, min(min(window_start(p, pos1), pos + 1), all));
     if (!__any_sync(kFull, hidden != 0)) return;
     const T* query = reinterpret_cast<const T*>(p.query) + row * p.qs[0] + qh * p.qs[1];
-    RowSums r;
-    // 16 bytes (8 of codes) at a time: the kernels of tiles only take calls whose rows allow it
-    warp_row<TC, true>(p, [&](int d) { return d < D ? load_elem(query + d) * p.scale_log2 : 0.f; }, seq, head, pos, 0, 1, r);
+    float q[8];
 #pragma unroll
-    for (int c = 0; c < FK_MAX_HEAD_DIM / 32; ++c)
-        if (c * 32 + lane < D) store_elem(out + c * 32 + lane, r.l == 0.f ? 0.f : r.acc[c] / r.l);
+    for (int e = 0; e < 8; ++e) q[e] = 8 * lane + e < D ? load_elem(query + 8 * lane + e) * p.scale_log2 : 0.f;
+    RowSums r;
+    warp_row<TC>(p, q, seq, head, pos, r);       // the kernels of tiles only take calls whose rows allow its wide loads
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (8 * lane + e < D) store_elem(out + 8 * lane + e, r.l == 0.f ? 0.f : r.acc[e] / r.l);
 }
 
 // Runs of key tiles: worker w of `workers` has [w * all / workers, (w + 1) * all / workers), or `least` tiles if that is more.
