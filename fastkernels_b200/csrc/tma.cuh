@@ -2,7 +2,7 @@
 //
 // Every wait gives up after kWaitCycles, records a code in a caller-supplied error word and lets
 // the caller carry on (with wrong numbers) instead of spinning forever; after the first time-out
-// in a block all later waits of that block give up almost immediately.
+// in a block all later waits of that block give up almost immediately.  (warp_wait: the caller stops instead.)
 #pragma once
 
 #include <cuda_runtime.h>

@@ -256,7 +256,9 @@ def paged_attention(query: Any, key_cache: Any, value_cache: Any, page_table: An
     A row that sees nothing (or only scores of -infinity) gives zeros.  Rows behind the last sequence keep what `out`
     held; in a new tensor they are zero.  What masked positions hold, NaN included, has no influence on a row.
     `max_query`, the largest number of rows of one sequence if the caller knows it, only chooses between kernels.
-    Sums and softmax statistics are fp32.
+    Sums and softmax statistics are fp32.  Softmax weights are rounded once before they multiply the values: to the query's
+    16-bit type, or to fp16 beside a float8_e4m3fn cache (there times their value's scale, next to the largest such product
+    that the row sees: 11 bits down to 2^-19 of it, nothing below 2^-30); float32 queries round nothing.
     """
     call = AttentionCall()
     kv_heads, dim, seqs = _pack_cache(call, key_cache, value_cache, page_table, lengths, query_starts, key_scale, value_scale)

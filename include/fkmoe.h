@@ -309,6 +309,8 @@ typedef struct fk_attention_call {
 int fk_kv_append(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
 int fk_kv_gather(const fk_kv_cache* cache, const fk_kv_rows* rows, void* stream);
 /* out = softmax(scale * query . key) value over the positions that each row sees; a row that sees none gives zeros.
+ * Sums are fp32; weights are rounded once, to the query's 16-bit type or (FK_E4M3) to fp16, there times their value's scale next to the row's
+ * largest such product; FK_F32 queries round nothing.
  * Every wait inside the kernels is bounded (fk_set_wait_limit_cycles); one that runs out makes the rows that depended on it NaN. */
 size_t fk_paged_attention_workspace_bytes(const fk_attention_call* call);
 int fk_paged_attention(const fk_attention_call* call, void* stream);
