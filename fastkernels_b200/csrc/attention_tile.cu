@@ -807,9 +807,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) attention_tile_kernel(const _
                 m = m_new;
                 float factor = alpha;
                 if (kCodes) {
+                    const bool none = m_out == -INFINITY;                // no product but zeros so far
                     m_out = fmaxf(m_out, fmaxf(most_out, ex[512 + (half ^ 1) * 128 + r]));
                     // kept within 2^kLazy of the largest product; p 2^-k_out below stays finite
-                    if (m_out > -INFINITY && (raised || m_out - m > k_out + kLazy)) {
+                    if (m_out > -INFINITY && (raised || none || m_out - m > k_out + kLazy)) {
                         const float k = fminf(fmaxf(ceilf(m_out - m), -112.f), 112.f);
                         if (alpha != 0.f) factor = tile_exp2((raised ? fell : 0.f) + k_out - k);
                         k_out = k;

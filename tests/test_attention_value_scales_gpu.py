@@ -98,3 +98,73 @@ def test_large_values_stay_finite(dim, kv_heads, group, new):
     b = batch(dim, kv_heads, group, new, seed=4)
     b.v_scale *= 2.0 ** 115 / (448.0 * b.v_scale.max())
     b.check(b.attend(max_query=max(new)))
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,new", FORMS)
+@pytest.mark.parametrize("zero", [0.0, O.LEAST / 448.0])
+@pytest.mark.parametrize("exponent", [-20, -40, -90, 40])
+def test_values_of_any_magnitude_behind_zeros(dim, kv_heads, group, new, zero, exponent):
+    """The first two tiles of keys and a last one hold zeros, with a scale of zero or the least one; all others are small, or large."""
+    b = batch(dim, kv_heads, group, new, seed=6)
+    b.v_scale *= 2.0 ** exponent
+    for s, length in enumerate([300, 70, 200]):
+        for pos in list(range(0, min(260, length - 10))) + [length - 1]:
+            pg, rw = spot(b, s, pos)
+            b.v[pg, :, rw] = 0.0
+            b.v_scale[pg, :, rw] = zero
+    b.check(b.attend(max_query=max(new)))
+
+
+def check_on_gpu(b, got, window=0, sinks=0):
+    """`Batch.check`, its definition in 64 bits on the GPU, a sequence at a time: for batches that take the oracle minutes."""
+    group = b.q.shape[1] // b.k.shape[1]
+    for s, length in enumerate(b.lengths.tolist()):
+        a, e = int(b.starts[s]), int(b.starts[s + 1])
+        at = torch.arange(length)
+        pg, rw = b.table[s, at // b.page].long(), at % b.page
+        k, v = ((t.float()[pg, :, rw].double() * scale[pg, :, rw].double().unsqueeze(-1)).cuda().repeat_interleave(group, 1) for t, scale in ((b.k, b.k_scale), (b.v, b.v_scale)))
+        q, at, pos = b.q[a:e].cuda().double(), at.cuda(), torch.arange(length - (e - a), length, device="cuda").view(-1, 1)
+        seen = ((at <= pos) & ((at > pos - window) | (at < sinks)) if window else at <= pos).unsqueeze(1)
+        scale = q.shape[2] ** -0.5
+        w = torch.softmax((torch.einsum("rhd,jhd->rhj", q, k) * scale).masked_fill(~seen, float("-inf")), -1)
+        out, mag = torch.einsum("rhj,jhd->rhd", w, v), torch.einsum("rhj,jhd->rhd", w, v.abs())
+        size = (torch.einsum("rhd,jhd->rhj", q.abs(), k.abs()) * scale).masked_fill(~seen, 0.0).amax(-1)
+        tol = O.bound(b.dtype, out, mag, size, seen.sum(-1).double().expand_as(size), q.shape[2])
+        err = (got[a:e].double() - out).abs()
+        assert torch.isfinite(got[a:e]).all() and (err <= tol).all(), f"sequence {s}: {(err / tol).max():.2f} times the bound"
+
+
+# several key tiles of one item in a row on every pair of SMs: what a row carries from tile to tile is used
+RUNS = [(128, 8, 4, 12, 40), (256, 4, 8, 24, 20)]
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,seqs,tokens", RUNS)
+@pytest.mark.parametrize("case", ["zeros", "least", "small after large", "large of no weight", "large that loses its weight", "large of a later token", "all magnitudes"])
+def test_magnitudes_over_many_tiles(dim, kv_heads, group, seqs, tokens, case):
+    length = 520
+    b = Batch(7, [tokens] * seqs, [length] * seqs, kv_heads=kv_heads, heads=kv_heads * group, dim=dim, dtype=BF, cache=E4)
+    b.q[:, :, 0] = 16.0
+    g = torch.Generator().manual_seed(8)
+    if case in ("zeros", "least"):
+        b.v_scale *= 2.0 ** -45
+    if case == "all magnitudes":
+        b.v_scale *= torch.exp2(40 * (torch.rand(b.v_scale.shape, generator=g) - 0.5))
+    for s in range(seqs):
+        for pos in range(length):
+            pg, rw = spot(b, s, pos)
+            if case in ("zeros", "least") and pos < 270:
+                b.v[pg, :, rw] = 0.0
+                b.v_scale[pg, :, rw] = 0.0 if case == "zeros" else O.LEAST / 448.0
+            if case == "small after large" and pos >= 150:
+                b.v_scale[pg, :, rw] *= 2.0 ** -12
+            if case == "large of no weight" and pos % 100 == 30:
+                set_key(b, pg, rw, -30.0 * (dim / 128) ** 0.5)
+                b.v_scale[pg, :, rw] *= 2.0 ** 45
+            if case == "large that loses its weight" and pos == 3:
+                b.v_scale[pg, :, rw] *= 2.0 ** 45
+            if case == "large that loses its weight" and pos >= 200 and pos % 7 == 0:
+                set_key(b, pg, rw, 30.0 * (dim / 128) ** 0.5)
+            if case == "large of a later token" and pos == length - 1:
+                b.v_scale[pg, :, rw] *= 2.0 ** 45
+    check_on_gpu(b, b.attend(max_query=tokens))
+    check_on_gpu(b, b.attend(max_query=tokens, window=300, sinks=5), 300, 5)
