@@ -83,3 +83,41 @@ def test_an_early_value_that_is_not_finite_costs_no_second_pass(bad, cache):
     assert not torch.isfinite(got[:512]).any() and torch.equal(got[512:], clean[512:])
     # the rows of a pass over 16384 keys by one warp each, eight to a warp, would take tens of milliseconds
     assert after <= 2 * before + 1.0, (before, after)
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,dtype,cache,page,new,length", [(128, 8, 4, F16, F16, 32, [40] * 16, 520), (256, 4, 8, BF, BF, 16, [20] * 32, 400), (128, 8, 4, BF, E4, 16, [70, 1, 40] * 8, 520),
+                                                                            (128, 8, 4, F16, F16, 12, [70, 1, 40] * 8, 520), (128, 8, 4, BF, BF, 16, [3] * 64, 700)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 2), (9, 0)])
+def test_items_of_several_tiles_in_a_row(dim, kv_heads, group, dtype, cache, page, new, length, window, sinks):
+    """Whole items among what a pair of SMs (or a warp) walks, next to items in parts: expected infinities and NaN are counted, the rest is
+    the definition in 64 bits without them."""
+    b = Batch(dim + len(new), new, [length] * len(new), kv_heads=kv_heads, heads=kv_heads * group, dim=dim, dtype=dtype, cache=cache, page=page)
+    for s, n in enumerate(new):
+        for pos, column, bad in [(length - 1, 3, NAN), (length - 1, 5, INF), (length - n - 8, 5, -INF), (length - n // 2 - 1, 7, INF), (length - 30, 9, NAN), (0, 3, INF), (1, 11, -INF), (200, 13, NAN)]:
+            if s % 3 or bad == bad:
+                pg, rw = spot(b, s, pos)
+                b.v[pg, s % kv_heads, rw, column] = NAN if cache == E4 else bad
+    got = b.attend(max_query=max(new), window=window, sinks=sinks)
+    clean = 0
+    for s, n in enumerate(new):
+        a, at = int(b.starts[s]), torch.arange(length)
+        pg, rw = b.table[s, at // page].long(), at % page
+        k, v = b.k.float()[pg, :, rw].double(), b.v.float()[pg, :, rw].double()
+        if cache == E4:
+            k, v = k * b.k_scale[pg, :, rw].double().unsqueeze(-1), v * b.v_scale[pg, :, rw].double().unsqueeze(-1)
+        q, k, v, at = b.q[a:a + n].cuda().double(), k.cuda().repeat_interleave(group, 1), v.cuda().repeat_interleave(group, 1), at.cuda()
+        pos = torch.arange(length - n, length, device="cuda").view(-1, 1)
+        seen = (at <= pos) & ((at > pos - window) | (at < sinks)) if window else at <= pos
+        nans, ups, downs = (torch.einsum("rj,jhd->rhd", seen.double(), x.double()) > 0 for x in (v.isnan(), v == INF, v == -INF))
+        nans = nans | (ups & downs)
+        flat = v.nan_to_num(0.0, 0.0, 0.0)
+        w = torch.softmax((torch.einsum("rhd,jhd->rhj", q, k) * dim ** -0.5).masked_fill(~seen.unsqueeze(1), -INF), -1)
+        out, mag = torch.einsum("rhj,jhd->rhd", w, flat), torch.einsum("rhj,jhd->rhd", w, flat.abs())
+        size = (torch.einsum("rhd,jhd->rhj", q.abs(), k.abs()) * dim ** -0.5).masked_fill(~seen.unsqueeze(1), 0.0).amax(-1)
+        mine = got[a:a + n].double()
+        assert torch.equal(mine.isnan(), nans) and torch.equal(mine == INF, ups & ~nans) and torch.equal(mine == -INF, downs & ~nans)
+        fine = ~(nans | ups | downs)
+        tol = O.bound(dtype, out, mag, size, seen.sum(-1).double().view(-1, 1).expand_as(size), dim)
+        assert ((mine - out).abs()[fine] <= tol[fine]).all()
+        clean += int((~fine).sum() == 0)
+    assert clean < len(new)
