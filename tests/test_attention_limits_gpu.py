@@ -56,3 +56,26 @@ def test_a_limit_below_the_time_of_a_call_stops_nothing_that_moves(dim, dtype, c
     finally:
         assert lib.fk_set_wait_limit_cycles(0) == 0
     assert torch.isfinite(want).all() and all(torch.equal(x, want) for x in got)
+
+
+@pytest.mark.parametrize("limit", [50, 400, 1000, 2000])
+@pytest.mark.parametrize("dim,kv_heads,group,dtype,cache,page,new", [(256, 2, 8, BF, BF, 16, [700, 1, 300]), (128, 8, 4, F16, F16, 32, [300, 1, 200]), (128, 8, 4, F16, F16, 12, [300, 1, 200]),
+                                                                     (128, 8, 4, BF, E4, 16, [300, 1, 200]), (256, 2, 8, BF, BF, 16, [1] * 40), (128, 8, 4, BF, E4, 16, [2] * 20)])
+def test_waits_that_run_out_somewhere_on_the_way(dim, kv_heads, group, dtype, cache, page, new, limit):
+    """Limits about as long as the waits: some warps give up in the middle of their run.  What is a number is the right one."""
+    lib = _lib.load()
+    g = torch.Generator().manual_seed(limit)
+    lengths = [max(n, int(x)) for n, x in zip(new, torch.randint(700, 3000, (len(new),), generator=g))]
+    b = Batch(dim + page, new, lengths, kv_heads=kv_heads, heads=kv_heads * group, dim=dim, page=page, dtype=dtype, cache=cache)
+    args = (b.q.cuda(), *b.dev())
+    want = fk.paged_attention(*args, max_query=max(new), **b.scales)
+    torch.cuda.synchronize()
+    try:
+        assert lib.fk_set_wait_limit_cycles(limit) == 0
+        got = [fk.paged_attention(*args, max_query=max(new), **b.scales) for _ in range(4)]
+        torch.cuda.synchronize()
+    finally:
+        assert lib.fk_set_wait_limit_cycles(0) == 0
+    for x in got:
+        assert torch.equal(torch.where(torch.isnan(x), want, x), want)
+    assert torch.equal(fk.paged_attention(*args, max_query=max(new), **b.scales), want)
