@@ -100,7 +100,7 @@ struct FewShape {
     static constexpr bool kCodes = FewOps<TC>::kCodes;
     static constexpr int kPitch = D * (int)sizeof(TC);                 // bytes of a row
     // Keys of a group: 32 where rows are short, so that what a group costs beside its bytes (waits, maxima, page numbers) is spread over more
-    // of them (128 dimensions in 8 bits, 128 x 8000: 16 keys 335 us where 32 took 233; 241 to 251 on other machines)
+    // of them (128 dimensions in 8 bits, 128 x 8000: 16 keys 335 us where 32 took 233; 241 to 256 on other machines)
     static constexpr int kTiles = kPitch <= 128 ? 2 : 1, kKeys = 16 * kTiles;
     static constexpr uint32_t kAllRows = 0xffffffffu >> (32 - kKeys);
     static constexpr int kSlot = kKeys * kPitch;
